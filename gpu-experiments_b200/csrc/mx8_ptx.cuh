@@ -266,6 +266,13 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
          | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// Instruction descriptor for kind::f8f6f4 with E4M3 A and B (K-major, no scales) and an fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+    return (1u << 4)                                 // D format f32; A and B format E4M3 are zero fields
+         | (static_cast<uint32_t>(N >> 3) << 17)
+         | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
 // The same descriptors split into 32-bit halves: the high word is a constant, the low word carries
 // the address field, so advancing to another stage or K offset is one 32-bit add.
 constexpr uint32_t DESC_SW128_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -318,6 +325,24 @@ __device__ __forceinline__ void tc_mma_bf16_lo(uint32_t d, uint32_t a_lo, uint32
             "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.u32 p, %4, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
             ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(ACC == 2 ? acc : static_cast<uint32_t>(ACC)), "n"(DESC_SW128_HI)
+            : "memory");
+}
+// E4M3 x E4M3 -> f32 without scales (kind::f8f6f4), K = 32 per instruction; ACC as above
+template <int CG, int ACC>
+__device__ __forceinline__ void tc_mma_e4m3_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+            ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(static_cast<uint32_t>(ACC)), "n"(DESC_SW128_HI)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+            ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(static_cast<uint32_t>(ACC)), "n"(DESC_SW128_HI)
             : "memory");
 }
 template <int CG>

@@ -1,0 +1,670 @@
+// Router of the MoE layer: softmax over the experts, top-k, per-expert counts and the balance loss, their gradient, and the
+// gradient of the routing weights.
+//
+// forward   p = softmax(l) in fp32; S_t = the k largest logits of token t, ties to the lower expert; w = p over S_t, divided by its
+//           sum when `normalize`; c_e = chosen (token, slot) pairs of expert e; P_e = sum_t p_te; V = tokens that take part;
+//           L = E / (k V^2) * sum_e c_e P_e.  An expert whose logit is -inf is switched off; a token without a live expert, or with
+//           its mask byte 0, takes no part (ids -1, weights 0, lse -inf).
+// backward  normalised  dl = w (dw - sum_S w dw) on S;  otherwise  dl = p ([in S] dw - sum_S w dw);
+//           both + p (b - sum_e b p), b_e = dL E c_e / (k V^2).
+//
+// One warp owns a token; lane l holds experts l*VPL .. l*VPL + VPL - 1, so lane order is expert order and a ballot breaks ties.
+// Sums over tokens are made in a fixed order (registers of a warp, then warps of a block, then blocks), never with floating-point
+// atomics: results do not change from run to run.
+#include <atomic>
+
+#include "mx8_host.cuh"
+#include "mx8_ptx.cuh"
+
+namespace mx8 {
+namespace router {
+
+constexpr int MAX_EXPERTS = 1024;
+constexpr int MAX_TOPK = 32;              // one lane per choice
+
+struct FwdParams {
+    const void* logits;
+    long long ld;                         // elements between rows
+    int vec;                              // rows may be read in whole-lane vectors
+    int tokens, experts, topk, normalize;
+    const uint8_t* mask;                  // nullptr: all tokens take part
+    int* idx;
+    float* weights;
+    float* lse;
+    int* counts;
+    float* prob_sum;
+    int* num_valid;
+    float* loss;
+    float* part_prob;                     // [blocks][experts]
+    int* part_count;                      // [blocks][experts]
+    int* part_valid;                      // [blocks]
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
+
+// lane's VPL consecutive logits; experts beyond the row's end read as -inf
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, float (&v)[VPL]) {
+    const int e0 = lane * VPL;
+    constexpr int BYTES = VPL * static_cast<int>(sizeof(T));
+    if (BYTES >= 4 && vec) {              // VPL divides the row length: a lane is whole or empty
+        if (e0 < experts) {
+            constexpr int W = BYTES >= 16 ? 4 : (BYTES / 4 > 0 ? BYTES / 4 : 1);      // words per load
+            uint32_t w[BYTES >= 4 ? BYTES / 4 : 1];
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(row + e0);
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; i += W) {
+                if constexpr (W == 4) {
+                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + 4 * i));
+                    w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+                } else if constexpr (W == 2) {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + 4 * i));
+                    w[i] = x.x; w[i + 1] = x.y;
+                } else {
+                    w[i] = __ldg(reinterpret_cast<const uint32_t*>(src + 4 * i));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+                else v[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) v[i] = -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) v[i] = e0 + i < experts ? to_float(row[e0 + i]) : -INFINITY;
+    }
+}
+
+// order-preserving key of a logit: 0 for -inf (switched off), NaN above everything, -0 equal to +0
+__device__ __forceinline__ uint32_t key_of(float v) {
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return v != v ? 0xFFFFFFFFu : (u == 0xFF800000u ? 0u : k);
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ float loss_of(double dot, int n, int experts, int topk) {
+    return n > 0 ? static_cast<float>(dot * experts / (static_cast<double>(topk) * n * n)) : 0.0f;
+}
+
+// double sum over a block in a fixed order; the result is valid in thread 0
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double s = 0;
+    if (threadIdx.x == 0)
+        for (int w = 0; w < static_cast<int>(blockDim.x + 31) / 32; ++w) s += scratch[w];
+    return s;
+}
+
+template <int VPL>
+struct Shape {
+    static constexpr int WARPS = VPL <= 8 ? 32 : 16;      // 64 registers a lane hold VPL = 8 logits and probability sums
+};
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(const FwdParams p) {
+    constexpr int WARPS = Shape<VPL>::WARPS;
+    extern __shared__ float smem[];
+    float* warp_prob = smem;                                               // [WARPS][experts]
+    int* count = reinterpret_cast<int*>(smem + WARPS * p.experts);         // [experts]
+    __shared__ int valid_sum;
+    __shared__ double scratch[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int e = threadIdx.x; e < p.experts; e += WARPS * 32) count[e] = 0;
+    if (threadIdx.x == 0) valid_sum = 0;
+    __syncthreads();
+    float prob[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) prob[i] = 0.0f;
+    int n_valid = 0;
+    for (long long t = static_cast<long long>(blockIdx.x) * WARPS + warp; t < p.tokens; t += static_cast<long long>(gridDim.x) * WARPS) {
+        uint32_t key[VPL];
+        float v[VPL];
+        const bool on = !p.mask || p.mask[t] != 0;
+        uint32_t best = 0;
+        if (on) {
+            load_row<T, VPL>(static_cast<const T*>(p.logits) + t * p.ld, lane, p.experts, p.vec != 0, v);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                key[i] = key_of(v[i]);
+                best = max(best, key[i]);
+            }
+        }
+        uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        if (top == 0) {                                    // masked, or every expert switched off
+            if (lane < p.topk) {
+                p.idx[t * p.topk + lane] = -1;
+                p.weights[t * p.topk + lane] = 0.0f;
+            }
+            if (lane == 0) p.lse[t] = -INFINITY;
+            continue;
+        }
+        const float mx = value_of(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            v[i] = expf(v[i] - mx);
+            sum += v[i];
+        }
+        sum = warp_sum(sum);
+        const float inv = 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) prob[i] += v[i] * inv;
+        ++n_valid;
+        // k rounds: the largest head, the lowest lane that has it, the lowest of its experts that has it
+        int my_idx = -1;
+        uint32_t my_key = 0;
+        for (int j = 0; j < p.topk; ++j) {
+            if (j) top = __reduce_max_sync(0xFFFFFFFFu, best);
+            if (top == 0) break;                           // fewer live experts than choices
+            const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+            int at = 0;
+            if (lane == owner) {
+                bool found = false;
+                best = 0;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) {
+                    if (!found && key[i] == top) {
+                        found = true;
+                        at = i;
+                        key[i] = 0;
+                    }
+                    best = max(best, key[i]);
+                }
+            }
+            at = __shfl_sync(0xFFFFFFFFu, at, owner);
+            if (lane == j) {
+                my_idx = owner * VPL + at;
+                my_key = top;
+            }
+        }
+        float w = my_idx >= 0 ? expf(value_of(my_key) - mx) : 0.0f;
+        const float den = p.normalize ? warp_sum(w) : sum;
+        w = my_idx >= 0 ? w / den : 0.0f;
+        if (lane < p.topk) {
+            p.idx[t * p.topk + lane] = my_idx;
+            p.weights[t * p.topk + lane] = w;
+            if (my_idx >= 0) atomicAdd(&count[my_idx], 1);
+        }
+        if (lane == 0) p.lse[t] = mx + logf(sum);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+        if (lane * VPL + i < p.experts) warp_prob[warp * p.experts + lane * VPL + i] = prob[i];
+    if (lane == 0 && n_valid) atomicAdd(&valid_sum, n_valid);
+    __syncthreads();
+    const bool last = gridDim.x == 1;
+    double dot = 0;
+    for (int e = threadIdx.x; e < p.experts; e += WARPS * 32) {
+        float s = 0.0f;
+#pragma unroll 8
+        for (int w = 0; w < WARPS; ++w) s += warp_prob[w * p.experts + e];
+        const int c = count[e];
+        if (last) {
+            p.counts[e] = c;
+            p.prob_sum[e] = s;
+            dot += static_cast<double>(c) * s;
+        } else {
+            p.part_prob[static_cast<size_t>(blockIdx.x) * p.experts + e] = s;
+            p.part_count[static_cast<size_t>(blockIdx.x) * p.experts + e] = c;
+        }
+    }
+    if (last) {
+        dot = block_sum(dot, scratch);
+        if (threadIdx.x == 0) {
+            *p.num_valid = valid_sum;
+            *p.loss = loss_of(dot, valid_sum, p.experts, p.topk);
+        }
+    } else if (threadIdx.x == 0) {
+        p.part_valid[blockIdx.x] = valid_sum;
+    }
+}
+
+// Sums the blocks' partial counts and probabilities and makes the loss; one block.
+__global__ void __launch_bounds__(1024) router_finish_kernel(const FwdParams p, int blocks) {
+    __shared__ double scratch[32];
+    __shared__ double sum_p[1024];
+    __shared__ int sum_c[1024];
+    // thread (slice, e): with fewer than 1024 experts several slices of the blocks are summed side by side
+    const int slices = 1024 / p.experts;                   // >= 1
+    const int e = threadIdx.x % p.experts, slice = threadIdx.x / p.experts;
+    double s = 0;
+    int c = 0;
+    if (slice < slices) {
+        for (int b = slice; b < blocks; b += slices) {
+            s += p.part_prob[static_cast<size_t>(b) * p.experts + e];
+            c += p.part_count[static_cast<size_t>(b) * p.experts + e];
+        }
+        sum_p[threadIdx.x] = s;
+        sum_c[threadIdx.x] = c;
+    }
+    int n = 0;
+    if (threadIdx.x < 32) {
+        for (int b = threadIdx.x; b < blocks; b += 32) n += p.part_valid[b];
+        n = __reduce_add_sync(0xFFFFFFFFu, n);
+    }
+    __syncthreads();
+    double dot = 0;
+    if (threadIdx.x < p.experts) {
+        s = 0;
+        c = 0;
+        for (int i = 0; i < slices; ++i) {
+            s += sum_p[i * p.experts + threadIdx.x];
+            c += sum_c[i * p.experts + threadIdx.x];
+        }
+        p.counts[threadIdx.x] = c;
+        p.prob_sum[threadIdx.x] = static_cast<float>(s);
+        dot = s * c;
+    }
+    dot = block_sum(dot, scratch);
+    if (threadIdx.x == 0) {
+        *p.num_valid = n;
+        *p.loss = loss_of(dot, n, p.experts, p.topk);
+    }
+}
+
+struct BwdParams {
+    const void* logits;
+    long long ld;
+    int vec;
+    int tokens, experts, topk, normalize;
+    const int* idx;
+    const float* weights;
+    const float* lse;
+    const int* counts;
+    const int* num_valid;
+    const float* d_weights;               // nullptr: zero
+    const float* d_loss;                  // nullptr: zero
+    void* d_logits;                       // [tokens][experts], contiguous
+    int vec_out;
+};
+
+constexpr int BWD_WARPS = 8;
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(BWD_WARPS * 32) router_bwd_kernel(const BwdParams p) {
+    extern __shared__ float smem[];                        // per warp: a row of gradients at the chosen experts, zero elsewhere
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* row = smem + warp * (32 * VPL);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) row[lane + 32 * i] = 0.0f;
+    __syncwarp();
+    float b[VPL];
+    {
+        const int n = *p.num_valid;
+        const float g = p.d_loss ? *p.d_loss : 0.0f;
+        const float f = n > 0 ? g * static_cast<float>(static_cast<double>(p.experts) / (static_cast<double>(p.topk) * n * n)) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) b[i] = p.d_loss && lane * VPL + i < p.experts ? f * static_cast<float>(p.counts[lane * VPL + i]) : 0.0f;
+    }
+    for (long long t = static_cast<long long>(blockIdx.x) * BWD_WARPS + warp; t < p.tokens; t += static_cast<long long>(gridDim.x) * BWD_WARPS) {
+        T* out = static_cast<T*>(p.d_logits) + t * p.experts;
+        const float lse = p.lse[t];
+        float v[VPL];
+        if (lse == -INFINITY) {                            // took no part
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) v[i] = 0.0f;
+        } else {
+            load_row<T, VPL>(static_cast<const T*>(p.logits) + t * p.ld, lane, p.experts, p.vec != 0, v);
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                v[i] = expf(v[i] - lse);
+                dot += v[i] * b[i];
+            }
+            int idx = -1;
+            float wdw = 0.0f, w = 0.0f, dw = 0.0f;
+            if (p.d_weights && lane < p.topk) {
+                idx = p.idx[t * p.topk + lane];
+                if (idx >= 0 && idx < p.experts) {
+                    w = p.weights[t * p.topk + lane];
+                    dw = p.d_weights[t * p.topk + lane];
+                    wdw = w * dw;
+                } else {
+                    idx = -1;
+                }
+            }
+            dot = warp_sum(dot);
+            float inner = 0.0f;
+            if (p.d_weights) {
+                const float s = warp_sum(wdw);
+                if (p.normalize) inner = w * (dw - s);
+                else {
+                    inner = wdw;
+                    dot += s;
+                }
+                if (idx >= 0) atomicAdd(&row[idx], inner);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) v[i] = v[i] * (b[i] - dot) + (p.d_weights ? row[lane * VPL + i] : 0.0f);
+            if (p.d_weights) {
+                __syncwarp();
+                if (idx >= 0) row[idx] = 0.0f;
+                __syncwarp();
+            }
+        }
+        const int e0 = lane * VPL;
+        constexpr int BYTES = VPL * static_cast<int>(sizeof(T));
+        if (BYTES >= 4 && p.vec_out) {
+            if (e0 < p.experts) {
+                uint32_t o[BYTES >= 4 ? BYTES / 4 : 1];
+#pragma unroll
+                for (int i = 0; i < BYTES / 4; ++i) {
+                    if constexpr (sizeof(T) == 4) o[i] = __float_as_uint(v[i]);
+                    else o[i] = pack_bf16x2(v[(2 * i) % VPL], v[(2 * i + 1) % VPL]);
+                }
+                if constexpr (BYTES >= 16) {
+#pragma unroll
+                    for (int i = 0; i < BYTES / 4; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + e0) + 4 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else if constexpr (BYTES == 8) {
+                    *reinterpret_cast<uint2*>(out + e0) = make_uint2(o[0], o[1]);
+                } else if constexpr (BYTES == 4) {
+                    *reinterpret_cast<uint32_t*>(out + e0) = o[0];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                if (e0 + i < p.experts) {
+                    if constexpr (sizeof(T) == 4) out[e0 + i] = v[i];
+                    else out[e0 + i] = static_cast<uint16_t>(pack_bf16x2(v[i], 0.0f));
+                }
+            }
+        }
+    }
+}
+
+// dw[t][j] = sum_h d_output[t][h] * combine[t*topk + j][h]: every byte of combine is used once, so the kernel is bound by reading
+// it.  One block of four warps owns a token and eight of its choices: a thread holds 8 columns of d_output and has the eight rows'
+// loads (16 bytes each) in flight together; fp32 sums, combined over the lanes and warps in a fixed order.
+constexpr int WG_THREADS = 128;
+constexpr int WG_K = 8;
+
+template <bool VEC>
+__global__ void __launch_bounds__(WG_THREADS) topk_weights_grad_kernel(const uint16_t* __restrict__ d_out, const uint16_t* __restrict__ combine,
+                                                                       const int* __restrict__ idx, float* __restrict__ dw, int hidden, int topk) {
+    const long long t = blockIdx.x;
+    const int j0 = blockIdx.y * WG_K;
+    const int nj = min(WG_K, topk - j0);
+    const uint16_t* g = d_out + t * hidden;
+    const uint16_t* rows = combine + (t * topk + j0) * hidden;
+    float acc[WG_K];
+    bool live[WG_K];
+#pragma unroll
+    for (int j = 0; j < WG_K; ++j) {
+        acc[j] = 0.0f;
+        live[j] = j < nj && (!idx || idx[t * topk + j0 + j] >= 0);         // a row that was never sent is not read
+    }
+    if constexpr (VEC) {
+        for (int h = threadIdx.x * 8; h < hidden; h += WG_THREADS * 8) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(g + h));
+            uint4 r[WG_K];
+#pragma unroll
+            for (int j = 0; j < WG_K; ++j)
+                if (live[j]) r[j] = __ldg(reinterpret_cast<const uint4*>(rows + static_cast<size_t>(j) * hidden + h));
+            const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < WG_K; ++j) {
+                if (!live[j]) continue;
+                const uint32_t rw[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[j] = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(rw[i] << 16), acc[j]);
+                    acc[j] = fmaf(__uint_as_float(aw[i] & 0xFFFF0000u), __uint_as_float(rw[i] & 0xFFFF0000u), acc[j]);
+                }
+            }
+        }
+    } else {
+        for (int h = threadIdx.x; h < hidden; h += WG_THREADS) {
+            const float a = to_float(g[h]);
+#pragma unroll
+            for (int j = 0; j < WG_K; ++j)
+                if (live[j]) acc[j] = fmaf(a, to_float(rows[static_cast<size_t>(j) * hidden + h]), acc[j]);
+        }
+    }
+    __shared__ float part[WG_THREADS / 32][WG_K];
+#pragma unroll
+    for (int j = 0; j < WG_K; ++j) acc[j] = warp_sum(acc[j]);
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int j = 0; j < WG_K; ++j) part[threadIdx.x >> 5][j] = acc[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < nj) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WG_THREADS / 32; ++w) s += part[w][threadIdx.x];
+        dw[t * topk + j0 + threadIdx.x] = s;
+    }
+}
+
+static int vpl_of(int experts) {
+    int v = 1;
+    while (v * 32 < experts) v *= 2;
+    return v;
+}
+
+// a row can be read in one vector per lane: whole lanes, and every lane's first element on the vector's boundary
+static int vec_ok(const void* base, long long ld, int experts, int vpl, int esize) {
+    const int chunk = vpl * esize >= 16 ? 16 : vpl * esize;
+    return chunk >= 4 && experts % vpl == 0 && reinterpret_cast<uintptr_t>(base) % chunk == 0 && (ld * esize) % chunk == 0;
+}
+
+static int grid_of(int tokens, int warps) {
+    // one block per multiprocessor; up to two rounds of one block stay a single launch, which then finishes the sums itself
+    const int need = (tokens + warps - 1) / warps;
+    return need <= 2 ? 1 : (need < sm_count() ? need : sm_count());
+}
+
+static int warps_of(int vpl) { return vpl <= 8 ? 32 : 16; }
+
+template <typename T, int VPL>
+static cudaError_t launch_fwd(const FwdParams& p, int grid, cudaStream_t st) {
+    constexpr int WARPS = Shape<VPL>::WARPS;
+    const size_t smem = sizeof(float) * (WARPS + 1) * static_cast<size_t>(p.experts);
+    auto kern = router_fwd_kernel<T, VPL>;
+    if (smem > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+    }
+    kern<<<grid, WARPS * 32, smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T, int VPL>
+static cudaError_t launch_bwd(const BwdParams& p, cudaStream_t st) {
+    const int need = (p.tokens + BWD_WARPS - 1) / BWD_WARPS, most = sm_count() * 8;
+    router_bwd_kernel<T, VPL><<<need < most ? need : most, BWD_WARPS * 32, sizeof(float) * BWD_WARPS * 32 * VPL, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t dispatch_fwd(const FwdParams& p, int vpl, int grid, cudaStream_t st) {
+    switch (vpl) {
+        case 1: return launch_fwd<T, 1>(p, grid, st);
+        case 2: return launch_fwd<T, 2>(p, grid, st);
+        case 4: return launch_fwd<T, 4>(p, grid, st);
+        case 8: return launch_fwd<T, 8>(p, grid, st);
+        case 16: return launch_fwd<T, 16>(p, grid, st);
+        default: return launch_fwd<T, 32>(p, grid, st);
+    }
+}
+
+template <typename T>
+static cudaError_t dispatch_bwd(const BwdParams& p, int vpl, cudaStream_t st) {
+    switch (vpl) {
+        case 1: return launch_bwd<T, 1>(p, st);
+        case 2: return launch_bwd<T, 2>(p, st);
+        case 4: return launch_bwd<T, 4>(p, st);
+        case 8: return launch_bwd<T, 8>(p, st);
+        case 16: return launch_bwd<T, 16>(p, st);
+        default: return launch_bwd<T, 32>(p, st);
+    }
+}
+
+static bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+static int check_shape(const char* what, int dtype, long long ld, int tokens, int experts, int topk) {
+    if (dtype != MX8_T_BF16 && dtype != MX8_T_F32) return MX8_ERR_ARG;
+    if (tokens <= 0 || experts <= 0 || topk <= 0 || topk > experts || ld < experts) {
+        note_cuda_error(what, "tokens and experts positive, 1 <= topk <= experts, row pitch >= experts");
+        return MX8_ERR_SIZE;
+    }
+    if (experts > MAX_EXPERTS || topk > MAX_TOPK || static_cast<long long>(tokens) * topk > 0x7FFFFFFFll) {
+        note_cuda_error(what, "at most 1024 experts, 32 choices and 2^31 - 1 (token, choice) pairs");
+        return MX8_ERR_LIMIT;
+    }
+    return MX8_OK;
+}
+
+}  // namespace router
+}  // namespace mx8
+
+extern "C" size_t mx8_router_topk_workspace_bytes(int tokens, int experts) {
+    using namespace mx8;
+    if (tokens <= 0 || experts <= 0 || experts > router::MAX_EXPERTS) return 0;
+    const int sms = sm_count();
+    const int grid = sms > 0 ? router::grid_of(tokens, router::warps_of(router::vpl_of(experts))) : 0;
+    return grid > 1 ? static_cast<size_t>(grid) * (8 * static_cast<size_t>(experts) + 4) : 0;
+}
+
+extern "C" int mx8_router_topk(const void* logits, int dtype, long long ld, int tokens, int experts, int topk, int normalize,
+                               const void* token_mask, void* topk_idx, void* topk_weights, void* lse, void* counts, void* prob_sum,
+                               void* num_valid, void* balance_loss, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace mx8;
+    if (!logits || !topk_idx || !topk_weights || !lse || !counts || !prob_sum || !num_valid || !balance_loss) return MX8_ERR_ARG;
+    int rc = router::check_shape("mx8_router_topk", dtype, ld, tokens, experts, topk);
+    if (rc != MX8_OK) return rc;
+    const int vpl = router::vpl_of(experts);
+    const int grid = router::grid_of(tokens, router::warps_of(vpl));
+    const size_t need = mx8_router_topk_workspace_bytes(tokens, experts);
+    if (need > 0 && (!workspace || workspace_bytes < need)) {
+        note_cuda_error("mx8_router_topk", "workspace smaller than mx8_router_topk_workspace_bytes(tokens, experts)");
+        return MX8_ERR_LIMIT;
+    }
+    if (router::misaligned(logits, dtype == MX8_T_F32 ? 4 : 2) || router::misaligned(topk_idx, 4) || router::misaligned(topk_weights, 4) ||
+        router::misaligned(lse, 4) || router::misaligned(counts, 4) || router::misaligned(prob_sum, 4) || router::misaligned(num_valid, 4) ||
+        router::misaligned(balance_loss, 4) || router::misaligned(workspace, 4)) return MX8_ERR_ALIGN;
+    if ((rc = check_device_sm100()) != MX8_OK) return rc;
+    router::FwdParams p{};
+    p.logits = logits;
+    p.ld = ld;
+    p.vec = router::vec_ok(logits, ld, experts, vpl, dtype == MX8_T_F32 ? 4 : 2);
+    p.tokens = tokens;
+    p.experts = experts;
+    p.topk = topk;
+    p.normalize = normalize != 0;
+    p.mask = static_cast<const uint8_t*>(token_mask);
+    p.idx = static_cast<int*>(topk_idx);
+    p.weights = static_cast<float*>(topk_weights);
+    p.lse = static_cast<float*>(lse);
+    p.counts = static_cast<int*>(counts);
+    p.prob_sum = static_cast<float*>(prob_sum);
+    p.num_valid = static_cast<int*>(num_valid);
+    p.loss = static_cast<float*>(balance_loss);
+    if (grid > 1) {
+        p.part_prob = static_cast<float*>(workspace);
+        p.part_count = reinterpret_cast<int*>(p.part_prob + static_cast<size_t>(grid) * experts);
+        p.part_valid = p.part_count + static_cast<size_t>(grid) * experts;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = dtype == MX8_T_F32 ? router::dispatch_fwd<float>(p, vpl, grid, st) : router::dispatch_fwd<uint16_t>(p, vpl, grid, st);
+    if (e == cudaSuccess && grid > 1) {
+        router::router_finish_kernel<<<1, 1024, 0, st>>>(p, grid);
+        e = cudaGetLastError();
+    }
+    if (e != cudaSuccess) {
+        note_cuda_error("router launch", cudaGetErrorString(e));
+        return MX8_ERR_CUDA;
+    }
+    return MX8_OK;
+}
+
+extern "C" int mx8_router_topk_bwd(const void* logits, int dtype, long long ld, int tokens, int experts, int topk, int normalize,
+                                   const void* topk_idx, const void* topk_weights, const void* lse, const void* counts,
+                                   const void* num_valid, const void* d_topk_weights, const void* d_balance_loss, void* d_logits,
+                                   void* stream) {
+    using namespace mx8;
+    if (!logits || !topk_idx || !topk_weights || !lse || !counts || !num_valid || !d_logits) return MX8_ERR_ARG;
+    if (!d_topk_weights && !d_balance_loss) return MX8_ERR_ARG;
+    int rc = router::check_shape("mx8_router_topk_bwd", dtype, ld, tokens, experts, topk);
+    if (rc != MX8_OK) return rc;
+    if (router::misaligned(logits, dtype == MX8_T_F32 ? 4 : 2) || router::misaligned(d_logits, dtype == MX8_T_F32 ? 4 : 2) ||
+        router::misaligned(topk_idx, 4) || router::misaligned(topk_weights, 4) || router::misaligned(lse, 4) || router::misaligned(counts, 4) ||
+        router::misaligned(num_valid, 4) || router::misaligned(d_topk_weights, 4) || router::misaligned(d_balance_loss, 4)) return MX8_ERR_ALIGN;
+    if ((rc = check_device_sm100()) != MX8_OK) return rc;
+    const int vpl = router::vpl_of(experts), esize = dtype == MX8_T_F32 ? 4 : 2;
+    router::BwdParams p{};
+    p.logits = logits;
+    p.ld = ld;
+    p.vec = router::vec_ok(logits, ld, experts, vpl, esize);
+    p.tokens = tokens;
+    p.experts = experts;
+    p.topk = topk;
+    p.normalize = normalize != 0;
+    p.idx = static_cast<const int*>(topk_idx);
+    p.weights = static_cast<const float*>(topk_weights);
+    p.lse = static_cast<const float*>(lse);
+    p.counts = static_cast<const int*>(counts);
+    p.num_valid = static_cast<const int*>(num_valid);
+    p.d_weights = static_cast<const float*>(d_topk_weights);
+    p.d_loss = static_cast<const float*>(d_balance_loss);
+    p.d_logits = d_logits;
+    p.vec_out = router::vec_ok(d_logits, experts, experts, vpl, esize);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = dtype == MX8_T_F32 ? router::dispatch_bwd<float>(p, vpl, st) : router::dispatch_bwd<uint16_t>(p, vpl, st);
+    if (e != cudaSuccess) {
+        note_cuda_error("router backward launch", cudaGetErrorString(e));
+        return MX8_ERR_CUDA;
+    }
+    return MX8_OK;
+}
+
+extern "C" int mx8_moe_bwd_topk_weights(const void* d_output, const void* combine_buffer, const void* topk_idx, void* d_topk_weights,
+                                        int tokens, int hidden, int topk, void* stream) {
+    using namespace mx8;
+    if (!d_output || !combine_buffer || !d_topk_weights) return MX8_ERR_ARG;
+    if (tokens <= 0 || hidden <= 0 || topk <= 0) {
+        note_cuda_error("mx8_moe_bwd_topk_weights", "tokens, hidden and topk positive");
+        return MX8_ERR_SIZE;
+    }
+    if (router::misaligned(d_output, 2) || router::misaligned(combine_buffer, 2) || router::misaligned(topk_idx, 4) ||
+        router::misaligned(d_topk_weights, 4)) return MX8_ERR_ALIGN;
+    if (topk > 65535 * router::WG_K) {
+        note_cuda_error("mx8_moe_bwd_topk_weights", "more than 524280 choices per token");
+        return MX8_ERR_LIMIT;
+    }
+    int rc = check_device_sm100();
+    if (rc != MX8_OK) return rc;
+    const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>((topk + router::WG_K - 1) / router::WG_K));
+    const auto* g = static_cast<const uint16_t*>(d_output);
+    const auto* c = static_cast<const uint16_t*>(combine_buffer);
+    const auto* i = static_cast<const int*>(topk_idx);
+    auto* w = static_cast<float*>(d_topk_weights);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (hidden % 8 == 0 && aligned16(d_output) && aligned16(combine_buffer))
+        router::topk_weights_grad_kernel<true><<<grid, router::WG_THREADS, 0, st>>>(g, c, i, w, hidden, topk);
+    else
+        router::topk_weights_grad_kernel<false><<<grid, router::WG_THREADS, 0, st>>>(g, c, i, w, hidden, topk);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        note_cuda_error("routing-weight gradient launch", cudaGetErrorString(e));
+        return MX8_ERR_CUDA;
+    }
+    return MX8_OK;
+}

@@ -6,12 +6,14 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmx8.so")
 
-OK, ERR_ARG, ERR_SHAPE, ERR_ALIGN, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE_TIMEOUT, ERR_LIMIT = range(8)
+OK, ERR_ARG, ERR_SHAPE, ERR_ALIGN, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE_TIMEOUT, ERR_LIMIT, ERR_SIZE = range(9)
 SCALE_RCEIL, SCALE_FLOOR = 0, 1
 C_BF16, C_F32, C_MXFP8 = 0, 1, 2
+T_BF16, T_F32 = 0, 1
 
 # every symbol include/mx8.h declares, with its ctypes signature
 _vp, _i = ctypes.c_void_p, ctypes.c_int
+_ll = ctypes.c_longlong
 class Window(ctypes.Structure):
     """mx8_window: rows [*row_begin, *row_end) (device ints) on at most max_sms multiprocessors."""
     _fields_ = [("row_begin", ctypes.c_void_p), ("row_end", ctypes.c_void_p), ("max_sms", ctypes.c_int), ("own_sms", ctypes.c_int)]
@@ -97,6 +99,13 @@ SIGNATURES = {
     "mx8_gemm_a_bf16_workspace": (ctypes.c_size_t, [_i, _i]),
     "mx8_gemm_a_bf16_fused": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mx8_gemm_a_bf16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, ctypes.c_size_t, _vp]),
+    "mx8_router_topk_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "mx8_router_topk": (_i, [_vp, _i, _ll, _i, _i, _i, _i] + [_vp] * 9 + [ctypes.c_size_t, _vp]),
+    "mx8_router_topk_bwd": (_i, [_vp, _i, _ll, _i, _i, _i, _i] + [_vp] * 9),
+    "mx8_moe_bwd_topk_weights": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "mx8_quantize_block128": (_i, [_vp, _i, _i, _i, _i, _ll, _vp, _i, _vp, _ll, _vp, _vp, _ll, _vp, _i, _vp]),
+    "mx8_gemm_block128": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _vp, _ll, _i, _i, _i, _i, _vp, _i, _vp]),
+    "mx8_gemm_block128_wgrad": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _i, _i, _i, _vp, _i, _vp]),
     "mx8_probe_mma_peak": (_i, [_i, ctypes.POINTER(ctypes.c_double), _vp]),
     "mx8_selftest_bounded_wait": (_i, [ctypes.c_uint, _vp]),
     "mx8_device_status": (_i, [ctypes.POINTER(_i), _vp]),
@@ -113,7 +122,7 @@ class Mx8Error(RuntimeError):
         self.code = code
         lib = load()
         msg = lib.mx8_strerror(code).decode()
-        detail = lib.mx8_last_cuda_error().decode() if code in (ERR_CUDA, ERR_LIMIT) else ""
+        detail = lib.mx8_last_cuda_error().decode() if code in (ERR_CUDA, ERR_LIMIT, ERR_SIZE) else ""
         super().__init__(f"{where}: mx8 status {code}: {msg}" + (f" [{detail}]" if detail else ""))
 
 

@@ -42,13 +42,20 @@ enum {
     MX8_ERR_CUDA = 4,           /* a CUDA runtime / driver call failed (mx8_last_cuda_error) */
     MX8_ERR_UNSUPPORTED = 5,    /* device is not compute capability 10.x                    */
     MX8_ERR_DEVICE_TIMEOUT = 6, /* a kernel's bounded wait expired (mx8_device_status)      */
-    MX8_ERR_LIMIT = 7           /* problem exceeds a built-in size limit (mx8_last_cuda_error has the text) */
+    MX8_ERR_LIMIT = 7,          /* problem exceeds a built-in size limit (mx8_last_cuda_error has the text) */
+    MX8_ERR_SIZE = 8            /* sizes or pitches do not fit the call (mx8_last_cuda_error has the text) */
 };
 
 /* scale rounding */
 enum {
     MX8_SCALE_RCEIL = 0, /* E = ceil(log2(amax / 448)); the reference's rule                  */
     MX8_SCALE_FLOOR = 1  /* E = floor(log2(amax)) - 8; OCP rule, E4M3 saturation live         */
+};
+
+/* element type of the router's logits and of the block-128 quantizer's input */
+enum {
+    MX8_T_BF16 = 0,
+    MX8_T_F32 = 1
 };
 
 /* GEMM output element type */
@@ -245,6 +252,70 @@ MX8_API int mx8_swiglu_bf16(const void* gate, const void* up, void* hidden, long
 MX8_API int mx8_swiglu_bwd_bf16(const void* d_hidden, const void* gate, const void* up, void* d_gate, void* d_up,
                                 long long n, void* stream);
 MX8_API int mx8_transpose_bf16(const void* in, void* out, int rows, int cols, void* stream);
+
+/* Router of the MoE layer: softmax over the experts, top-k, per-expert counts and the balance loss.
+ *   logits [tokens][experts] (MX8_T_BF16 or MX8_T_F32), `ld` elements between rows; token_mask (may be NULL): one byte per token,
+ *   0 = the token takes no part and its logits are not read.
+ * p = softmax(logits) in fp32; the topk largest logits of a token are its choices, largest first, ties to the lower expert (a NaN
+ * counts as the largest value).  topk_weights = p at the choices, divided by their sum when normalize != 0.  A logit of -inf
+ * switches the expert off for that token: it is never chosen; choices that a token cannot fill have id -1 and weight 0.  A token
+ * without a live expert takes no part: ids -1, weights 0, lse -inf.  A NaN or +inf logit makes its token's weights and the sums NaN.
+ * Outputs: topk_idx int32 and topk_weights float [tokens][topk]; lse float [tokens] (log of the softmax's sum, for the backward);
+ * counts int32 [experts] (choices per expert); prob_sum float [experts] (sum of p over the tokens); num_valid int32 [1];
+ * balance_loss float [1] = experts / (topk * num_valid^2) * sum_e counts[e] * prob_sum[e], 1 when every expert gets the same share
+ * (0 when num_valid is 0).  topk_idx has the layout that mx8_moe_schedule reads, topk_weights the one of mx8_moe_fwd_epilogue.
+ * Sums over tokens are made in a fixed order.  workspace: mx8_router_topk_workspace_bytes(tokens, experts) bytes, overwritten
+ * (may be NULL when that is 0).  experts <= 1024, topk <= 32. */
+MX8_API size_t mx8_router_topk_workspace_bytes(int tokens, int experts);
+MX8_API int mx8_router_topk(const void* logits, int dtype, long long ld, int tokens, int experts, int topk, int normalize,
+                            const void* token_mask, void* topk_idx, void* topk_weights, void* lse, void* counts, void* prob_sum,
+                            void* num_valid, void* balance_loss, void* workspace, size_t workspace_bytes, void* stream);
+
+/* d_logits [tokens][experts] (type of logits, contiguous) from the gradients of topk_weights (float [tokens][topk]) and of
+ * balance_loss (float [1]); either may be NULL (zero), not both.  The other arguments are mx8_router_topk's inputs and outputs.
+ * The counts are constants, as they have no derivative.  counts and num_valid may have been summed over ranks before the call: the
+ * gradient is then that of the loss over all of them.  Tokens that took no part get zeros, and entries of d_topk_weights at
+ * choices with id -1 are not read. */
+MX8_API int mx8_router_topk_bwd(const void* logits, int dtype, long long ld, int tokens, int experts, int topk, int normalize,
+                                const void* topk_idx, const void* topk_weights, const void* lse, const void* counts,
+                                const void* num_valid, const void* d_topk_weights, const void* d_balance_loss, void* d_logits,
+                                void* stream);
+
+/* Gradient of the routing weights of mx8_moe_fwd_epilogue: d_topk_weights[t][j] = sum_h d_output[t][h] * combine_buffer[t*topk + j][h]
+ * (bf16 in, fp32 sums in a fixed order, float out).  topk_idx (int32 [tokens][topk], may be NULL): choices with a negative id get 0 and
+ * their row is not read. */
+MX8_API int mx8_moe_bwd_topk_weights(const void* d_output, const void* combine_buffer, const void* topk_idx, void* d_topk_weights,
+                                     int tokens, int hidden, int topk, void* stream);
+
+/* Block-128 format: E4M3 bytes with one fp32 scale per block of 128 (row blocks 1 x 128, or squares of 128 x 128), any M, N >= 1.
+ * scale = amax / 448 with amax the largest |x| of the block, at least 2^-110; byte = e4m3(x * (448 / amax)).
+ *   x [E][M][N] (MX8_T_BF16 or MX8_T_F32), `ldx` elements between rows (matrices M * ldx apart);
+ *   row_index (may be NULL; E == 1): int32 [M], row m is x[row_index[m]], zeros when that is outside [0, src_rows);
+ *   fp8 [E][M][.] with pitch `ld` bytes, sc:       row blocks [E][ceil(N/128)][M], squares [E][ceil(M/128)][ceil(N/128)];
+ *   fp8_t [E][N][.] with pitch `ld_t` bytes, sc_t: the transpose, row blocks [E][ceil(M/128)][N], squares the transposed scales.
+ * Pass fp8 == sc == NULL or fp8_t == sc_t == NULL to skip that orientation.  Bytes between a row's end and its pitch are left alone.
+ * An infinity or NaN makes its block dequantize to NaN. */
+MX8_API int mx8_quantize_block128(const void* x, int dtype, int E, int M, int N, long long ldx, const void* row_index, int src_rows,
+                                  void* fp8, long long ld, void* sc, void* fp8_t, long long ld_t, void* sc_t, int square, void* stream);
+
+/* C[M][N] = dequant(A) . dequant(B)^T on block-128 operands, fp32 sums.  A [M][K] with row blocks: A_sc [ceil(K/128)][M], `ldsa` floats
+ * between K blocks.  B [N][K]: squares (b_square != 0, B_sc [ceil(N/128)][ceil(K/128)]) or row blocks (B_sc [ceil(K/128)][N], pitch
+ * ldsb).  lda, ldb: bytes between rows, multiples of 16 (K need not be one); C bf16 or float, `ldc` elements between rows.  The product
+ * of two scales has to lie within the range of fp32.
+ * num_groups > 0: the rows of A are those of num_groups groups back to back, group_rows[g] of them (device int32, any size >= 0),
+ * B [num_groups][N][K] with squares [num_groups][ceil(N/128)][ceil(K/128)]; rows of C behind the last group are left alone.  Sizes
+ * that do not fit M are cut and set the device status word.  At most 256 groups. */
+MX8_API int mx8_gemm_block128(const void* A, long long lda, const void* A_sc, long long ldsa, const void* B, long long ldb,
+                              const void* B_sc, long long ldsb, int b_square, void* C, long long ldc, int M, int N, int K, int c_dtype,
+                              const void* group_rows, int num_groups, void* stream);
+
+/* Weight gradients on block-128 operands: for every group g, C_g [M][N] = dequant(A_t[:, rows_g]) . dequant(B_t[:, rows_g])^T, A_t [M][rows]
+ * and B_t [N][rows] with row blocks along `rows` (the transposed outputs of mx8_quantize_block128), rows_g the consecutive
+ * group_rows[g] columns of group g (device int32, multiples of 128; others are cut and set the device status word).  A group without
+ * rows yields zeros.  C is [num_groups][M][ldc]. */
+MX8_API int mx8_gemm_block128_wgrad(const void* A_t, long long lda, const void* A_t_sc, long long ldsa, const void* B_t, long long ldb,
+                                    const void* B_t_sc, long long ldsb, void* C, long long ldc, int M, int N, int rows, int c_dtype,
+                                    const void* group_rows, int num_groups, void* stream);
 
 /* Row windows: the MoE layer cut into minibatches of consecutive local experts, so that the transfer
  * legs (dispatch, combine) of one minibatch can run beside the GEMMs of another on a second stream.

@@ -1,0 +1,377 @@
+"""Block-128 quantizer and matrix products against plain 64-bit forms, and the MoE layer built from them and the router."""
+import pytest
+import torch
+
+import mx8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+FLOOR = 2.0 ** -110
+
+
+def cdiv(a):
+    return (a + 127) // 128
+
+
+def bits(t):
+    return t.contiguous().view(torch.uint8)
+
+
+def inverse(amax):
+    """448 / amax with one rounding (a Python number divided by a tensor is reciprocal times number: two)"""
+    return torch.full_like(amax, 448.0) / amax
+
+
+def quant_ref(x, square=False):
+    """x [M, N] on the CPU -> (bytes, scales) by the definition in fp32: the kernel has to give the same bits"""
+    M, N = x.shape
+    full = torch.zeros(cdiv(M) * 128, cdiv(N) * 128)
+    full[:M, :N] = x.float()
+    if square:
+        t = full.view(cdiv(M), 128, cdiv(N), 128)
+        amax = t.abs().amax((1, 3)).clamp(min=FLOOR)
+        q = (t * inverse(amax)[:, None, :, None]).view(full.shape)[:M, :N]
+        return q.to(torch.float8_e4m3fn), amax / 448.0
+    t = full.view(-1, cdiv(N), 128)
+    amax = t.abs().amax(2).clamp(min=FLOOR)
+    q = (t * inverse(amax)[:, :, None]).view(full.shape)[:M, :N]
+    return q.to(torch.float8_e4m3fn), (amax / 448.0)[:M].t().contiguous()
+
+
+def check_quant(x, square=False, row_index=None):
+    q, sc, qt, sct = mx8.quantize_block128(x, True, True, square=square, row_index=row_index)
+    assert mx8.device_status() == 0
+    xs = x.cpu().float()
+    if row_index is not None:
+        i = row_index.cpu().long()
+        ok = (i >= 0) & (i < xs.shape[0])
+        xs = torch.where(ok[:, None], xs[torch.where(ok, i, 0)], 0.0)
+    mats = xs if xs.dim() == 3 else xs[None]
+    lead = x.dim() == 3
+    for e in range(mats.shape[0]):
+        pick = (lambda t: t[e].cpu()) if lead else (lambda t: t.cpu())
+        for got, got_sc, ref in ((q, sc, quant_ref(mats[e], square)), (qt, sct, quant_ref(mats[e].t().contiguous(), square))):
+            assert torch.equal(pick(got_sc), ref[1])
+            assert torch.equal(bits(pick(got)), bits(ref[0]))
+            # and against x itself in 64 bits: half a step of 3 bits (2^-4), or of the smallest step 2^-9 of a block, plus the two
+            # fp32 roundings on the way
+            wide = torch.repeat_interleave(torch.repeat_interleave(ref[1].double(), 128, 0), 128, 1)[:got.shape[-2], :got.shape[-1]] if square \
+                else torch.repeat_interleave(ref[1].double().t(), 128, 1)[:, :got.shape[-1]]
+            want = mats[e].double() if got is q else mats[e].t().double()
+            assert ((pick(got).double() * wide - want).abs() <= (2.0 ** -4 + 2.0 ** -21) * want.abs() + 2.0 ** -10 * wide).all()
+    # one orientation alone gives the same
+    a = mx8.quantize_block128(x, True, False, square=square, row_index=row_index)
+    b = mx8.quantize_block128(x, False, True, square=square, row_index=row_index)
+    assert a[2] is None and a[3] is None and b[0] is None and b[1] is None
+    assert torch.equal(bits(a[0]), bits(q)) and torch.equal(a[1], sc) and torch.equal(bits(b[2]), bits(qt)) and torch.equal(b[3], sct)
+
+
+def make_x(*shape, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g)
+    x[..., 0, :] = 0.0                                            # a row of zero blocks
+    x.view(-1)[::97] *= 1000.0
+    return x.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (7, 200), (128, 128), (129, 257), (300, 1000), (513, 64), (1030, 384), (2, 130, 140), (3, 256, 128)])
+def test_quantize(shape, dtype):
+    x = make_x(*shape, seed=sum(shape), dtype=dtype)
+    check_quant(x)
+    check_quant(x, square=True)
+
+
+def test_quantize_strided_offset_and_gathered():
+    wide = make_x(300, 700, seed=1)
+    for sl in (wide[:, :500], wide[:, 3:260], wide[::2, 4:132]):
+        check_quant(sl)
+        check_quant(sl, square=True)
+    g = torch.Generator().manual_seed(2)
+    for rows in (1, 130, 500):
+        idx = torch.randint(-1, 301, (rows,), generator=g, dtype=torch.int32)       # -1 and 300 lie outside: zero rows
+        if rows > 4:
+            idx[3] = idx[2]                                                         # the same row twice
+        check_quant(wide[:, :260], row_index=idx.to(DEV))
+
+
+def test_quantize_tiny_large_and_non_finite():
+    x = torch.zeros(130, 256)
+    x[0, :128] = 2.0 ** -130                                      # below the floor of amax
+    x[1, 128:] = 3.0e38
+    x[2, 5] = 2.0 ** -149
+    check_quant(x.to(DEV))
+    for bad in (float("inf"), float("nan")):
+        y = make_x(130, 256, seed=3, dtype=torch.float32)
+        y[4, 7] = bad
+        q, sc, qt, sct = mx8.quantize_block128(y, True, True)
+        deq = q.float() * torch.repeat_interleave(sc.t(), 128, 1)
+        deqt = qt.float() * torch.repeat_interleave(sct.t(), 128, 1)[:, :130]
+        assert torch.isnan(deq[4, 7]) and torch.isnan(deqt[7, 4])
+        if bad != bad:
+            assert torch.isnan(deq[4, :128]).all() and torch.isnan(deqt[7, :128]).all()
+        assert torch.isfinite(deq[5:]).all() and torch.isfinite(deqt[8:]).all() and torch.isfinite(deq[4, 128:]).all()
+
+
+# ------------------------------------------------------------------------------------------------ products
+def rows64(q, sc):
+    return q.cpu().double() * torch.repeat_interleave(sc.cpu().double().t(), 128, 1)[:, :q.shape[1]]
+
+
+def square64(q, sc):
+    return q.cpu().double() * torch.repeat_interleave(torch.repeat_interleave(sc.cpu().double(), 128, 0)[:q.shape[0]], 128, 1)[:, :q.shape[1]]
+
+
+def check_c(c, a64, b64, what=""):
+    """Products of two E4M3 values are exact in fp32; a block of 128 of them added in fp32 in any order, or cut instead of rounded,
+    is off by at most 128 * 2^-23 of the sum of magnitudes; the scales' product and the block's scaling add two roundings and every
+    further block one (2^-24 each).  The output type adds half a step (bf16: 2^-8)."""
+    want, size = a64 @ b64.t(), a64.abs() @ b64.abs().t()
+    tol = (128 * 2.0 ** -23 + (cdiv(a64.shape[1]) + 4) * 2.0 ** -24) * size
+    if c.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    off = (c.cpu().double() - want).abs()
+    assert (off <= tol + 1e-300).all(), f"{what}: {float((off / (tol + 1e-300)).nan_to_num(nan=1e9).max()):.3g} times the bound"
+
+
+def operands(M, N, K, b, seed=0):
+    a = make_x(M, K, seed=seed)
+    w = make_x(N, K, seed=seed + 1, dtype=torch.float32) * 0.02
+    qa, sa, _, _ = mx8.quantize_block128(a)
+    qb, sb, _, _ = mx8.quantize_block128(w, square=(b == "square"))
+    return qa, sa, qb, sb, rows64(qa, sa), (square64 if b == "square" else rows64)(qb, sb)
+
+
+@pytest.mark.parametrize("b", ["square", "rows"])
+@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 128, 128), (1, 520, 1040), (3, 300, 100), (16, 256, 512), (17, 129, 272), (32, 1000, 640),
+                                   (33, 64, 130), (64, 512, 384), (65, 100, 200), (128, 128, 128), (128, 256, 256), (129, 257, 144), (200, 72, 1000),
+                                   (300, 1030, 520), (1000, 640, 1152), (2100, 2304, 200)])
+def test_product(shape, b):
+    M, N, K = shape
+    qa, sa, qb, sb, a64, b64 = operands(M, N, K, b, seed=M + N + K)
+    for dtype in (torch.bfloat16, torch.float32):
+        c = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
+        assert mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks=b) is c
+        assert mx8.device_status() == 0
+        check_c(c, a64, b64, f"{shape} {b} {dtype}")
+        again = torch.full_like(c, 7.0)
+        mx8.gemm_block128(qa, sa, qb, sb, again, b_blocks=b)
+        assert torch.equal(c, again)
+
+
+def test_product_into_and_from_slices():
+    M, N, K = 150, 200, 300
+    for m in (M, 5):
+        qa, sa, qb, sb, a64, b64 = operands(m, N, K, "square", seed=m)
+        big = torch.full((m + 2, N + 9), 3.0, dtype=torch.bfloat16, device=DEV)
+        mx8.gemm_block128(qa, sa, qb, sb, big[1:m + 1, 5:N + 5])
+        assert mx8.device_status() == 0
+        check_c(big[1:m + 1, 5:N + 5], a64, b64)
+        edge = big.clone()
+        edge[1:m + 1, 5:N + 5] = 3.0
+        assert (edge == 3.0).all()
+    # rows of A inside a larger buffer, with the larger buffer's scales
+    qa, sa, qb, sb, a64, b64 = operands(M, N, K, "rows", seed=8)
+    c = torch.empty(40, N, device=DEV)
+    mx8.gemm_block128(qa[100:140], sa[:, 100:140], qb, sb, c, b_blocks="rows")
+    check_c(c, a64[100:140], b64)
+
+
+def test_non_finite_blocks_reach_their_rows_only():
+    qa, sa, qb, sb, a64, b64 = operands(200, 300, 256, "square", seed=4)
+    sa[1, 7] = float("nan")
+    c = torch.empty(200, 300, device=DEV)
+    mx8.gemm_block128(qa, sa, qb, sb, c)
+    assert torch.isnan(c[7]).all()
+    keep = torch.arange(200) != 7
+    check_c(c[keep.to(DEV)], a64[keep], b64)
+
+
+@pytest.mark.parametrize("sizes", [[5], [0, 1, 0, 130, 7, 0], [128, 256, 1], [0, 0, 0], [300, 0, 0, 0, 0, 0, 0, 2], [1] * 40, [3] * 256])
+def test_grouped_product(sizes):
+    G, R, N, K = len(sizes), sum(sizes), 200, 272
+    if G > 100:
+        N, K = 40, 144
+    cap = R + 37
+    a = make_x(cap, K, seed=R)
+    w = make_x(G, N, K, seed=G, dtype=torch.float32) * 0.02
+    qa, sa, _, _ = mx8.quantize_block128(a)
+    qb, sb, _, _ = mx8.quantize_block128(w, square=True)
+    grp = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        c = torch.full((cap, N), 5.0, dtype=dtype, device=DEV)
+        mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=grp)
+        assert mx8.device_status() == 0
+        a64, at = rows64(qa, sa), 0
+        for g, n in enumerate(sizes):
+            if n:
+                check_c(c[at:at + n], a64[at:at + n], square64(qb[g], sb[g]), f"group {g}")
+            at += n
+        assert (c[at:] == 5.0).all()
+
+
+@pytest.mark.parametrize("sizes", [[128], [0, 256, 128, 0], [384, 0, 0, 128, 640], [128] * 9])
+@pytest.mark.parametrize("mn", [(64, 40), (200, 300), (129, 520)])
+def test_weight_gradient_product(sizes, mn):
+    G, R = len(sizes), sum(sizes)
+    M, N = mn
+    pad = 64                                                       # rows behind the last group take no part
+    y, x = make_x(R + pad, M, seed=R, dtype=torch.float32), make_x(R + pad, N, seed=R + 1)
+    _, _, qa, sa = mx8.quantize_block128(y, False, True)
+    _, _, qb, sb = mx8.quantize_block128(x, False, True)
+    grp = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        c = torch.full((G, M, N), float("nan"), dtype=dtype, device=DEV)
+        mx8.gemm_block128_wgrad(qa, sa, qb, sb, c, grp)
+        assert mx8.device_status() == 0
+        a64, b64, at = rows64(qa, sa), rows64(qb, sb), 0
+        for g, n in enumerate(sizes):
+            if n:
+                check_c(c[g], a64[:, at:at + n], b64[:, at:at + n], f"group {g}")
+            else:
+                assert (c[g] == 0).all()
+            at += n
+
+
+def test_group_sizes_that_do_not_fit_are_cut_and_reported():
+    K, N = 256, 64
+    qa, sa, _, _ = mx8.quantize_block128(make_x(100, K))
+    qb, sb, _, _ = mx8.quantize_block128(make_x(3, N, K), square=True)
+    guard = torch.full((140, N), 9.0, device=DEV)
+    for sizes in ([50, 60, 10], [-4, 20, 10], [2 ** 31 - 1] * 3):
+        mx8.gemm_block128(qa, sa, qb, sb, guard[:100], group_rows=torch.tensor(sizes, dtype=torch.int32, device=DEV))
+        with pytest.raises(mx8.Mx8Error):
+            mx8.device_status()
+        assert (guard[100:] == 9.0).all()
+        assert mx8.device_status() == 0
+    _, _, qt, st = mx8.quantize_block128(make_x(300, 64), False, True)
+    c = torch.empty(2, 64, 64, device=DEV)
+    for sizes in ([100, 128], [256, 256], [-128, 128]):
+        mx8.gemm_block128_wgrad(qt, st, qt, st, c, torch.tensor(sizes, dtype=torch.int32, device=DEV))
+        with pytest.raises(mx8.Mx8Error):
+            mx8.device_status()
+
+
+def test_refusals():
+    qa, sa, qb, sb, _, _ = operands(20, 40, 200, "square")
+    c = torch.empty(20, 40, dtype=torch.bfloat16, device=DEV)
+    g = torch.tensor([20], dtype=torch.int32, device=DEV)
+    for bad in (lambda: mx8.gemm_block128(qa, sa, qb, sb, c[:10]), lambda: mx8.gemm_block128(qa, sa, qb, sb, c.half()),
+                lambda: mx8.gemm_block128(qa, sa.t(), qb, sb, c), lambda: mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks="rows"),
+                lambda: mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks="columns"), lambda: mx8.gemm_block128(qa, sa.double(), qb, sb, c),
+                lambda: mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=g), lambda: mx8.gemm_block128(qa.cpu(), sa, qb, sb, c),
+                lambda: mx8.gemm_block128(qa, sa.cpu(), qb, sb, c), lambda: mx8.gemm_block128(qa, sa, qb[:, :100], sb, c),
+                lambda: mx8.gemm_block128(qa, sa, qb[None], sb[None], c, group_rows=g.long()),
+                lambda: mx8.gemm_block128(qa[:0], sa[:, :0], qb, sb, c[:0]),
+                lambda: mx8.quantize_block128(torch.zeros(4, 4, dtype=torch.float16, device=DEV)),
+                lambda: mx8.quantize_block128(torch.zeros(4, 8, device=DEV).t()), lambda: mx8.quantize_block128(torch.zeros(4, 8, device=DEV), False, False),
+                lambda: mx8.quantize_block128(torch.zeros(4, 8, device=DEV), square=True, row_index=g),
+                lambda: mx8.quantize_block128(torch.zeros(4, 8, device=DEV), row_index=g.long()),
+                lambda: mx8.gemm_block128_wgrad(qa, sa, qa, sa, torch.empty(2, 20, 20, device=DEV), g)):
+        with pytest.raises(ValueError):
+            bad()
+    tight = qa.contiguous()                                        # rows of 200 bytes: no 16-byte boundary
+    with pytest.raises(mx8.Mx8Error):
+        mx8.gemm_block128(tight, sa, qb, sb, c)
+
+
+def test_side_stream_and_graphs_at_once():
+    qa, sa, qb, sb, a64, b64 = operands(40, 640, 1024, "square", seed=20)
+    qc, scc, qd, sd, c64, d64 = operands(600, 640, 1024, "square", seed=21)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for ops, M in (((qa, sa, qb, sb), 40), ((qc, scc, qd, sd), 600)):
+        out = torch.zeros(M, 640, device=DEV)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            mx8.gemm_block128(*ops, out)
+        graphs.append(gr)
+        outs.append(out)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s, gr in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert mx8.device_status() == 0
+    check_c(outs[0], a64, b64)
+    check_c(outs[1], c64, d64)
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_moe_layer_forward_and_backward_from_the_router_to_the_weight_gradients():
+    """One training step of an MoE layer on one rank: router, schedule, gathered quantization, experts' products, SwiGLU, combine,
+    weighted sum; then back to the logits and the weights.  Every stage against 64 bits on the inputs it actually had."""
+    T, H, I, E, k = 300, 256, 192, 8, 2
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    wr = torch.randn(E, H, generator=g) * H ** -0.5
+    w = {n: (torch.randn(E, *s, generator=g) * 0.06).to(DEV) for n, s in (("gate", (I, H)), ("up", (I, H)), ("down", (H, I)))}
+    logits = (x.float().cpu() @ wr.t()).to(DEV)
+    mask = torch.arange(T, device=DEV) < T - 20
+    idx, wt, lse, counts, _, n, loss = mx8.router_topk(logits, k, token_mask=mask)
+    cap = (T * k // 256 + E) * 256
+    peer_rank, peer_tok, rows, per_expert = mx8.schedule(idx[None].contiguous(), E, cap, 0)
+    assert mx8.device_status() == 0
+    src = torch.where(peer_rank >= 0, peer_tok // k, -1).to(torch.int32)
+    assert int((src >= 0).sum()) == int(counts.sum()) == (T - 20) * k
+    qx, sx, qxt, sxt = mx8.quantize_block128(x, True, True, row_index=src)
+    quant = {name: mx8.quantize_block128(v, True, True, square=True) for name, v in w.items()}
+    new = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    gate = mx8.gemm_block128(qx, sx, *quant["gate"][:2], new(cap, I), group_rows=per_expert)
+    up = mx8.gemm_block128(qx, sx, *quant["up"][:2], new(cap, I), group_rows=per_expert)
+    hid = mx8.swiglu_bf16(gate, up)
+    qh, sh, qht, sht = mx8.quantize_block128(hid, True, True)
+    y = mx8.gemm_block128(qh, sh, *quant["down"][:2], new(cap, H), group_rows=per_expert)
+    buf = new(T * k, H)
+    mx8.combine(y, peer_rank, peer_tok, rows, [buf.data_ptr()], T * k)
+    out = mx8.fwd_epilogue(None, buf, wt)
+    assert mx8.device_status() == 0
+    sizes = per_expert.tolist()
+
+    def grouped(c, qa, sa, qb, sb):
+        a64, at = rows64(qa, sa), 0
+        for e, m in enumerate(sizes):
+            if m:
+                check_c(c[at:at + m], a64[at:at + m], square64(qb[e], sb[e]), f"expert {e}")
+            at += m
+
+    grouped(gate, qx, sx, *quant["gate"][:2])
+    grouped(up, qx, sx, *quant["up"][:2])
+    grouped(y, qh, sh, *quant["down"][:2])
+    want = (buf.cpu().double().view(T, k, H) * wt.cpu().double()[:, :, None]).sum(1)
+    # k products and sums in fp32, then bf16
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -22 * (buf.cpu().double().view(T, k, H).abs() * wt.cpu().double()[:, :, None]).sum(1)).all()
+    assert (out[T - 20:] == 0).all()
+
+    # ---- backward
+    d_out = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    d_wt = mx8.bwd_topk_weights(d_out, buf, idx)
+    d_loss = torch.tensor([0.01], device=DEV)
+    d_logits = mx8.router_topk_bwd(logits, idx, wt, lse, counts, n, d_wt, d_loss)
+    ref_wt = torch.where(idx.cpu() >= 0, (buf.cpu().double().view(T, k, H) * d_out.cpu().double()[:, None]).sum(2), 0.0)
+    assert ((d_wt.cpu().double() - ref_wt).abs() <= 32 * 2.0 ** -24 * (buf.cpu().double().view(T, k, H) * d_out.cpu().double()[:, None]).abs().sum(2)).all()
+    p = torch.softmax(logits.cpu().double(), 1)
+    i = idx.cpu().long().clamp(min=0)
+    ww, dd = wt.cpu().double(), d_wt.cpu().double()
+    b = 0.01 * counts.cpu().double() * E / (k * int(n) ** 2)
+    ref = torch.zeros(T, E, dtype=torch.float64).scatter_add_(1, i, ww * (dd - (ww * dd).sum(1, keepdim=True))) + p * (b - p @ b[:, None])
+    ref = torch.where(mask.cpu()[:, None], ref, 0.0)
+    assert ((d_logits.cpu().double() - ref).abs() <= 2.0 ** -16 * ((ww * dd).abs().sum(1, keepdim=True) + b.max())).all()
+
+    d_buf = new(T * k, H)
+    mx8.bwd_prologue(d_out, wt, d_buf)
+    safe = torch.where(peer_rank >= 0, peer_tok, 0).long()
+    d_y = torch.where((peer_rank >= 0)[:, None], d_buf[safe], torch.zeros((), dtype=torch.bfloat16, device=DEV))
+    qd, sd, qdt, sdt = mx8.quantize_block128(d_y, True, True)
+    d_hid = mx8.gemm_block128(qd, sd, *quant["down"][2:], new(cap, I), group_rows=per_expert)
+    grouped(d_hid, qd, sd, *quant["down"][2:])
+    d_down = mx8.gemm_block128_wgrad(qdt, sdt, qht, sht, torch.empty(E, H, I, device=DEV), per_expert)
+    a64, b64, at = rows64(qdt, sdt), rows64(qht, sht), 0
+    for e, m in enumerate(sizes):
+        if m:
+            check_c(d_down[e], a64[:, at:at + m], b64[:, at:at + m], f"expert {e} weights")
+        else:
+            assert (d_down[e] == 0).all()
+        at += m
+    assert mx8.device_status() == 0

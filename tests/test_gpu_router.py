@@ -1,0 +1,287 @@
+"""Router, balance loss, their gradient and the gradient of the routing weights against plain 64-bit forms."""
+import pytest
+import torch
+
+import mx8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+NEG = float("-inf")
+# relative error of a softmax value: the difference l - max is rounded (half a step of |l - max| < 32 is 2^-20 absolute in the
+# exponent), exp is good to two steps of 2^-23, a sum of 1024 terms in fp32 to 10 * 2^-24 (tree over 32 lanes of 32), one division:
+# 2^-20 + 2^-22 + 2^-20.6 + 2^-24 < 2^-18.5 for numerator and denominator together
+P_TOL = 2.0 ** -18
+
+
+def route_ref(logits, k, normalize, mask=None):
+    """64-bit forward on the CPU"""
+    l = logits.detach().cpu().double()
+    T, E = l.shape
+    on = (l > NEG).any(1) | torch.isnan(l).any(1)
+    if mask is not None:
+        on &= mask.cpu()
+    order = torch.sort(torch.where(torch.isnan(l), torch.inf, l), dim=1, descending=True, stable=True).indices[:, :k]
+    taken = (torch.gather(l, 1, order) != NEG) & on[:, None]
+    idx = torch.where(taken, order, -1)
+    p = torch.where(on[:, None], torch.softmax(l, 1), 0.0)
+    w = torch.where(taken, torch.gather(p, 1, order), 0.0)
+    if normalize:
+        w = torch.where(taken, w / w.sum(1, keepdim=True), 0.0)
+    counts = torch.zeros(E, dtype=torch.int64).scatter_add_(0, idx[taken], torch.ones_like(idx[taken]))
+    n = int(on.sum())
+    loss = float((counts.double() * p.sum(0)).sum() * E / (k * n * n)) if n else 0.0
+    lse = torch.where(on, torch.logsumexp(l, 1), NEG)
+    return idx, w, lse, counts, p.sum(0), n, loss
+
+
+def check_forward(logits, k, normalize, mask=None):
+    out = mx8.router_topk(logits, k, normalize=normalize, token_mask=mask)
+    assert mx8.device_status() == 0
+    idx, w, lse, counts, prob, n, loss = [t.cpu() for t in out]
+    ridx, rw, rlse, rcounts, rprob, rn, rloss = route_ref(logits, k, normalize, mask)
+    assert idx.dtype == torch.int32 and torch.equal(idx.long(), ridx)
+    assert torch.equal(counts.long(), rcounts) and int(n) == rn
+    assert torch.allclose(w.double(), rw, rtol=P_TOL, atol=2.0 ** -140)
+    live = rlse > NEG
+    assert torch.equal(lse == NEG, ~live)
+    # the logarithm adds half a step of its own and of the maximum it is added to
+    assert ((lse[live].double() - rlse[live]).abs() <= 2.0 ** -18 + 2.0 ** -23 * rlse[live].abs()).all()
+    # sums over tokens: fp32 per warp and block (at most 2^13 terms in a row, here far fewer), then 64 bits
+    tokens = max(1, logits.shape[0] // 2000 + 40)
+    assert torch.allclose(prob.double(), rprob, rtol=P_TOL + tokens * 2.0 ** -24, atol=2.0 ** -120)
+    assert abs(float(loss) - rloss) <= (P_TOL + tokens * 2.0 ** -24) * abs(rloss)
+    return out
+
+
+def make_logits(T, E, dtype, seed, ties=False):
+    g = torch.Generator().manual_seed(seed)
+    l = torch.randn(T, E, generator=g)
+    if ties:
+        l = torch.round(l * 2) / 2
+    return l.to(dtype).to(DEV)
+
+
+SHAPES = [(1, 1, 1), (1, 8, 8), (3, 60, 4), (16, 256, 8), (64, 256, 8), (65, 256, 8), (1000, 257, 6), (5003, 64, 2), (129, 1024, 32),
+          (70, 512, 1), (7, 33, 32), (2000, 128, 6), (33, 1000, 5), (300, 4, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward(shape, dtype):
+    T, E, k = shape
+    for normalize in (True, False):
+        check_forward(make_logits(T, E, dtype, T + E), k, normalize)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ties_go_to_the_lower_expert(dtype):
+    check_forward(make_logits(200, 96, dtype, 1, ties=True), 8, True)
+    flat = torch.zeros(9, 256, dtype=dtype, device=DEV)
+    flat[3, ::2] = -0.0                                       # both zeros are the same value
+    check_forward(flat, 8, True)
+
+
+def test_masks_switched_off_experts_and_lowest_values():
+    l = make_logits(200, 64, torch.float32, 2)
+    l[5] = NEG                                                 # nothing left
+    l[6, 1:] = NEG                                             # fewer than topk
+    l[7, 10:] = torch.finfo(torch.float32).min                 # a mask of the type's lowest value is a value
+    l[8] = torch.finfo(torch.float32).min
+    l[:, 11] = NEG
+    mask = torch.ones(200, dtype=torch.bool, device=DEV)
+    mask[150:] = False
+    mask[0] = False
+    for normalize in (True, False):
+        check_forward(l, 12, normalize, mask)
+    b = l.to(torch.bfloat16)
+    b[7, 10:] = torch.finfo(torch.bfloat16).min
+    check_forward(b, 4, True, mask)
+    # a batch in which no token takes part
+    out = mx8.router_topk(l, 4, token_mask=torch.zeros(200, dtype=torch.bool, device=DEV))
+    assert int(out[5]) == 0 and float(out[6]) == 0.0 and int(out[3].abs().sum()) == 0 and float(out[4].abs().sum()) == 0.0
+    assert (out[0] == -1).all() and (out[1] == 0).all() and (out[2] == NEG).all()
+
+
+def test_values_in_masked_tokens_are_not_read_and_live_nan_is_reported():
+    l = make_logits(100, 48, torch.float32, 3)
+    want = mx8.router_topk(l[:60].contiguous(), 4)
+    mask = torch.arange(100, device=DEV) < 60
+    l[60:] = float("nan")
+    l[70, 3] = float("inf")
+    got = mx8.router_topk(l, 4, token_mask=mask)
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a[:60], b)
+    assert torch.equal(got[3], want[3]) and torch.isfinite(got[4]).all() and torch.isfinite(got[6]).all()
+    # a NaN or an infinity in a live token: first choice, NaN weights, NaN loss, ids inside the range
+    for bad in (float("nan"), float("inf")):
+        x = make_logits(10, 48, torch.float32, 4)
+        x[2, 17] = bad
+        idx, w, lse, counts, prob, n, loss = mx8.router_topk(x, 4)
+        assert int(idx[2, 0]) == 17 and bool(((idx >= 0) & (idx < 48)).all()) and int(counts.sum()) == 40
+        assert torch.isnan(w[2]).all() and torch.isnan(loss).all() and torch.isfinite(w[3]).all()
+
+
+def test_strided_rows_and_offsets():
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = make_logits(130, 300, dtype, 5)
+        for sl in (wide[:, :256], wide[:, 3:259], wide[:, 1:61], wide[::2, 8:264]):
+            got = mx8.router_topk(sl, 6)
+            want = mx8.router_topk(sl.contiguous(), 6)
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+            d = torch.randn(sl.shape[0], 6, device=DEV)
+            one = torch.ones(1, device=DEV)
+            args = (got[0], got[1], got[2], got[3], got[5], d, one)
+            assert torch.equal(mx8.router_topk_bwd(sl, *args), mx8.router_topk_bwd(sl.contiguous(), *args))
+
+
+def bwd_ref(logits, idx, normalize, counts, n, k, dw, dl):
+    """64-bit gradient by automatic differentiation of the forward formula with the choices and counts held"""
+    l = logits.detach().cpu().double().requires_grad_(True)
+    T, E = l.shape
+    on = (l.detach() > NEG).any(1) & (idx >= 0).any(1)
+    safe = torch.where(on[:, None], l, torch.zeros_like(l))
+    p = torch.softmax(safe, 1) * on[:, None]
+    taken = idx >= 0
+    w = torch.where(taken, torch.gather(p, 1, idx.clamp(min=0)), 0.0)
+    if normalize:
+        w = torch.where(taken, w / torch.where(on, w.sum(1), 1.0)[:, None], 0.0)
+    total = torch.zeros((), dtype=torch.float64)
+    if dw is not None:
+        total = total + (w * torch.where(taken, dw.cpu().double(), 0.0)).sum()
+    if dl is not None:
+        total = total + float(dl) * (counts.double() * p.sum(0)).sum() * E / (k * max(n, 1) ** 2)
+    total.backward()
+    g = l.grad
+    # size of the terms that cancel: the bound of the rounding error
+    size = (w.detach().abs() * (dw.cpu().double().nan_to_num().abs() if dw is not None else 0.0)).sum(1, keepdim=True)
+    if dl is not None:
+        size = size + abs(float(dl)) * counts.double().max() * E / (k * max(n, 1) ** 2)
+    return torch.nan_to_num(g), size
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_backward(shape, dtype):
+    T, E, k = shape
+    logits = make_logits(T, E, dtype, 7 * T + E)
+    mask = torch.arange(T, device=DEV) < max(1, T - T // 5)
+    if E > 4 and T > 3:
+        logits[:, 2] = NEG
+        logits[1] = NEG
+    g = torch.Generator().manual_seed(T)
+    dw = torch.randn(T, k, generator=g).to(DEV)
+    dl = torch.tensor([3.0], device=DEV)
+    for normalize in (True, False):
+        idx, w, lse, counts, _, n, _ = mx8.router_topk(logits, k, normalize=normalize, token_mask=mask)
+        dw_in = torch.where(idx >= 0, dw, float("nan"))                  # what lies at unfilled choices is not read
+        for a, b in ((dw_in, dl), (dw_in, None), (None, dl)):
+            got = mx8.router_topk_bwd(logits, idx, w, lse, counts, n, a, b, normalize=normalize)
+            assert mx8.device_status() == 0 and got.dtype == dtype and got.shape == (T, E)
+            want, size = bwd_ref(logits, idx.cpu().long(), normalize, counts.cpu(), int(n), k, a, b)
+            # p, w and the two sums are good to P_TOL of `size`; bf16 rounds the result by half a step of 2^-7
+            tol = 4 * P_TOL * size + (2.0 ** -8 * want.abs() if dtype == torch.bfloat16 else 0.0) + 2.0 ** -120
+            assert ((got.cpu().double() - want).abs() <= tol).all()
+            assert (got.cpu()[~mask.cpu()] == 0).all()
+
+
+def test_backward_against_differences_of_the_forward():
+    # S = sum w dw + dl * loss; central differences of the kernel's own forward.  Logits are multiples of 1/4 apart, so a step of 2^-6
+    # changes no choice; |third derivative| of softmax terms is below 1 per unit of dw, so the truncation is below 2^-12 / 6 * sum|dw|,
+    # and the rounding of S (2^-18 relative) divided by 2 h = 2^-5 below 2^-13 * |S|
+    T, E, k, h = 3, 8, 3, 2.0 ** -6
+    g = torch.Generator().manual_seed(1)
+    base = torch.stack([torch.randperm(E, generator=g) for _ in range(T)]).float() / 4
+    dw, dl = torch.randn(T, k, generator=g), 0.7
+    for normalize in (True, False):
+        def value(l):
+            o = mx8.router_topk(l.to(DEV), k, normalize=normalize)
+            return float((o[1].cpu().double() * dw.double()).sum() + dl * o[6].cpu().double())
+        o = mx8.router_topk(base.to(DEV), k, normalize=normalize)
+        got = mx8.router_topk_bwd(base.to(DEV), o[0], o[1], o[2], o[3], o[5], dw.to(DEV), torch.tensor([dl], device=DEV), normalize=normalize).cpu()
+        tol = 2.0 ** -12 / 6 * float(dw.abs().sum() + 8 * dl) + 2.0 ** -13 * float(dw.abs().sum() + dl * 4)
+        for t in range(T):
+            for e in range(E):
+                hi, lo = base.clone(), base.clone()
+                hi[t, e] += h
+                lo[t, e] -= h
+                assert abs((value(hi) - value(lo)) / (2 * h) - float(got[t, e])) <= tol
+
+
+def test_counts_summed_over_ranks_give_the_gradient_of_the_joint_loss():
+    T, E, k = 120, 32, 4
+    l = make_logits(T, E, torch.float32, 9)
+    whole = mx8.router_topk(l, k)
+    parts = [mx8.router_topk(x, k) for x in (l[:50].contiguous(), l[50:].contiguous())]
+    counts, n = parts[0][3] + parts[1][3], parts[0][5] + parts[1][5]
+    assert torch.equal(counts, whole[3]) and int(n) == T
+    one = torch.ones(1, device=DEV)
+    want = mx8.router_topk_bwd(l, whole[0], whole[1], whole[2], whole[3], whole[5], None, one)
+    got = torch.cat([mx8.router_topk_bwd(x.contiguous(), o[0], o[1], o[2], counts, n, None, one) for x, o in zip((l[:50], l[50:]), parts)])
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 8), (3, 8, 128), (61, 8, 2048), (17, 9, 1032), (5, 3, 77), (2, 32, 4096), (130, 2, 7168)])
+def test_bwd_topk_weights(shape):
+    T, k, H = shape
+    g = torch.Generator().manual_seed(T * k + H)
+    d = torch.randn(T, H, generator=g).to(torch.bfloat16)
+    c = torch.randn(T * k, H, generator=g).to(torch.bfloat16)
+    got = mx8.bwd_topk_weights(d.to(DEV), c.to(DEV)).cpu().double()
+    terms = c.double().view(T, k, H) * d.double().view(T, 1, H)
+    # H products in fp32 with fused adds, at most H/256 + 8 + 7 of them in a chain per thread, lanes and warps
+    tol = (H / 128 + 16) * 2.0 ** -24 * terms.abs().sum(2)
+    assert ((got - terms.sum(2)).abs() <= tol).all()
+    idx = torch.randint(-1, 4, (T, k), generator=g, dtype=torch.int32)
+    c2 = c.clone()
+    c2[(idx < 0).reshape(-1)] = float("nan")                       # rows that no expert sent
+    part = mx8.bwd_topk_weights(d.to(DEV), c2.to(DEV), idx.to(DEV)).cpu().double()
+    assert torch.equal(part, torch.where(idx >= 0, got, 0.0))
+
+
+def test_refusals():
+    l = make_logits(8, 16, torch.float32, 0)
+    o = mx8.router_topk(l, 2)
+    for bad in (lambda: mx8.router_topk(l, 17), lambda: mx8.router_topk(l, 0)):
+        with pytest.raises(mx8.Mx8Error):
+            bad()
+    dw, dl = torch.zeros(8, 2, device=DEV), torch.zeros(1, device=DEV)
+    for bad in (lambda: mx8.router_topk(l.half(), 2), lambda: mx8.router_topk(l.t(), 2), lambda: mx8.router_topk(l[:0], 2),
+                lambda: mx8.router_topk(l, 2, token_mask=torch.ones(7, dtype=torch.bool, device=DEV)),
+                lambda: mx8.router_topk(l, 2, token_mask=torch.ones(8, dtype=torch.int32, device=DEV)),
+                lambda: mx8.router_topk(l, 2, token_mask=torch.ones(8, dtype=torch.bool)),
+                lambda: mx8.router_topk_bwd(l, o[0], o[1], o[2], o[3], o[5]),
+                lambda: mx8.router_topk_bwd(l, o[0], o[1], o[2], o[3], o[5], dw[:4], dl),
+                lambda: mx8.router_topk_bwd(l, o[0].long(), o[1], o[2], o[3], o[5], dw, dl),
+                lambda: mx8.router_topk_bwd(l, o[0], o[1], o[2], o[3][:8], o[5], dw, dl),
+                lambda: mx8.bwd_topk_weights(torch.zeros(3, 8, dtype=torch.bfloat16, device=DEV), torch.zeros(7, 8, dtype=torch.bfloat16, device=DEV)),
+                lambda: mx8.bwd_topk_weights(torch.zeros(3, 8, device=DEV), torch.zeros(6, 8, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_repeatable_on_a_side_stream_and_in_a_graph():
+    l = make_logits(4097, 256, torch.bfloat16, 12)
+    want = mx8.router_topk(l, 8)
+    dw, dl = torch.randn(4097, 8, device=DEV), torch.ones(1, device=DEV)
+    want_d = mx8.router_topk_bwd(l, want[0], want[1], want[2], want[3], want[5], dw, dl)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = mx8.router_topk(l, 8)
+        got_d = mx8.router_topk_bwd(l, got[0], got[1], got[2], got[3], got[5], dw, dl)
+    s.synchronize()
+    for a, b in zip(got + (got_d,), want + (want_d,)):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    src = torch.zeros_like(l)
+    with torch.cuda.graph(graph):
+        out = mx8.router_topk(src, 8)
+        out_d = mx8.router_topk_bwd(src, out[0], out[1], out[2], out[3], out[5], dw, dl)
+    src.copy_(l)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out + (out_d,), want + (want_d,)):
+        assert torch.equal(a, b)
