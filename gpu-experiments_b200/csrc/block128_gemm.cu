@@ -1,17 +1,18 @@
 // Matrix product of the block-128 format for sm_100a:
 //   C[i][j] = sum_kb sa[kb][i] * sb(kb, j) * sum_{k in block kb} A[i][k] * B[j][k],   A, B E4M3, scales fp32, C bf16 or fp32.
 // The scales are no powers of two and belong to 128 values of k, so the tensor core sums one block at a time (four
-// tcgen05.mma.kind::f8f6f4 of K = 32 into TMEM, fp32) and registers add the blocks up: acc += (sa sb) * partial, one rounding each.
+// tcgen05.mma.kind::f8f6f4 of K = 32 into TMEM, fp32) and registers add the blocks up: acc += scale * partial, one rounding each.
 //
-// One CTA per tile, ten (or six) warps: warp 0 streams operand tiles with TMA (128-byte swizzle) into a ring of stages, warp 1 issues
-// the MMAs of block kb into one of two TMEM buffers, the other warps read the buffer with tcgen05.ld, scale and add it into
-// registers while the MMAs of block kb + 1 fill the other buffer, and at the end write C.  128 x 256 x 128 is 512 tensor cycles; the
-// promotion of such a partial tile is 256 cycles of each fp32 pipe, so the two overlap when nothing stalls.
+// A CTA, or a pair of CTAs on one tile (cta_group::2), holds 128 rows of X each and up to TN rows of Y: warp 0 streams operand tiles
+// with TMA (128-byte swizzle) into a ring of stages, warp 1 issues the MMAs of block kb into one of two TMEM buffers, four or eight
+// warps read the buffer with tcgen05.ld, scale and add it into registers while the MMAs of block kb + 1 fill the other buffer, and at
+// the end write C.
 //
-// X is the operand whose rows are the 128 lanes of TMEM, Y the one whose rows are its columns: X = A, Y = B for many rows of A;
-// for few (SWAP) X = B, so that 128 rows of weights fill the lanes and the tokens, 16 to 64 of them, the columns.
-// split > 1: a cluster of `split` CTAs shares a tile, each takes a part of the K blocks, and the partial tiles are added through
-// distributed shared memory in rank order: no workspace, no atomics, the same result in every run.
+// X is the operand whose rows are the lanes of TMEM, Y the one whose rows are its columns.  X = A, Y = B for many rows of A.  For few
+// rows, and for rows that belong to experts (SWAP), X = B: the weights fill the lanes and a tile has as many columns (a
+// multiple of 16 or 32) as there are tokens, so that ragged groups cost what they hold.
+// split > 1: `split` CTAs or pairs of one cluster share a tile, each takes a part of the K blocks, and the partial tiles are added
+// through distributed shared memory in rank order: no workspace, no atomics, the same result in every run.
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
 #include <atomic>
 
@@ -27,40 +28,45 @@ constexpr int DEV_BAD_GROUPS = 17;            // device status: group sizes that
 constexpr int DEV_SMEM_BASE = 18;             // device status: dynamic shared memory does not start on a 1024-byte boundary
 constexpr int RED_PITCH = 129;                // floats between columns of the tile that a split adds up
 
-template <int TN_, bool SWAP_, bool COLVEC_>
+// where the two scales of a partial value vary inside a promoting warp
+enum Scales { ROW, COL, BOTH };               // by lane (Y's is one number), by column (X's is one number), by both
+
+template <int CG_, int TN_, bool SWAP_, Scales SC_>
 struct Cfg {
-    static constexpr int TN = TN_;
-    static constexpr bool SWAP = SWAP_, COLVEC = COLVEC_;
+    static constexpr int CG = CG_, TN = TN_;
+    static constexpr bool SWAP = SWAP_;
+    static constexpr Scales SC = SC_;
     static constexpr int EPI = TN >= 128 ? 8 : 4;             // promoting warps
-    static constexpr int CW = TN / (EPI / 4);                 // columns of a promoting warp
-    static constexpr int LW = CW < 32 ? CW : 32;              // columns per tcgen05.ld
-    static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN * BK;
+    static constexpr int EPI0 = TN >= 128 ? 4 : 2;            // the first of them
+    static constexpr int THREADS = 32 * (EPI0 + EPI);
+    static constexpr int CW = TN / (EPI / 4);                 // most columns of a promoting warp
+    static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN / CG * BK;
+    static constexpr int Y_BOX = SWAP ? (CG == 2 ? 32 : 16) : TN / CG;      // rows of Y per TMA copy: only boxes with tokens are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
-    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 4 : TN == 32 ? 5 : 6;
-    static constexpr int THREADS = 32 * (2 + EPI);
-    static constexpr int TMEM_COLS = 2 * TN < 32 ? 32 : 2 * TN;
-    static constexpr int EPI_BYTES = 32 * 32 * 4;             // per warp: 32 x 32 floats of C, or its columns' scales (two buffers)
+    static constexpr int STAGES = TN == 256 ? 6 : 4;
+    static constexpr int TMEM_COLS = 2 * TN;
+    static constexpr int EPI_BYTES = SWAP ? 2 * CW * 4 : 32 * 32 * 4;      // per warp: two buffers of column scales; 32 rows of 128 bytes of C
     static constexpr int epi_off = STAGES * STAGE;
     static constexpr int bar_off = epi_off + EPI * EPI_BYTES;
     static constexpr int n_bars = 2 * STAGES + 4;
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
-    static_assert(dynamic <= 232448, "shared memory budget exceeded");
+    static constexpr int PER_SM = TN >= 128 ? 1 : 2;
+    static_assert(dynamic * PER_SM <= 232448 - 1024 * (PER_SM - 1), "shared memory budget exceeded");
     static_assert(TN * RED_PITCH * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
     static_assert(2 * CW * 4 <= EPI_BYTES, "two buffers of column scales");
 };
 
 struct Params {
     int kblocks;                              // of K
-    int tiles_x, tiles_y, group_x;            // tile grid (per group), rasterisation
-    int x_rows, y_rows;                       // rows of X and Y per matrix (bounds of C)
-    const float* xs;                          // scale of X's row r in block kb at xs[r_off + kb * xs_k]
+    int tiles_x, tiles_y, group_x;            // tile grid (tiles_y: dense and weight gradient), rasterisation
+    int x_rows, y_rows;                       // rows of X and Y per matrix
+    const float* xs;                          // scale of X's row r in block kb: xs[r + kb * xs_k], squares: xs[(r / 128) * kblocks + kb]
     long long xs_k;
-    int xs_square;                            // xs is [row blocks][kblocks]
-    const float* ys;
+    int xs_square;
+    const float* ys;                          // the same for Y (never squares with SWAP, squares only with ROW)
     long long ys_k;
-    int y_group;                              // rows of Y per group
     void* c;
     long long ldc;
     int c_f32;
@@ -73,89 +79,74 @@ struct Params {
 };
 
 struct Tile {
-    int x0, xn;                               // first row of X, rows that exist in this tile
-    int y0, y_tma, yn;                        // first column inside C, first row of Y, columns that exist
+    int x0, x_tma;                            // first row of X of this CTA: inside its matrix, in the tensor map
+    int y0, y_end, ncols;                     // first row of Y, one past the last, columns of the MMA (both CTAs together)
     int k0, k1;                               // K blocks
     long long c_row;                          // first row of C of this tile's matrix
     int g;
 };
 
-__device__ __forceinline__ void tile_xy(int t, int group_x, int tiles_x, int tiles_y, int& tx, int& ty) {
-    const int per = group_x * tiles_y;
-    const int grp = t / per;
-    const int in = t - grp * per;
-    const int rows = min(group_x, tiles_x - grp * group_x);
-    tx = grp * group_x + in % rows;
-    ty = in / rows;
-}
+// columns of an MMA: a multiple of 16 for one CTA, of 32 for a pair (16 rows of Y in each)
+template <int CG>
+__device__ __forceinline__ int round_cols(int n) { return (n + 16 * CG - 1) / (16 * CG) * (16 * CG); }
 
 // seg[g] = first row of group g, seg[MAX_GROUPS + 1 + g] = first tile of group g
 template <class C>
-__device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, int rank) {
+__device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, int pair_rank, int part) {
     Tile o;
-    int tx, ty;
     o.g = 0;
     o.c_row = 0;
     o.k0 = 0;
     o.k1 = p.kblocks;
-    int base = 0, tiles_x = p.tiles_x;
+    int first = 0, row0 = 0, rows = p.y_rows, tx, ty;
     if (p.groups > 0) {
-        const int* first = seg + MAX_GROUPS + 1;
-        int lo = 0, hi = p.groups - 1;                        // last group whose first tile is <= t and that has tiles
+        const int* firsts = seg + MAX_GROUPS + 1;
+        int lo = 0, hi = p.groups - 1;                        // last group whose first tile is <= t: the one that has tile t
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (first[mid] <= t) lo = mid; else hi = mid - 1;
+            if (firsts[mid] <= t) lo = mid; else hi = mid - 1;
         }
         o.g = lo;
-        base = first[lo];
-        if (!p.wgrad) tiles_x = (first[lo + 1] - base) / p.tiles_y;
+        first = firsts[lo];
     }
-    tile_xy(t - base, p.group_x, tiles_x, p.tiles_y, tx, ty);
-    o.x0 = tx * 128;
-    o.xn = min(128, p.x_rows - o.x0);
-    o.y0 = ty * C::TN;
-    o.y_tma = o.y0;
-    o.yn = min(C::TN, p.y_rows - o.y0);
-    if (p.groups > 0) {
-        if (p.wgrad) {
+    if constexpr (C::SWAP) {
+        // the tokens of a group in as few tiles as hold them, of equal width; a weight tile's token tiles one after the other
+        if (p.groups > 0) {
+            row0 = seg[o.g];
+            rows = seg[o.g + 1] - row0;
+        }
+        const int nt = (rows + C::TN - 1) / C::TN, width = round_cols<C::CG>((rows + nt - 1) / nt);
+        tx = (t - first) / nt;
+        ty = (t - first) - tx * nt;
+        o.y0 = row0 + ty * width;
+        o.y_end = min(o.y0 + width, row0 + rows);
+        o.x0 = tx * 128 * C::CG;
+        o.x_tma = o.x0 + o.g * p.x_rows;
+    } else {
+        // groups of `group_x` tile rows, column-major inside, so that CTAs running together share panels in L2
+        const int in_all = t - first, per = p.group_x * p.tiles_y;
+        const int grp = in_all / per, in = in_all - grp * per, n = min(p.group_x, p.tiles_x - grp * p.group_x);
+        tx = grp * p.group_x + in % n;
+        ty = in / n;
+        o.y0 = ty * C::TN;
+        o.y_end = min(o.y0 + C::TN, p.y_rows);
+        o.x0 = tx * 128 * C::CG;
+        o.x_tma = o.x0;
+        if (p.groups > 0) {                                   // weight gradient
             o.k0 = seg[o.g] / BK;
             o.k1 = seg[o.g + 1] / BK;
             o.c_row = static_cast<long long>(o.g) * p.x_rows;
-        } else {
-            o.x0 += seg[o.g];
-            o.xn = min(128, seg[o.g + 1] - o.x0);
-            o.y_tma += o.g * p.y_group;
         }
     }
+    o.ncols = round_cols<C::CG>(o.y_end - o.y0);
+    o.x0 += pair_rank * 128;
+    o.x_tma += pair_rank * 128;
     if (p.split > 1) {
         const int n = o.k1 - o.k0, k0 = o.k0;
-        o.k0 = k0 + n * rank / p.split;
-        o.k1 = k0 + n * (rank + 1) / p.split;
+        o.k0 = k0 + n * part / p.split;
+        o.k1 = k0 + n * (part + 1) / p.split;
     }
     return o;
-}
-
-template <int N>
-__device__ __forceinline__ void tc_ld(uint32_t taddr, uint32_t (&r)[N]) {
-    if constexpr (N == 32) {
-        tc_ld_32x32(taddr, r);
-    } else {
-        static_assert(N == 16, "");
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-            : "r"(taddr)
-            : "memory");
-    }
-}
-__device__ __forceinline__ void tc_wait(uint32_t (&r)[32]) { tc_wait_ld(r); }
-__device__ __forceinline__ void tc_wait(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
 }
 
 // pairs of floats in 64-bit registers: one instruction for two columns
@@ -181,6 +172,26 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+template <int N>
+__device__ __forceinline__ void set_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void set_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Arrive on a barrier of the pair's leading CTA.  What it orders are TMEM reads, which tcgen05.fence::before_thread_sync covers; the
+// release.cluster form would also wait for the warp's outstanding global loads, once per K block (1.21 instead of 0.5 us a block).
+__device__ __forceinline__ void arrive_pair(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Arrive on `bar` of this CTA, or of both CTAs of the pair that starts at cluster rank `first`, once this thread's MMAs are complete.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar, int first) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(static_cast<uint16_t>(3u << first)) : "memory");
+    else
+        tc_commit<1>(bar);
+}
 
 __device__ __forceinline__ void store_c(const Params& p, long long row, int col, float v) {
     const long long at = row * p.ldc + col;
@@ -188,9 +199,109 @@ __device__ __forceinline__ void store_c(const Params& p, long long row, int col,
     else static_cast<uint16_t*>(p.c)[at] = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
+// One warp's 32 rows x CW columns of C (row = lane): turned through shared memory, 128 bytes of a row at a time, so that a store covers
+// whole 128-byte pieces of rows (16 bytes per lane).  The 16-byte piece k of row r lies in slot k ^ (r % 8): conflict-free both ways.
+template <int CW>
+__device__ __forceinline__ void write_rows(const Params& p, const uint64_t (&acc)[CW / 2], uint32_t stg, long long row0, int rows, int col0, int cols,
+                                           int lane) {
+    const int esize = p.c_f32 ? 4 : 2, per = 128 / esize;                 // columns in 128 bytes
+    uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * esize;
+    const long long pitch = p.ldc * esize;
+    const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0;
+    const uint32_t put = stg + lane * 128 + ((lane & 7) << 4);
+#pragma unroll
+    for (int j = 0; j < CW; j += 32) {
+        if (!p.c_f32 && (j & 32)) continue;
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            uint32_t w[4];
+            if (p.c_f32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(half_of(acc[j / 2 + 2 * k + i / 2], i & 1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(half_of(acc[(j / 2 + 4 * k + i) % (CW / 2)], 0), half_of(acc[(j / 2 + 4 * k + i) % (CW / 2)], 1));
+            }
+            st_shared_v4(put ^ (k << 4), w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+        if (wide && cols - j >= per) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3);
+                uint32_t w[4];
+                ld_shared_v4(stg + r * 128 + (((lane ^ r) & 7) << 4), w[0], w[1], w[2], w[3]);
+                if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 7) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else {
+            const int left = cols - j - lane * (4 / esize);
+#pragma unroll 1
+            for (int r = 0; r < rows; ++r) {
+                uint32_t w;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+                uint8_t* to = c + r * pitch + j * esize + lane * 4;
+                if (p.c_f32) {
+                    if (left >= 1) *reinterpret_cast<uint32_t*>(to) = w;
+                } else {
+                    if (left >= 1) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
+                    if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
+
+// Prefix sums of the group sizes by one warp; sizes that do not fit are cut to what the operands have, and reported.
 template <class C>
-__global__ void __launch_bounds__(C::THREADS, C::SWAP ? 2 : 1)
+__device__ __forceinline__ void group_prefix(const Params& p, int* seg, int lane) {
+    int tile = 0;
+    long long row = 0;
+    bool bad = false;
+    const int cap = p.wgrad ? p.rows_cap / BK * BK : p.rows_cap;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        const int g = g0 + lane;
+        int n = g < p.groups ? p.group_rows[g] : 0;
+        if (n < 0 || (p.wgrad && n % BK) || n > cap) {
+            bad = true;
+            n = max(0, min(n, cap));
+            if (p.wgrad) n -= n % BK;
+        }
+        long long end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, end, o);
+            if (lane >= o) end += u;
+        }
+        end += row;
+        if (end > cap) bad = true;
+        const int e = static_cast<int>(min(end, static_cast<long long>(cap))), b = static_cast<int>(min(end - n, static_cast<long long>(cap)));
+        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + C::TN - 1) / C::TN * p.tiles_x;
+        int tt = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, tt, o);
+            if (lane >= o) tt += u;
+        }
+        if (g < p.groups) {
+            seg[g] = b;
+            seg[MAX_GROUPS + 1 + g] = tile + tt - nt;
+            if (g == p.groups - 1) {
+                seg[p.groups] = e;
+                seg[MAX_GROUPS + 1 + p.groups] = tile + tt;
+            }
+        }
+        row = __shfl_sync(0xFFFFFFFFu, end, 31);
+        tile += __shfl_sync(0xFFFFFFFFu, tt, 31);
+    }
+    if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicCAS(p.status, 0, DEV_BAD_GROUPS);
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, C::PER_SM)
 gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y, const Params p) {
+    constexpr int CG = C::CG, S = C::STAGES;
     // the swizzle counts from 1024-byte boundaries; with no static shared memory the dynamic part starts on one
     extern __shared__ __align__(1024) uint8_t base_ptr[];
     const uint32_t base = smem_u32(base_ptr);
@@ -198,235 +309,225 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         if (threadIdx.x == 0) atomicCAS(p.status, 0, DEV_SMEM_BASE);
         return;
     }
-    constexpr int S = C::STAGES;
     const uint32_t full0 = base + C::bar_off, empty0 = full0 + S * 8, accfull0 = empty0 + S * 8, accfree0 = accfull0 + 16;
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + C::misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + C::misc_off + 8);
     int* seg = reinterpret_cast<int*>(base_ptr + C::seg_off);
     const AbortCtl ab{abort_flag, p.status};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-    const int unit = blockIdx.x / p.split, units = gridDim.x / p.split;
+    const int cluster = CG * p.split;                         // CTAs that share a tile
+    const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int pair_rank = CG == 2 ? rank & 1 : 0, part = rank / CG, first_rank = rank - pair_rank;
+    const int unit = blockIdx.x / cluster, units = gridDim.x / cluster;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < S; ++s) {
-            mbar_init(full0 + s * 8, 1);
-            mbar_init(empty0 + s * 8, 1);
+            mbar_init(full0 + s * 8, 1);                      // the leading CTA's arrive.expect_tx
+            mbar_init(empty0 + s * 8, 1);                     // one tcgen05.commit
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(accfull0 + b * 8, 1);
-            mbar_init(accfree0 + b * 8, C::EPI);
+            mbar_init(accfree0 + b * 8, C::EPI * CG);         // promoting warps of the pair, on the leading CTA's barrier
         }
         fence_mbar_init();
         prefetch_tmap(&tm_x);
         prefetch_tmap(&tm_y);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_ptr)), C::TMEM_COLS);
-        tmem_relinquish<1>();
+        tmem_alloc<CG>(smem_u32(const_cast<uint32_t*>(tmem_ptr)), C::TMEM_COLS);
+        tmem_relinquish<CG>();
     }
-    if (warp == 2 && p.groups > 0) {
-        // prefix sums of the group sizes; sizes that do not fit are cut to what the operands have, and reported
-        int row = 0, tile = 0;
-        bool bad = false;
-        for (int g0 = 0; g0 < p.groups; g0 += 32) {
-            const int g = g0 + lane;
-            int n = g < p.groups ? p.group_rows[g] : 0;
-            if (n < 0 || (p.wgrad && n % BK) || n > p.rows_cap) {
-                bad = true;
-                n = max(0, min(n, p.rows_cap));
-                if (p.wgrad) n -= n % BK;
-            }
-            long long r = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xFFFFFFFFu, r, o);
-                if (lane >= o) r += u;
-            }
-            long long first = row + r - n, end = row + r;
-            if (end > p.rows_cap) bad = true;
-            const int cap = p.wgrad ? p.rows_cap / BK * BK : p.rows_cap;
-            first = min(first, static_cast<long long>(cap));
-            end = min(end, static_cast<long long>(cap));
-            int nt = p.wgrad ? p.tiles_x * p.tiles_y : static_cast<int>((end - first + 127) / 128) * p.tiles_y;
-            if (g >= p.groups) nt = 0;
-            int tt = nt;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xFFFFFFFFu, tt, o);
-                if (lane >= o) tt += u;
-            }
-            if (g < p.groups) {
-                seg[g] = static_cast<int>(first);
-                seg[MAX_GROUPS + 1 + g] = tile + tt - nt;
-                if (g == p.groups - 1) {
-                    seg[p.groups] = static_cast<int>(end);
-                    seg[MAX_GROUPS + 1 + p.groups] = tile + tt;
-                }
-            }
-            row = static_cast<int>(__shfl_sync(0xFFFFFFFFu, end, 31));
-            tile += __shfl_sync(0xFFFFFFFFu, tt, 31);
-        }
-        if (__any_sync(0xFFFFFFFFu, bad) && lane == 0) atomicCAS(p.status, 0, DEV_BAD_GROUPS);
-    }
+    if (warp == 2 && p.groups > 0) group_prefix<C>(p, seg, lane);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_ptr, 0);
     const int num_tiles = p.groups > 0 ? __shfl_sync(0xFFFFFFFFu, seg[MAX_GROUPS + 1 + p.groups], 0) : p.tiles_x * p.tiles_y;
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ producer
-        const bool leader = elect_one();
-        uint32_t stage = 0, ph = 0;
-        bool ok = true;
-        for (int t = unit; t < num_tiles && ok; t += units) {
-            const Tile ti = tile_at<C>(t, p, seg, rank);
-            const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x0, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y_tma, 0);
-            const int k0 = __shfl_sync(0xFFFFFFFFu, ti.k0, 0), k1 = __shfl_sync(0xFFFFFFFFu, ti.k1, 0);
-            for (int kb = k0; kb < k1; ++kb) {
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty0 + stage * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY))) { ok = false; break; }
-                if (leader) {
-                    const uint32_t dst = base + stage * C::STAGE, bar = full0 + stage * 8;
-                    mbar_arrive_expect_tx(bar, C::STAGE);
-                    tma_load_2d(dst, &tm_x, kb * BK, x0, bar);
-                    tma_load_2d(dst + C::X_BYTES, &tm_y, kb * BK, y0, bar);
+    if (warp < C::EPI0) {
+        // with eight promoting warps three warpgroups run, launched with 168 registers a thread: 4 * 40 + 8 * 232 = 12 * 168
+        if constexpr (C::EPI == 8) set_regs_less<40>();
+        if (warp == 0) {
+            // ------------------------------------------------------------ producer
+            const bool leader = elect_one();
+            uint32_t stage = 0, ph = 0;
+            const uint32_t full_lead = CG == 2 ? map_to_cta(full0, first_rank) : full0;
+            bool ok = true;
+            for (int t = unit; t < num_tiles && ok; t += units) {
+                const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
+                const int ny = ti.ncols / CG, boxes = (ny + C::Y_BOX - 1) / C::Y_BOX;     // rows and copies of Y of this CTA
+                const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x_tma, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y0 + pair_rank * ny, 0);
+                const int k0 = __shfl_sync(0xFFFFFFFFu, ti.k0, 0), k1 = __shfl_sync(0xFFFFFFFFu, ti.k1, 0);
+                const int nb = __shfl_sync(0xFFFFFFFFu, boxes, 0);
+                for (int kb = k0; kb < k1; ++kb) {
+                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty0 + stage * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY))) { ok = false; break; }
+                    if (leader) {
+                        const uint32_t dst = base + stage * C::STAGE, bytes = C::X_BYTES + nb * C::Y_BOX * BK;
+                        if (CG == 1 || pair_rank == 0) mbar_arrive_expect_tx(full0 + stage * 8, CG * bytes);
+                        const uint32_t bar = full_lead + stage * 8;
+                        if constexpr (CG == 2) tma_load_2d_pair(dst, &tm_x, kb * BK, x0, bar);
+                        else tma_load_2d(dst, &tm_x, kb * BK, x0, bar);
+#pragma unroll
+                        for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i) {
+                            if (i >= nb) break;
+                            const uint32_t to = dst + C::X_BYTES + i * C::Y_BOX * BK;
+                            if constexpr (CG == 2) tma_load_2d_pair(to, &tm_y, kb * BK, y0 + i * C::Y_BOX, bar);
+                            else tma_load_2d(to, &tm_y, kb * BK, y0 + i * C::Y_BOX, bar);
+                        }
+                    }
+                    __syncwarp();
+                    if (++stage == S) { stage = 0; ph ^= 1; }
                 }
-                __syncwarp();
-                if (++stage == S) { stage = 0; ph ^= 1; }
             }
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA
-        const bool leader = elect_one();
-        constexpr uint32_t idesc = idesc_e4m3(128, C::TN);
-        uint32_t stage = 0, ph = 0, it = 0;
-        bool ok = true;
-        for (int t = unit; t < num_tiles && ok; t += units) {
-            const Tile ti = tile_at<C>(t, p, seg, rank);
-            const int n = __shfl_sync(0xFFFFFFFFu, ti.k1 - ti.k0, 0);
-            for (int i = 0; i < n; ++i, ++it) {
-                const uint32_t buf = it & 1, use = it >> 1;
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(full0 + stage * 8, ph, ab, DEV_TIMEOUT_FULL))) { ok = false; break; }
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(accfree0 + buf * 8, (use & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE))) { ok = false; break; }
-                tc_fence_after();
-                if (leader) {
-                    const uint32_t x = desc_sw128_lo(base + stage * C::STAGE), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
-                    const uint32_t d = tmem + buf * C::TN;
-                    tc_mma_e4m3_lo<1, 0>(d, x, y, idesc);
-                    tc_mma_e4m3_lo<1, 1>(d, x + 2, y + 2, idesc);
-                    tc_mma_e4m3_lo<1, 1>(d, x + 4, y + 4, idesc);
-                    tc_mma_e4m3_lo<1, 1>(d, x + 6, y + 6, idesc);
-                    tc_commit<1>(empty0 + stage * 8);
-                    tc_commit<1>(accfull0 + buf * 8);
+        } else if (warp == 1 && pair_rank == 0) {
+            // ------------------------------------------------------------ MMA (leading CTA of a pair)
+            const bool leader = elect_one();
+            uint32_t stage = 0, ph = 0, it = 0;
+            bool ok = true;
+            for (int t = unit; t < num_tiles && ok; t += units) {
+                const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
+                const int n = __shfl_sync(0xFFFFFFFFu, ti.k1 - ti.k0, 0);
+                const uint32_t idesc = idesc_e4m3(128 * CG, __shfl_sync(0xFFFFFFFFu, ti.ncols, 0));
+                for (int i = 0; i < n; ++i, ++it) {
+                    const uint32_t buf = it & 1, use = it >> 1;
+                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(full0 + stage * 8, ph, ab, DEV_TIMEOUT_FULL))) { ok = false; break; }
+                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(accfree0 + buf * 8, (use & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE))) { ok = false; break; }
+                    tc_fence_after();
+                    if (leader) {
+                        const uint32_t x = desc_sw128_lo(base + stage * C::STAGE), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
+                        const uint32_t d = tmem + buf * C::TN;
+                        tc_mma_e4m3_lo<CG, 0>(d, x, y, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
+                        commit<CG>(empty0 + stage * 8, first_rank);
+                        commit<CG>(accfull0 + buf * 8, first_rank);
+                    }
+                    __syncwarp();
+                    if (++stage == S) { stage = 0; ph ^= 1; }
                 }
-                __syncwarp();
-                if (++stage == S) { stage = 0; ph ^= 1; }
             }
         }
     } else {
         // ------------------------------------------------------------ promotion and C
-        const int ew = warp - 2, q = warp & 3, half = ew >> 2;          // TMEM lane quadrant, column half
-        uint8_t* stg = base_ptr + C::epi_off + ew * C::EPI_BYTES;
-        float* stgf = reinterpret_cast<float*>(stg);
-        const uint32_t my_tmem = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * C::CW;
-        const int col0 = half * C::CW;
+        if constexpr (C::EPI == 8) set_regs_more<232>();
+        const int ew = warp - C::EPI0, q = warp & 3, half = ew >> 2;    // TMEM lane quadrant, column half
+        float* stgf = reinterpret_cast<float*>(base_ptr + C::epi_off + ew * C::EPI_BYTES);
+        const uint32_t free_lead = CG == 2 ? map_to_cta(accfree0, first_rank) : accfree0;
+        const int r = q * 32 + lane;                                     // row of this CTA's tile
         uint32_t it = 0;
         bool ok = true;
         for (int t = unit; t < num_tiles && ok; t += units) {
-            const Tile ti = tile_at<C>(t, p, seg, rank);
-            const int r = q * 32 + lane;                                 // row of the tile
-            // scales of this lane's row; rows beyond the tile take the last one's
-            const int xr = ti.x0 + min(r, ti.xn - 1);
-            long long x_off = p.xs_square ? static_cast<long long>(xr / 128) * p.kblocks : xr;
-            const float* xs = p.xs + x_off;
-            const float* ys;
-            int yc[C::CW / 32 > 0 ? C::CW / 32 : 1];
-            if constexpr (C::COLVEC) {
-                ys = p.ys;
-#pragma unroll
-                for (int i = 0; i < (C::CW + 31) / 32; ++i) yc[i] = ti.y0 + min(col0 + i * 32 + lane, ti.yn - 1);
+            const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
+            // this warp's columns; with tokens in the columns both halves get the same share
+            const int cw = C::EPI == 4 ? ti.ncols : C::SWAP ? ti.ncols / 2 : C::CW;
+            const int col0 = half * cw, mine = min(cw, ti.ncols - col0);  // <= 0: nothing
+            const uint32_t my_tmem = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
+            // scales; rows and columns beyond the tile take the last one's
+            const int xr = min(ti.x0 + r, p.x_rows - 1);
+            const float* xs = p.xs;
+            if (p.xs_square) xs += (static_cast<long long>(ti.g) * ((p.x_rows + 127) / 128) + xr / 128) * p.kblocks;
+            else xs += xr;
+            const float* ys = p.ys;
+            int yc[C::CW / 32];
+            if constexpr (C::SC == ROW) {
+                ys += static_cast<long long>(min(ti.y0 + col0, p.y_rows - 1) / 128) * p.kblocks;
             } else {
-                const int nb = ti.g * ((p.y_rows + 127) / 128) + (ti.y0 + min(col0, ti.yn - 1)) / 128;
-                ys = p.ys + static_cast<long long>(nb) * p.kblocks;
+#pragma unroll
+                for (int i = 0; i < C::CW / 32; ++i) yc[i] = min(ti.y0 + col0 + i * 32 + lane, ti.y_end - 1);
             }
             uint64_t acc[C::CW / 2];
 #pragma unroll
             for (int i = 0; i < C::CW / 2; ++i) acc[i] = 0;
-            float xn = 0.0f, yn = 0.0f, ycol[(C::CW + 31) / 32];
+            float xn = 0.0f, yn = 0.0f, ycol[C::CW / 32];
             auto fetch = [&](int kb) {
                 xn = __ldg(xs + kb * p.xs_k);
-                if constexpr (C::COLVEC) {
-#pragma unroll
-                    for (int i = 0; i < (C::CW + 31) / 32; ++i) ycol[i] = __ldg(ys + kb * p.ys_k + yc[i]);
-                } else {
+                if constexpr (C::SC == ROW) {
                     yn = __ldg(ys + kb);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < C::CW / 32; ++i)
+                        if (i * 32 < mine) ycol[i] = __ldg(ys + kb * p.ys_k + yc[i]);
                 }
             };
             if (ti.k0 < ti.k1) fetch(ti.k0);
             for (int kb = ti.k0; kb < ti.k1; ++kb, ++it) {
                 const uint32_t buf = it & 1;
                 float s = xn;
-                if constexpr (C::COLVEC) {
+                if constexpr (C::SC == ROW) {
+                    s *= yn;
+                } else {
                     // two buffers: the other one may still be read by slower lanes of this warp
 #pragma unroll
-                    for (int i = 0; i < (C::CW + 31) / 32; ++i)
-                        if (i * 32 + lane < C::CW) stgf[buf * C::CW + i * 32 + lane] = ycol[i];
+                    for (int i = 0; i < C::CW / 32; ++i)
+                        if (i * 32 < mine) stgf[buf * C::CW + i * 32 + lane] = C::SC == COL ? ycol[i] * xn : ycol[i];
                     __syncwarp();
-                } else {
-                    s *= yn;
                 }
                 if (kb + 1 < ti.k1) fetch(kb + 1);
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL))) { ok = false; break; }
                 tc_fence_after();
                 const uint64_t ss = pair(__float_as_uint(s), __float_as_uint(s));
-#pragma unroll
-                for (int c = 0; c < C::CW; c += C::LW) {
-                    uint32_t v[C::LW];
-                    tc_ld<C::LW>(my_tmem + buf * C::TN + c, v);
-                    tc_wait(v);
-                    if (c + C::LW == C::CW) {                            // the buffer's values are all in registers
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(accfree0 + buf * 8);
+                auto release = [&]() {                                   // the buffer's values are all in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (CG == 2) arrive_pair(free_lead + buf * 8);
+                        else mbar_arrive(free_lead + buf * 8);
                     }
+                };
+                // the next 32 columns are on their way while these are added
+                constexpr int NB = C::EPI == 8 ? 2 : 1;
+                uint32_t v[NB][32];
+                if (mine > 0) tc_ld_32x32(my_tmem + buf * C::TN, v[0]);
+                else release();
 #pragma unroll
-                    for (int i = 0; i < C::LW; i += 2) {
-                        uint64_t part = pair(v[i], v[i + 1]);
-                        if constexpr (C::COLVEC) {
-                            const uint64_t cs = *reinterpret_cast<const uint64_t*>(&stgf[buf * C::CW + c + i]);
-                            part = mul2(part, cs);
+                for (int c = 0; c < C::CW / 32; ++c) {
+                    if (c * 32 < mine) {
+                        tc_wait_ld(v[c % NB]);
+                        const bool more = c + 1 < C::CW / 32 && (c + 1) * 32 < mine;
+                        if (!more) release();
+                        else if (NB == 2) tc_ld_32x32(my_tmem + buf * C::TN + (c + 1) * 32, v[(c + 1) % NB]);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            uint64_t a = pair(v[c % NB][i], v[c % NB][i + 1]), b = pair(v[c % NB][i + 2], v[c % NB][i + 3]);
+                            uint64_t fa = ss, fb = ss;
+                            if constexpr (C::SC != ROW) {
+                                const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&stgf[buf * C::CW + c * 32 + i]);
+                                if constexpr (C::SC == BOTH) {
+                                    a = mul2(a, cs.x);
+                                    b = mul2(b, cs.y);
+                                } else {
+                                    fa = cs.x;
+                                    fb = cs.y;
+                                }
+                            }
+                            acc[c * 16 + i / 2] = fma2(a, fa, acc[c * 16 + i / 2]);
+                            acc[c * 16 + i / 2 + 1] = fma2(b, fb, acc[c * 16 + i / 2 + 1]);
                         }
-                        acc[(c + i) / 2] = fma2(part, ss, acc[(c + i) / 2]);
+                        if (NB == 1 && more) tc_ld_32x32(my_tmem + buf * C::TN + (c + 1) * 32, v[0]);
                     }
                 }
             }
             if (!ok) break;
+            const int cols = min(mine, ti.y_end - ti.y0 - col0);          // that exist
             if (p.split > 1) {
                 // this CTA's MMAs are complete (its last accumulator arrived), so the stage ring is free
                 float* red = reinterpret_cast<float*>(base_ptr);
 #pragma unroll
-                for (int i = 0; i < C::CW; ++i) red[(col0 + i) * RED_PITCH + r] = half_of(acc[i / 2], i & 1);
+                for (int i = 0; i < C::CW; ++i)
+                    if (i < cols) red[(col0 + i) * RED_PITCH + r] = half_of(acc[i / 2], i & 1);
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
+                if (ti.x0 + r < p.x_rows) {
 #pragma unroll
-                for (int i = 0; i < C::CW; ++i)
-                    if (r < ti.xn && col0 + i < ti.yn) store_c(p, ti.y0 + col0 + i, ti.x0 + r, half_of(acc[i / 2], i & 1));
-            } else {
-                // 32 x 32 pieces turned through shared memory so that a store covers consecutive columns
-#pragma unroll
-                for (int c = 0; c < C::CW; c += 32) {
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) stgf[lane * 32 + (i ^ lane)] = half_of(acc[(c + i) / 2], i & 1);
-                    __syncwarp();
-                    const int rows = min(32, ti.xn - q * 32);
-                    if (col0 + c + lane < ti.yn)
-                        for (int i = 0; i < rows; ++i) store_c(p, ti.c_row + ti.x0 + q * 32 + i, ti.y0 + col0 + c + lane, stgf[i * 32 + (lane ^ i)]);
+                    for (int i = 0; i < C::CW; ++i)
+                        if (i < cols) store_c(p, ti.y0 + col0 + i, ti.x0 + r, half_of(acc[i / 2], i & 1));
                 }
-                __syncwarp();
+            } else {
+                write_rows<C::CW>(p, acc, smem_u32(stgf), ti.c_row + ti.x0 + q * 32, min(32, p.x_rows - ti.x0 - q * 32), ti.y0 + col0, cols, lane);
             }
         }
     }
@@ -434,34 +535,31 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     if (p.split > 1) {
         __syncwarp();
         cluster_sync_all();
-        if (warp >= 2 && unit < num_tiles) {
-            const Tile ti = tile_at<C>(unit, p, seg, rank);
-            const int ew = warp - 2;
+        if (warp >= C::EPI0 && unit < num_tiles) {
+            const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
+            const int ew = warp - C::EPI0, xn = min(128, p.x_rows - ti.x0), yn = ti.y_end - ti.y0;
             if constexpr (C::SWAP) {
-                // rank r writes its share of the tile's columns (rows of C); a lane is a row of the tile (column of C)
-                const int c1 = C::TN * (rank + 1) / p.split;
-                for (int c = C::TN * rank / p.split + (ew >> 2); c < min(c1, ti.yn); c += C::EPI / 4) {
-                    const int r = (ew & 3) * 32 + lane;
+                // part k writes its share of the tile's columns (rows of C); a lane is a row of the tile (column of C)
+                const int c1 = yn * (part + 1) / p.split, r = (ew & 3) * 32 + lane;
+                for (int c = yn * part / p.split + (ew >> 2); c < c1; c += C::EPI / 4) {
                     const uint32_t at = base + (c * RED_PITCH + r) * 4;
                     float s = 0.0f;
-                    for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k));
-                    if (r < ti.xn) store_c(p, ti.y0 + c, ti.x0 + r, s);
+                    for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
+                    if (r < xn) store_c(p, ti.y0 + c, ti.x0 + r, s);
                 }
             } else {
-                // rank r writes its share of the tile's rows; a lane is a column
-                const int r1 = 128 * (rank + 1) / p.split;
-                for (int r = 128 * rank / p.split + ew; r < min(r1, ti.xn); r += C::EPI) {
-                    for (int c = lane; c < ti.yn; c += 32) {
+                // part k writes its share of the tile's rows; a lane is a column
+                const int r1 = min(128 * (part + 1) / p.split, xn);
+                for (int r = 128 * part / p.split + ew; r < r1; r += C::EPI) {
+                    for (int c = lane; c < yn; c += 32) {
                         const uint32_t at = base + (c * RED_PITCH + r) * 4;
                         float s = 0.0f;
-                        for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k));
+                        for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
                         store_c(p, ti.c_row + ti.x0 + r, ti.y0 + c, s);
                     }
                 }
             }
         }
-        __syncwarp();
-        cluster_sync_all();                                              // nobody leaves while its tile is read
     }
 
     if (*abort_flag) {
@@ -471,10 +569,11 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     }
     __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    // nobody leaves while its tile is read, its TMEM written or its barriers arrived on
+    if (cluster > 1) cluster_sync_all(); else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc<1>(tmem, C::TMEM_COLS);
+        tmem_dealloc<CG>(tmem, C::TMEM_COLS);
     }
 }
 
@@ -502,35 +601,28 @@ static int operand_map(CUtensorMap* m, const void* base, long long rows, int K, 
 template <class C>
 static int launch(const Args& a, int split, cudaStream_t stream) {
     CUtensorMap mx, my;
-    const long long b_rows = a.groups > 0 && !a.wgrad ? static_cast<long long>(a.groups) * a.N : a.N;
+    const bool grouped = a.groups > 0 && !a.wgrad;
     int rc;
     if (C::SWAP) {
-        if ((rc = operand_map(&mx, a.B, b_rows, a.K, a.ldb, 128)) != MX8_OK) return rc;
-        if ((rc = operand_map(&my, a.A, a.M, a.K, a.lda, C::TN)) != MX8_OK) return rc;
+        if ((rc = operand_map(&mx, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
+        if ((rc = operand_map(&my, a.A, a.M, a.K, a.lda, C::Y_BOX)) != MX8_OK) return rc;
     } else {
         if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, 128)) != MX8_OK) return rc;
-        if ((rc = operand_map(&my, a.B, b_rows, a.K, a.ldb, C::TN)) != MX8_OK) return rc;
+        if ((rc = operand_map(&my, a.B, a.N, a.K, a.ldb, C::Y_BOX)) != MX8_OK) return rc;
     }
     Params p{};
     p.kblocks = (a.K + BK - 1) / BK;
     p.x_rows = C::SWAP ? a.N : a.M;
     p.y_rows = C::SWAP ? a.M : a.N;
-    p.tiles_x = (p.x_rows + 127) / 128;
+    p.tiles_x = (p.x_rows + 128 * C::CG - 1) / (128 * C::CG);
     p.tiles_y = (p.y_rows + C::TN - 1) / C::TN;
     p.group_x = 16;                           // 16 tile rows walked together keep their X panels and the Y panel in L2
-    if (C::SWAP) {
-        p.xs = a.B_sc;
-        p.xs_square = a.b_square;
-        p.xs_k = a.b_square ? 1 : a.ldsb;
-        p.ys = a.A_sc;
-        p.ys_k = a.ldsa;
-    } else {
-        p.xs = a.A_sc;
-        p.xs_k = a.ldsa;
-        p.ys = a.B_sc;
-        p.ys_k = a.b_square ? 1 : a.ldsb;
-    }
-    p.y_group = a.N;
+    const float* bs = a.B_sc;
+    p.xs = C::SWAP ? bs : a.A_sc;
+    p.xs_square = C::SWAP && a.b_square;
+    p.xs_k = C::SWAP ? (a.b_square ? 1 : a.ldsb) : a.ldsa;
+    p.ys = C::SWAP ? a.A_sc : bs;
+    p.ys_k = C::SWAP ? a.ldsa : (a.b_square ? 1 : a.ldsb);
     p.c = a.c;
     p.ldc = a.ldc;
     p.c_f32 = a.c_f32;
@@ -547,24 +639,26 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
         note_cuda_error("cudaFuncSetAttribute(gemm_block128)", cudaGetErrorString(e));
         return MX8_ERR_CUDA;
     }
-    // tiles that there can be: with groups every one may add a partial tile row
+    // tiles that there can be: with groups every one may add a partial tile
     long long tiles = static_cast<long long>(p.tiles_x) * p.tiles_y;
-    if (a.groups > 0) tiles = a.wgrad ? tiles * a.groups : static_cast<long long>(p.tiles_x + a.groups) * p.tiles_y;
-    if (tiles > 0x7FFFFFFFll / 8) {
-        note_cuda_error("gemm_block128", "more than 2^28 tiles");
+    if (a.wgrad) tiles *= a.groups;
+    else if (grouped) tiles += static_cast<long long>(p.tiles_x) * a.groups;
+    if (tiles > 0x7FFFFFFFll / 16) {
+        note_cuda_error("gemm_block128", "more than 2^27 tiles");
         return MX8_ERR_LIMIT;
     }
-    long long grid = tiles * split;
-    const long long resident = static_cast<long long>(sm_count()) * (C::SWAP ? 2 : 1);
-    if (split == 1 && grid > resident) grid = resident;        // persistent; a split tile needs a cluster of its own
+    const int cluster = C::CG * split;
+    long long units = tiles;
+    const long long resident = sm_count() / C::CG * C::PER_SM;
+    if (split == 1 && units > resident) units = resident;      // persistent; a split tile needs a cluster of its own
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::dynamic;
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = static_cast<unsigned>(split);
+    at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
@@ -577,37 +671,28 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     return MX8_OK;
 }
 
+// parts of K so that `units` tiles fill `room` places; a part has two K blocks at least, a cluster eight CTAs at most
+static int split_for(long long units, long long room, int kblocks, int most) {
+    long long s = units > 0 ? room / units : 1;
+    if (s > most) s = most;
+    if (s > kblocks / 2) s = kblocks / 2;
+    return s < 1 ? 1 : static_cast<int>(s);
+}
+
 static int run(const Args& a, cudaStream_t st) {
-    const int kb = (a.K + BK - 1) / BK;
-    const int sms = sm_count();
-    if (a.groups == 0 && a.M <= 64) {
-        // few rows: weights on the TMEM lanes; the K blocks are split until two CTAs per multiprocessor are there
-        const int tiles = (a.N + 127) / 128;
-        int split = 2 * sms / tiles;
-        split = split < 1 ? 1 : split > 8 ? 8 : split;
-        if (split > kb) split = kb;
-        if (a.M <= 16) return launch<Cfg<16, true, true>>(a, split, st);
-        if (a.M <= 32) return launch<Cfg<32, true, true>>(a, split, st);
-        return launch<Cfg<64, true, true>>(a, split, st);
+    const int kb = (a.K + BK - 1) / BK, sms = sm_count();
+    const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256;
+    if (a.wgrad) return launch<Cfg<2, 256, false, BOTH>>(a, 1, st);
+    if (a.groups > 0) return launch<Cfg<2, 256, true, COL>>(a, 1, st);
+    if (a.M <= 64) {
+        // few rows: 128 weights a tile, two CTAs on a multiprocessor
+        const int split = split_for(n128, 2 * sms, kb, 8);
+        return a.b_square ? launch<Cfg<1, 64, true, COL>>(a, split, st) : launch<Cfg<1, 64, true, BOTH>>(a, split, st);
     }
-    const long long mt = (a.M + 127) / 128;
-    const long long t256 = mt * ((a.N + 255) / 256), t128 = mt * ((a.N + 127) / 128);
-    if (a.groups > 0 || t256 >= sms || a.N > 128) {
-        int split = 1;
-        if (a.groups == 0 && t256 * 2 <= sms) {
-            split = static_cast<int>(sms / t256);
-            if (split > 8) split = 8;
-            if (split > kb) split = kb;
-        }
-        return a.b_square ? launch<Cfg<256, false, false>>(a, split, st) : launch<Cfg<256, false, true>>(a, split, st);
-    }
-    int split = 1;
-    if (t128 * 2 <= sms) {
-        split = static_cast<int>(sms / t128);
-        if (split > 8) split = 8;
-        if (split > kb) split = kb;
-    }
-    return a.b_square ? launch<Cfg<128, false, false>>(a, split, st) : launch<Cfg<128, false, true>>(a, split, st);
+    const int split = split_for(m256 * n256, sms / 2, kb, 4);
+    if (!a.b_square) return launch<Cfg<2, 256, false, BOTH>>(a, split, st);
+    if (a.M <= 1024) return launch<Cfg<2, 256, true, COL>>(a, split, st);
+    return launch<Cfg<2, 256, false, ROW>>(a, split, st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {
