@@ -3,14 +3,19 @@
 // The scales are no powers of two and belong to 128 values of k, so the tensor core sums one block at a time (four
 // tcgen05.mma.kind::f8f6f4 of K = 32 into TMEM, fp32) and registers add the blocks up: acc += scale * partial, one rounding each.
 //
-// A CTA, or a pair of CTAs on one tile (cta_group::2), holds 128 rows of X each and up to TN rows of Y: warp 0 streams operand tiles
-// with TMA (128-byte swizzle) into a ring of stages, warp 1 issues the MMAs of block kb into one of two TMEM buffers, four or eight
-// warps read the buffer with tcgen05.ld, scale and add it into registers while the MMAs of block kb + 1 fill the other buffer, and at
-// the end write C.
+// A CTA, or a pair of CTAs on one tile (cta_group::2), holds 128 rows of X each and TN rows of Y:
+//   warp 0      streams operand tiles with TMA (128-byte swizzle) into a ring of stages
+//   warp 1      issues the MMAs of block kb into one of two TMEM buffers (leading CTA of a pair)
+//   warp 2      brings the block's scales into a ring of their own with 4-byte asynchronous copies, several blocks ahead
+//   4 .. 19     (or 4 .. 7) promote: each reads 32 lanes x 64 columns of the buffer, scales and adds them into registers while the
+//               MMAs of block kb + 1 fill the other buffer, and at the end writes its part of C
+// Sixteen promoting warps of 64 columns hide one another's waits; eight warps of 128 columns, with 232 registers each, took 1120
+// cycles a block, most of it in a chain of waits, against 512 of the MMAs.
 //
-// X is the operand whose rows are the lanes of TMEM, Y the one whose rows are its columns.  X = A, Y = B for many rows of A.  For few
-// rows, and for rows that belong to experts (SWAP), X = B: the weights fill the lanes and a tile has as many columns (a
-// multiple of 16 or 32) as there are tokens, so that ragged groups cost what they hold.
+// X is the operand whose rows are the lanes of TMEM, Y the one whose rows are its columns: X = A, Y = B.  For few rows of A (SWAP)
+// X = B: the weights fill the lanes and a tile has as many columns (a multiple of 16) as there are rows of A.
+// Scales that vary by lane cost a register; scales that vary by column have to reach every lane through shared memory, 128 bytes a
+// cycle, which is why squares (one scale per 128 columns) have a form of their own (ROW).
 // split > 1: `split` CTAs or pairs of one cluster share a tile, each takes a part of the K blocks, and the partial tiles are added
 // through distributed shared memory in rank order: no workspace, no atomics, the same result in every run.
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
@@ -27,45 +32,47 @@ constexpr int MAX_GROUPS = 256;
 constexpr int DEV_BAD_GROUPS = 17;            // device status: group sizes that do not fit the operands
 constexpr int DEV_SMEM_BASE = 18;             // device status: dynamic shared memory does not start on a 1024-byte boundary
 constexpr int RED_PITCH = 129;                // floats between columns of the tile that a split adds up
+constexpr int CW = 64;                        // columns of a promoting warp
+constexpr int EPI0 = 4;                       // the first promoting warp
 
-// where the two scales of a partial value vary inside a promoting warp
-enum Scales { ROW, COL, BOTH };               // by lane (Y's is one number), by column (X's is one number), by both
+// ROW: Y's scale is one number per 128 columns.  BOTH: it varies by column.
+enum Scales { ROW, BOTH };
 
 template <int CG_, int TN_, bool SWAP_, Scales SC_>
 struct Cfg {
     static constexpr int CG = CG_, TN = TN_;
     static constexpr bool SWAP = SWAP_;
     static constexpr Scales SC = SC_;
-    static constexpr int EPI = TN >= 128 ? 8 : 4;             // promoting warps
-    static constexpr int EPI0 = TN >= 128 ? 4 : 2;            // the first of them
+    static constexpr int EPI = TN / CW * 4;                   // promoting warps: four lane quadrants for each 64 columns
     static constexpr int THREADS = 32 * (EPI0 + EPI);
-    static constexpr int CW = TN / (EPI / 4);                 // most columns of a promoting warp
     static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN / CG * BK;
-    static constexpr int Y_BOX = SWAP ? (CG == 2 ? 32 : 16) : TN / CG;      // rows of Y per TMA copy: only boxes with tokens are fetched
+    static constexpr int Y_BOX = SWAP ? 16 : TN / CG;         // rows of Y per TMA copy: with SWAP only boxes with rows are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
     static constexpr int STAGES = TN == 256 ? 6 : 4;
     static constexpr int TMEM_COLS = 2 * TN;
-    static constexpr int EPI_BYTES = SWAP ? 2 * CW * 4 : 32 * 32 * 4;      // per warp: two buffers of column scales; 32 rows of 128 bytes of C
-    static constexpr int epi_off = STAGES * STAGE;
-    static constexpr int bar_off = epi_off + EPI * EPI_BYTES;
-    static constexpr int n_bars = 2 * STAGES + 4;
+    static constexpr int D = SC == ROW ? 8 : 4;               // blocks of scales in the ring
+    static constexpr int SLOT = 128 + (SC == ROW ? 4 : TN);   // floats: X's rows, then Y's columns (ROW: two numbers)
+    static constexpr int TURN = SWAP ? 0 : 32 * 32;           // per promoting warp: 32 rows of 32 bytes in which C is turned
+    static constexpr int turn_off = STAGES * STAGE;
+    static constexpr int ring_off = turn_off + EPI * TURN;
+    static constexpr int bar_off = ring_off + D * SLOT * 4;
+    static constexpr int n_bars = 2 * STAGES + 4 + 2 * D;     // full, empty; accumulator full[2], free[2]; scales full, free
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
-    static constexpr int PER_SM = TN >= 128 ? 1 : 2;
+    static constexpr int PER_SM = TN == 256 ? 1 : 2;
     static_assert(dynamic * PER_SM <= 232448 - 1024 * (PER_SM - 1), "shared memory budget exceeded");
     static_assert(TN * RED_PITCH * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
-    static_assert(2 * CW * 4 <= EPI_BYTES, "two buffers of column scales");
 };
 
 struct Params {
     int kblocks;                              // of K
-    int tiles_x, tiles_y, group_x;            // tile grid (tiles_y: dense and weight gradient), rasterisation
+    int tiles_x, tiles_y, group_x;            // tile grid (of one matrix), rasterisation
     int x_rows, y_rows;                       // rows of X and Y per matrix
     const float* xs;                          // scale of X's row r in block kb: xs[r + kb * xs_k], squares: xs[(r / 128) * kblocks + kb]
     long long xs_k;
     int xs_square;
-    const float* ys;                          // the same for Y (never squares with SWAP, squares only with ROW)
+    const float* ys;                          // the same for Y: squares with ROW, row blocks with BOTH
     long long ys_k;
     void* c;
     long long ldc;
@@ -79,8 +86,9 @@ struct Params {
 };
 
 struct Tile {
-    int x0, x_tma;                            // first row of X of this CTA: inside its matrix, in the tensor map
-    int y0, y_end, ncols;                     // first row of Y, one past the last, columns of the MMA (both CTAs together)
+    int x0, x_end;                            // first row of X of this CTA, one past the last row of the matrix or group
+    int y0, y_end, y_tma;                     // first row of Y inside its matrix, one past the tile's last, first row in the tensor map
+    int ncols;                                // columns of the MMA (both CTAs together)
     int k0, k1;                               // K blocks
     long long c_row;                          // first row of C of this tile's matrix
     int g;
@@ -98,7 +106,10 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     o.c_row = 0;
     o.k0 = 0;
     o.k1 = p.kblocks;
-    int first = 0, row0 = 0, rows = p.y_rows, tx, ty;
+    o.x0 = 0;
+    o.x_end = p.x_rows;
+    int first = 0, tiles_x = p.tiles_x;
+    o.y_tma = 0;
     if (p.groups > 0) {
         const int* firsts = seg + MAX_GROUPS + 1;
         int lo = 0, hi = p.groups - 1;                        // last group whose first tile is <= t: the one that has tile t
@@ -108,43 +119,30 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
         }
         o.g = lo;
         first = firsts[lo];
-    }
-    if constexpr (C::SWAP) {
-        // the tokens of a group in as few tiles as hold them, of equal width; a weight tile's token tiles one after the other
-        if (p.groups > 0) {
-            row0 = seg[o.g];
-            rows = seg[o.g + 1] - row0;
-        }
-        const int nt = (rows + C::TN - 1) / C::TN, width = round_cols<C::CG>((rows + nt - 1) / nt);
-        tx = (t - first) / nt;
-        ty = (t - first) - tx * nt;
-        o.y0 = row0 + ty * width;
-        o.y_end = min(o.y0 + width, row0 + rows);
-        o.x0 = tx * 128 * C::CG;
-        o.x_tma = o.x0 + o.g * p.x_rows;
-    } else {
-        // groups of `group_x` tile rows, column-major inside, so that CTAs running together share panels in L2
-        const int in_all = t - first, per = p.group_x * p.tiles_y;
-        const int grp = in_all / per, in = in_all - grp * per, n = min(p.group_x, p.tiles_x - grp * p.group_x);
-        tx = grp * p.group_x + in % n;
-        ty = in / n;
-        o.y0 = ty * C::TN;
-        o.y_end = min(o.y0 + C::TN, p.y_rows);
-        o.x0 = tx * 128 * C::CG;
-        o.x_tma = o.x0;
-        if (p.groups > 0) {                                   // weight gradient
-            o.k0 = seg[o.g] / BK;
-            o.k1 = seg[o.g + 1] / BK;
-            o.c_row = static_cast<long long>(o.g) * p.x_rows;
+        if (p.wgrad) {
+            o.k0 = seg[lo] / BK;
+            o.k1 = seg[lo + 1] / BK;
+            o.c_row = static_cast<long long>(lo) * p.x_rows;
+        } else {
+            o.x0 = seg[lo];
+            o.x_end = seg[lo + 1];
+            tiles_x = (o.x_end - o.x0 + 128 * C::CG - 1) / (128 * C::CG);
+            o.y_tma = lo * p.y_rows;
         }
     }
+    // groups of `group_x` tile rows, column-major inside, so that CTAs running together share panels in L2
+    const int in_all = t - first, per = p.group_x * p.tiles_y;
+    const int grp = in_all / per, in = in_all - grp * per, n = min(p.group_x, tiles_x - grp * p.group_x);
+    const int ty = in / n, tx = grp * p.group_x + in - ty * n;
+    o.x0 += (tx * C::CG + pair_rank) * 128;
+    o.y0 = ty * C::TN;
+    o.y_tma += o.y0;
+    o.y_end = min(o.y0 + C::TN, p.y_rows);
     o.ncols = round_cols<C::CG>(o.y_end - o.y0);
-    o.x0 += pair_rank * 128;
-    o.x_tma += pair_rank * 128;
     if (p.split > 1) {
-        const int n = o.k1 - o.k0, k0 = o.k0;
-        o.k0 = k0 + n * part / p.split;
-        o.k1 = k0 + n * (part + 1) / p.split;
+        const int nk = o.k1 - o.k0, k0 = o.k0;
+        o.k0 = k0 + nk * part / p.split;
+        o.k1 = k0 + nk * (part + 1) / p.split;
     }
     return o;
 }
@@ -172,15 +170,48 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+// 32 lanes x 16 columns
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// four bytes, global -> shared, asynchronously; `arrive_when_copied` arrives on `bar` once all of this thread's earlier copies landed
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void set_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void set_regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // Arrive on a barrier of the pair's leading CTA.  What it orders are TMEM reads, which tcgen05.fence::before_thread_sync covers; the
-// release.cluster form would also wait for the warp's outstanding global loads, once per K block (1.21 instead of 0.5 us a block).
-__device__ __forceinline__ void arrive_pair(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+// release.cluster form would also wait for the warp's outstanding global loads, once per K block (1.21 instead of 0.7 us a block).
+template <int CG>
+__device__ __forceinline__ void arrive_lane0(uint32_t addr, int lane) {      // predicated, so that the warp does not diverge
+    if constexpr (CG == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(addr), "r"(lane) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(addr), "r"(lane) : "memory");
+}
+
+// A whole warp waits: one probe, and the bounded wait only when it fails.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const AbortCtl& ab, int code) {
+    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, ab, code));
 }
 
 // Arrive on `bar` of this CTA, or of both CTAs of the pair that starts at cluster rank `first`, once this thread's MMAs are complete.
@@ -199,22 +230,22 @@ __device__ __forceinline__ void store_c(const Params& p, long long row, int col,
     else static_cast<uint16_t*>(p.c)[at] = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
-// One warp's 32 rows x CW columns of C (row = lane): turned through shared memory, 128 bytes of a row at a time, so that a store covers
-// whole 128-byte pieces of rows (16 bytes per lane).  The 16-byte piece k of row r lies in slot k ^ (r % 8): conflict-free both ways.
-template <int CW>
-__device__ __forceinline__ void write_rows(const Params& p, const uint64_t (&acc)[CW / 2], uint32_t stg, long long row0, int rows, int col0, int cols,
+// One warp's 32 rows x 64 columns of C (row = lane): turned through shared memory, 32 bytes of a row at a time, so that a store covers
+// whole sectors of rows (16 bytes per lane).  The 16-byte piece k of row r lies in slot k ^ ((r / 4) % 2): conflict-free both ways.
+__device__ __forceinline__ void write_rows(const Params& p, const uint64_t (&acc)[CW / 2], uint32_t turn, long long row0, int rows, int col0, int cols,
                                            int lane) {
-    const int esize = p.c_f32 ? 4 : 2, per = 128 / esize;                 // columns in 128 bytes
+    if (cols <= 0 || rows <= 0) return;
+    const int esize = p.c_f32 ? 4 : 2, per = 32 / esize;                  // columns in 32 bytes
     uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * esize;
     const long long pitch = p.ldc * esize;
     const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0;
-    const uint32_t put = stg + lane * 128 + ((lane & 7) << 4);
+    const uint32_t put = turn + lane * 32 + (((lane >> 2) & 1) << 4), get = turn + (lane >> 1) * 32 + (((lane ^ (lane >> 3)) & 1) << 4);
 #pragma unroll
-    for (int j = 0; j < CW; j += 32) {
-        if (!p.c_f32 && (j & 32)) continue;
+    for (int j = 0; j < CW; j += 8) {
+        if (!p.c_f32 && (j & 8)) continue;
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 2; ++k) {
             uint32_t w[4];
             if (p.c_f32) {
 #pragma unroll
@@ -228,19 +259,20 @@ __device__ __forceinline__ void write_rows(const Params& p, const uint64_t (&acc
         __syncwarp();
         if (wide && cols - j >= per) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3);
+            for (int i = 0; i < 2; ++i) {
+                const int r = i * 16 + (lane >> 1);
                 uint32_t w[4];
-                ld_shared_v4(stg + r * 128 + (((lane ^ r) & 7) << 4), w[0], w[1], w[2], w[3]);
-                if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 7) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                ld_shared_v4(get + i * 16 * 32, w[0], w[1], w[2], w[3]);
+                if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 1) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         } else {
-            const int left = cols - j - lane * (4 / esize);
+            // four rows at a time, a word per lane
+            const int word = lane & 7, left = cols - j - word * (4 / esize);
 #pragma unroll 1
-            for (int r = 0; r < rows; ++r) {
+            for (int r = lane >> 3; r < rows; r += 4) {
                 uint32_t w;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
-                uint8_t* to = c + r * pitch + j * esize + lane * 4;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * 32 + (((word >> 2) ^ ((r >> 2) & 1)) << 4) + (word & 3) * 4));
+                uint8_t* to = c + r * pitch + j * esize + word * 4;
                 if (p.c_f32) {
                     if (left >= 1) *reinterpret_cast<uint32_t*>(to) = w;
                 } else {
@@ -277,7 +309,7 @@ __device__ __forceinline__ void group_prefix(const Params& p, int* seg, int lane
         end += row;
         if (end > cap) bad = true;
         const int e = static_cast<int>(min(end, static_cast<long long>(cap))), b = static_cast<int>(min(end - n, static_cast<long long>(cap)));
-        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + C::TN - 1) / C::TN * p.tiles_x;
+        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + 128 * C::CG - 1) / (128 * C::CG) * p.tiles_y;
         int tt = nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -301,7 +333,7 @@ __device__ __forceinline__ void group_prefix(const Params& p, int* seg, int lane
 template <class C>
 __global__ void __launch_bounds__(C::THREADS, C::PER_SM)
 gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_y, const Params p) {
-    constexpr int CG = C::CG, S = C::STAGES;
+    constexpr int CG = C::CG, S = C::STAGES, D = C::D;
     // the swizzle counts from 1024-byte boundaries; with no static shared memory the dynamic part starts on one
     extern __shared__ __align__(1024) uint8_t base_ptr[];
     const uint32_t base = smem_u32(base_ptr);
@@ -310,8 +342,10 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         return;
     }
     const uint32_t full0 = base + C::bar_off, empty0 = full0 + S * 8, accfull0 = empty0 + S * 8, accfree0 = accfull0 + 16;
+    const uint32_t scfull0 = accfree0 + 16, scfree0 = scfull0 + D * 8;
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + C::misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + C::misc_off + 8);
+    float* ring = reinterpret_cast<float*>(base_ptr + C::ring_off);
     int* seg = reinterpret_cast<int*>(base_ptr + C::seg_off);
     const AbortCtl ab{abort_flag, p.status};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -330,6 +364,10 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             mbar_init(accfull0 + b * 8, 1);
             mbar_init(accfree0 + b * 8, C::EPI * CG);         // promoting warps of the pair, on the leading CTA's barrier
         }
+        for (int d = 0; d < D; ++d) {
+            mbar_init(scfull0 + d * 8, 32);                   // the lanes of warp 2
+            mbar_init(scfree0 + d * 8, C::EPI);
+        }
         fence_mbar_init();
         prefetch_tmap(&tm_x);
         prefetch_tmap(&tm_y);
@@ -347,43 +385,42 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_ptr, 0);
     const int num_tiles = p.groups > 0 ? __shfl_sync(0xFFFFFFFFu, seg[MAX_GROUPS + 1 + p.groups], 0) : p.tiles_x * p.tiles_y;
 
-    if (warp < C::EPI0) {
-        // with eight promoting warps three warpgroups run, launched with 168 registers a thread: 4 * 40 + 8 * 232 = 12 * 168
-        if constexpr (C::EPI == 8) set_regs_less<40>();
+    if (warp < EPI0) {
+        // with sixteen promoting warps five warpgroups run, launched with 96 registers a thread: 56 + 4 * 104 < 5 * 96
+        if constexpr (C::EPI == 16) set_regs_less<56>();
         if (warp == 0) {
-            // ------------------------------------------------------------ producer
+            // ------------------------------------------------------------ operands
             const bool leader = elect_one();
             uint32_t stage = 0, ph = 0;
             const uint32_t full_lead = CG == 2 ? map_to_cta(full0, first_rank) : full0;
             bool ok = true;
             for (int t = unit; t < num_tiles && ok; t += units) {
                 const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
-                const int ny = ti.ncols / CG, boxes = (ny + C::Y_BOX - 1) / C::Y_BOX;     // rows and copies of Y of this CTA
-                const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x_tma, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y0 + pair_rank * ny, 0);
+                const int ny = ti.ncols / CG;                 // rows of Y of this CTA
+                const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x0, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y_tma + pair_rank * ny, 0);
                 const int k0 = __shfl_sync(0xFFFFFFFFu, ti.k0, 0), k1 = __shfl_sync(0xFFFFFFFFu, ti.k1, 0);
-                const int nb = __shfl_sync(0xFFFFFFFFu, boxes, 0);
+                const int boxes = __shfl_sync(0xFFFFFFFFu, (ny + C::Y_BOX - 1) / C::Y_BOX, 0);
                 for (int kb = k0; kb < k1; ++kb) {
-                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty0 + stage * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY))) { ok = false; break; }
+                    if (!warp_wait(empty0 + stage * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
                     if (leader) {
-                        const uint32_t dst = base + stage * C::STAGE, bytes = C::X_BYTES + nb * C::Y_BOX * BK;
+                        const uint32_t dst = base + stage * C::STAGE, bytes = C::X_BYTES + boxes * C::Y_BOX * BK;
                         if (CG == 1 || pair_rank == 0) mbar_arrive_expect_tx(full0 + stage * 8, CG * bytes);
                         const uint32_t bar = full_lead + stage * 8;
-                        if constexpr (CG == 2) tma_load_2d_pair(dst, &tm_x, kb * BK, x0, bar);
-                        else tma_load_2d(dst, &tm_x, kb * BK, x0, bar);
+                        auto load = [&](uint32_t to, const CUtensorMap* m, int y) {
+                            if constexpr (CG == 2) tma_load_2d_pair(to, m, kb * BK, y, bar);
+                            else tma_load_2d(to, m, kb * BK, y, bar);
+                        };
+                        load(dst, &tm_x, x0);
 #pragma unroll
-                        for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i) {
-                            if (i >= nb) break;
-                            const uint32_t to = dst + C::X_BYTES + i * C::Y_BOX * BK;
-                            if constexpr (CG == 2) tma_load_2d_pair(to, &tm_y, kb * BK, y0 + i * C::Y_BOX, bar);
-                            else tma_load_2d(to, &tm_y, kb * BK, y0 + i * C::Y_BOX, bar);
-                        }
+                        for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i)
+                            if (i < boxes) load(dst + C::X_BYTES + i * C::Y_BOX * BK, &tm_y, y0 + i * C::Y_BOX);
                     }
                     __syncwarp();
                     if (++stage == S) { stage = 0; ph ^= 1; }
                 }
             }
         } else if (warp == 1 && pair_rank == 0) {
-            // ------------------------------------------------------------ MMA (leading CTA of a pair)
+            // ------------------------------------------------------------ MMA
             const bool leader = elect_one();
             uint32_t stage = 0, ph = 0, it = 0;
             bool ok = true;
@@ -392,9 +429,9 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 const int n = __shfl_sync(0xFFFFFFFFu, ti.k1 - ti.k0, 0);
                 const uint32_t idesc = idesc_e4m3(128 * CG, __shfl_sync(0xFFFFFFFFu, ti.ncols, 0));
                 for (int i = 0; i < n; ++i, ++it) {
-                    const uint32_t buf = it & 1, use = it >> 1;
-                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(full0 + stage * 8, ph, ab, DEV_TIMEOUT_FULL))) { ok = false; break; }
-                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(accfree0 + buf * 8, (use & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE))) { ok = false; break; }
+                    const uint32_t buf = it & 1;
+                    if (!warp_wait(full0 + stage * 8, ph, ab, DEV_TIMEOUT_FULL)) { ok = false; break; }
+                    if (!warp_wait(accfree0 + buf * 8, ((it >> 1) & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE)) { ok = false; break; }
                     tc_fence_after();
                     if (leader) {
                         const uint32_t x = desc_sw128_lo(base + stage * C::STAGE), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
@@ -403,131 +440,170 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                         tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
                         tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
                         tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
-                        commit<CG>(empty0 + stage * 8, first_rank);
                         commit<CG>(accfull0 + buf * 8, first_rank);
+                        commit<CG>(empty0 + stage * 8, first_rank);
                     }
                     __syncwarp();
                     if (++stage == S) { stage = 0; ph ^= 1; }
                 }
             }
+        } else if (warp == 2) {
+            // ------------------------------------------------------------ scales; rows and columns beyond the tile take the last one's
+            constexpr int NY = C::TN / 32;
+            uint32_t slot = 0, ph = 0;
+            bool ok = true;
+            for (int t = unit; t < num_tiles && ok; t += units) {
+                const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
+                // offsets instead of pointers for every copy: this warp has few registers
+                const int x_last = ti.x_end - 1 - lane, y_last = ti.y_end - 1 - lane;
+                const float *xk = p.xs + lane, *yk = p.ys + lane;
+                int x_off = ti.x0, y_off = ti.y0;
+                if (p.xs_square) xk += static_cast<long long>(min(ti.x0, p.x_rows - 1) / 128) * p.kblocks - lane;      // the tile's one number
+                xk += ti.k0 * p.xs_k;
+                if constexpr (C::SC == ROW) {
+                    const int nb = (p.y_rows + 127) / 128;                // lane 0, 1: the number of the tile's 128 columns
+                    yk += (static_cast<long long>(ti.g) * nb + min(ti.y0 / 128 + lane, nb - 1)) * p.kblocks + ti.k0 - lane;
+                } else {
+                    yk += ti.k0 * p.ys_k;
+                }
+                for (int kb = ti.k0; kb < ti.k1; ++kb) {
+                    if (!warp_wait(scfree0 + slot * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
+                    const uint32_t to = smem_u32(ring + slot * C::SLOT + lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(x_off + i * 32, x_last)));
+                    if constexpr (C::SC == ROW) {
+                        if (lane < 2) copy4(to + 512, yk);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NY; ++i)
+                            if (i * 32 < ti.ncols) copy4(to + 512 + i * 128, yk + min(y_off + i * 32, y_last));
+                    }
+                    xk += p.xs_k;
+                    yk += p.ys_k;
+                    arrive_when_copied(scfull0 + slot * 8);
+                    if (++slot == D) { slot = 0; ph ^= 1; }
+                }
+            }
         }
     } else {
         // ------------------------------------------------------------ promotion and C
-        if constexpr (C::EPI == 8) set_regs_more<232>();
-        const int ew = warp - C::EPI0, q = warp & 3, half = ew >> 2;    // TMEM lane quadrant, column half
-        float* stgf = reinterpret_cast<float*>(base_ptr + C::epi_off + ew * C::EPI_BYTES);
+        if constexpr (C::EPI == 16) set_regs_more<104>();
+        const int ew = warp - EPI0, q = warp & 3;                        // TMEM lane quadrant
+        const int col0 = (ew >> 2) * CW;
+        const uint32_t turn = base + C::turn_off + ew * C::TURN;
         const uint32_t free_lead = CG == 2 ? map_to_cta(accfree0, first_rank) : accfree0;
+        const uint32_t my_tmem = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
         const int r = q * 32 + lane;                                     // row of this CTA's tile
-        uint32_t it = 0;
+        uint32_t it = 0;                                                 // blocks of this CTA so far: buffer and ring slot follow from it
         bool ok = true;
+        const float* my_ring = ring + r;
         for (int t = unit; t < num_tiles && ok; t += units) {
-            const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
-            // this warp's columns; with tokens in the columns both halves get the same share
-            const int cw = C::EPI == 4 ? ti.ncols : C::SWAP ? ti.ncols / 2 : C::CW;
-            const int col0 = half * cw, mine = min(cw, ti.ncols - col0);  // <= 0: nothing
-            const uint32_t my_tmem = tmem + (static_cast<uint32_t>(q * 32) << 16) + col0;
-            // scales; rows and columns beyond the tile take the last one's
-            const int xr = min(ti.x0 + r, p.x_rows - 1);
-            const float* xs = p.xs;
-            if (p.xs_square) xs += (static_cast<long long>(ti.g) * ((p.x_rows + 127) / 128) + xr / 128) * p.kblocks;
-            else xs += xr;
-            const float* ys = p.ys;
-            int yc[C::CW / 32];
-            if constexpr (C::SC == ROW) {
-                ys += static_cast<long long>(min(ti.y0 + col0, p.y_rows - 1) / 128) * p.kblocks;
-            } else {
-#pragma unroll
-                for (int i = 0; i < C::CW / 32; ++i) yc[i] = min(ti.y0 + col0 + i * 32 + lane, ti.y_end - 1);
+            int blocks, mine;                                            // columns from this warp's first on; <= 0: it only takes part in the barriers
+            {
+                const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
+                blocks = ti.k1 - ti.k0;
+                mine = ti.ncols - col0;
             }
-            uint64_t acc[C::CW / 2];
+            uint64_t acc[CW / 2];
 #pragma unroll
-            for (int i = 0; i < C::CW / 2; ++i) acc[i] = 0;
-            float xn = 0.0f, yn = 0.0f, ycol[C::CW / 32];
-            auto fetch = [&](int kb) {
-                xn = __ldg(xs + kb * p.xs_k);
+            for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
+            float s = 0.0f;
+            auto row_scale = [&](uint32_t n) {                           // of the CTA's block n
+                ok = warp_wait(scfull0 + (n & (D - 1)) * 8, (n / D) & 1, ab, DEV_TIMEOUT_FULL);
+                s = my_ring[(n & (D - 1)) * C::SLOT];
                 if constexpr (C::SC == ROW) {
-                    yn = __ldg(ys + kb);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < C::CW / 32; ++i)
-                        if (i * 32 < mine) ycol[i] = __ldg(ys + kb * p.ys_k + yc[i]);
+                    s *= ring[(n & (D - 1)) * C::SLOT + 128 + (col0 >> 7)];
+                    __syncwarp();
+                    arrive_lane0<1>(scfree0 + (n & (D - 1)) * 8, lane);
                 }
             };
-            if (ti.k0 < ti.k1) fetch(ti.k0);
-            for (int kb = ti.k0; kb < ti.k1; ++kb, ++it) {
+            if (blocks > 0) row_scale(it);
+            for (; blocks > 0 && ok; --blocks) {
                 const uint32_t buf = it & 1;
-                float s = xn;
-                if constexpr (C::SC == ROW) {
-                    s *= yn;
-                } else {
-                    // two buffers: the other one may still be read by slower lanes of this warp
-#pragma unroll
-                    for (int i = 0; i < C::CW / 32; ++i)
-                        if (i * 32 < mine) stgf[buf * C::CW + i * 32 + lane] = C::SC == COL ? ycol[i] * xn : ycol[i];
-                    __syncwarp();
-                }
-                if (kb + 1 < ti.k1) fetch(kb + 1);
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL))) { ok = false; break; }
+                if (!warp_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
+                const uint32_t src = my_tmem + buf * C::TN;
                 const uint64_t ss = pair(__float_as_uint(s), __float_as_uint(s));
-                auto release = [&]() {                                   // the buffer's values are all in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if constexpr (CG == 2) arrive_pair(free_lead + buf * 8);
-                        else mbar_arrive(free_lead + buf * 8);
+                const float* cs = ring + (it & (D - 1)) * C::SLOT + 128 + col0;     // BOTH
+                auto add = [&](const uint32_t (&v)[16], int c) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        uint64_t a = pair(v[i], v[i + 1]), b = pair(v[i + 2], v[i + 3]);
+                        if constexpr (C::SC == BOTH) {
+                            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(cs + c + i);
+                            a = mul2(a, y.x);
+                            b = mul2(b, y.y);
+                        }
+                        acc[(c + i) / 2] = fma2(a, ss, acc[(c + i) / 2]);
+                        acc[(c + i) / 2 + 1] = fma2(b, ss, acc[(c + i) / 2 + 1]);
                     }
                 };
-                // the next 32 columns are on their way while these are added
-                constexpr int NB = C::EPI == 8 ? 2 : 1;
-                uint32_t v[NB][32];
-                if (mine > 0) tc_ld_32x32(my_tmem + buf * C::TN, v[0]);
-                else release();
+                if constexpr (C::SC == ROW) {
+                    // 64 columns in four loads, two in flight
+                    uint32_t va[16], vb[16];
+                    tc_ld16(src, va);
+                    tc_ld16(src + 16, vb);
+                    tc_wait16(va);
+                    tc_wait16(vb);
+                    add(va, 0);
+                    tc_ld16(src + 32, va);
+                    add(vb, 16);
+                    tc_ld16(src + 48, vb);
+                    tc_wait16(va);
+                    tc_wait16(vb);
+                    tc_fence_before();
+                    __syncwarp();
+                    arrive_lane0<CG>(free_lead + buf * 8, lane);         // the buffer's values are all in registers
+                    add(va, 32);
+                    add(vb, 48);
+                } else {
+                    // one in flight: the column scales want the registers
+                    uint32_t v[16];
 #pragma unroll
-                for (int c = 0; c < C::CW / 32; ++c) {
-                    if (c * 32 < mine) {
-                        tc_wait_ld(v[c % NB]);
-                        const bool more = c + 1 < C::CW / 32 && (c + 1) * 32 < mine;
-                        if (!more) release();
-                        else if (NB == 2) tc_ld_32x32(my_tmem + buf * C::TN + (c + 1) * 32, v[(c + 1) % NB]);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            uint64_t a = pair(v[c % NB][i], v[c % NB][i + 1]), b = pair(v[c % NB][i + 2], v[c % NB][i + 3]);
-                            uint64_t fa = ss, fb = ss;
-                            if constexpr (C::SC != ROW) {
-                                const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&stgf[buf * C::CW + c * 32 + i]);
-                                if constexpr (C::SC == BOTH) {
-                                    a = mul2(a, cs.x);
-                                    b = mul2(b, cs.y);
-                                } else {
-                                    fa = cs.x;
-                                    fb = cs.y;
-                                }
-                            }
-                            acc[c * 16 + i / 2] = fma2(a, fa, acc[c * 16 + i / 2]);
-                            acc[c * 16 + i / 2 + 1] = fma2(b, fb, acc[c * 16 + i / 2 + 1]);
+                    for (int c = 0; c < CW; c += 16) {
+                        if (C::SWAP && c >= mine) break;
+                        tc_ld16(src + c, v);
+                        tc_wait16(v);
+                        if (c + 16 == CW) {
+                            tc_fence_before();
+                            __syncwarp();
+                            arrive_lane0<CG>(free_lead + buf * 8, lane);
                         }
-                        if (NB == 1 && more) tc_ld_32x32(my_tmem + buf * C::TN + (c + 1) * 32, v[0]);
+                        add(v, c);
+                    }
+                    if (C::SWAP && mine <= CW - 16) {
+                        tc_fence_before();
+                        __syncwarp();
+                        arrive_lane0<CG>(free_lead + buf * 8, lane);
                     }
                 }
+                if constexpr (C::SC == BOTH) {
+                    __syncwarp();
+                    arrive_lane0<1>(scfree0 + (it & (D - 1)) * 8, lane);
+                }
+                ++it;
+                if (blocks > 1) row_scale(it);
             }
             if (!ok) break;
-            const int cols = min(mine, ti.y_end - ti.y0 - col0);          // that exist
+            int again = t;                                               // found anew: nothing of it has to stay in registers during the loop
+            asm volatile("" : "+r"(again));
+            const Tile ti = tile_at<C>(again, p, seg, pair_rank, part);
+            const int cols = min(CW, ti.y_end - ti.y0 - col0);            // that exist
             if (p.split > 1) {
                 // this CTA's MMAs are complete (its last accumulator arrived), so the stage ring is free
                 float* red = reinterpret_cast<float*>(base_ptr);
 #pragma unroll
-                for (int i = 0; i < C::CW; ++i)
+                for (int i = 0; i < CW; ++i)
                     if (i < cols) red[(col0 + i) * RED_PITCH + r] = half_of(acc[i / 2], i & 1);
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
                 if (ti.x0 + r < p.x_rows) {
 #pragma unroll
-                    for (int i = 0; i < C::CW; ++i)
+                    for (int i = 0; i < CW; ++i)
                         if (i < cols) store_c(p, ti.y0 + col0 + i, ti.x0 + r, half_of(acc[i / 2], i & 1));
                 }
             } else {
-                write_rows<C::CW>(p, acc, smem_u32(stgf), ti.c_row + ti.x0 + q * 32, min(32, p.x_rows - ti.x0 - q * 32), ti.y0 + col0, cols, lane);
+                write_rows(p, acc, turn, ti.c_row + ti.x0 + q * 32, min(32, ti.x_end - ti.x0 - q * 32), ti.y0 + col0, cols, lane);
             }
         }
     }
@@ -535,9 +611,9 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     if (p.split > 1) {
         __syncwarp();
         cluster_sync_all();
-        if (warp >= C::EPI0 && unit < num_tiles) {
+        if (warp >= EPI0 && unit < num_tiles) {
             const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-            const int ew = warp - C::EPI0, xn = min(128, p.x_rows - ti.x0), yn = ti.y_end - ti.y0;
+            const int ew = warp - EPI0, xn = min(128, p.x_rows - ti.x0), yn = ti.y_end - ti.y0;
             if constexpr (C::SWAP) {
                 // part k writes its share of the tile's columns (rows of C); a lane is a row of the tile (column of C)
                 const int c1 = yn * (part + 1) / p.split, r = (ew & 3) * 32 + lane;
@@ -567,6 +643,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         const uint64_t t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
     }
+    if (warp == 2) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
     tc_fence_before();
     // nobody leaves while its tile is read, its TMEM written or its barriers arrived on
@@ -604,11 +681,11 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     const bool grouped = a.groups > 0 && !a.wgrad;
     int rc;
     if (C::SWAP) {
-        if ((rc = operand_map(&mx, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
+        if ((rc = operand_map(&mx, a.B, a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
         if ((rc = operand_map(&my, a.A, a.M, a.K, a.lda, C::Y_BOX)) != MX8_OK) return rc;
     } else {
         if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, 128)) != MX8_OK) return rc;
-        if ((rc = operand_map(&my, a.B, a.N, a.K, a.ldb, C::Y_BOX)) != MX8_OK) return rc;
+        if ((rc = operand_map(&my, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, C::Y_BOX)) != MX8_OK) return rc;
     }
     Params p{};
     p.kblocks = (a.K + BK - 1) / BK;
@@ -642,7 +719,7 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     // tiles that there can be: with groups every one may add a partial tile
     long long tiles = static_cast<long long>(p.tiles_x) * p.tiles_y;
     if (a.wgrad) tiles *= a.groups;
-    else if (grouped) tiles += static_cast<long long>(p.tiles_x) * a.groups;
+    else if (grouped) tiles += static_cast<long long>(p.tiles_y) * a.groups;
     if (tiles > 0x7FFFFFFFll / 16) {
         note_cuda_error("gemm_block128", "more than 2^27 tiles");
         return MX8_ERR_LIMIT;
@@ -683,16 +760,11 @@ static int run(const Args& a, cudaStream_t st) {
     const int kb = (a.K + BK - 1) / BK, sms = sm_count();
     const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256;
     if (a.wgrad) return launch<Cfg<2, 256, false, BOTH>>(a, 1, st);
-    if (a.groups > 0) return launch<Cfg<2, 256, true, COL>>(a, 1, st);
-    if (a.M <= 64) {
-        // few rows: 128 weights a tile, two CTAs on a multiprocessor
-        const int split = split_for(n128, 2 * sms, kb, 8);
-        return a.b_square ? launch<Cfg<1, 64, true, COL>>(a, split, st) : launch<Cfg<1, 64, true, BOTH>>(a, split, st);
-    }
+    if (a.groups > 0) return launch<Cfg<2, 256, false, ROW>>(a, 1, st);
+    // few rows: 128 weights a tile, two CTAs on a multiprocessor
+    if (a.M <= 64) return launch<Cfg<1, 64, true, BOTH>>(a, split_for(n128, 2 * sms, kb, 8), st);
     const int split = split_for(m256 * n256, sms / 2, kb, 4);
-    if (!a.b_square) return launch<Cfg<2, 256, false, BOTH>>(a, split, st);
-    if (a.M <= 1024) return launch<Cfg<2, 256, true, COL>>(a, split, st);
-    return launch<Cfg<2, 256, false, ROW>>(a, split, st);
+    return a.b_square ? launch<Cfg<2, 256, false, ROW>>(a, split, st) : launch<Cfg<2, 256, false, BOTH>>(a, split, st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {
