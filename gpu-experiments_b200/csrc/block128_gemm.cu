@@ -6,7 +6,8 @@
 // A CTA, or a pair of CTAs on one tile (cta_group::2), holds 128 rows of X each and TN rows of Y:
 //   warp 0      streams operand tiles with TMA (128-byte swizzle) into a ring of stages
 //   warp 1      issues the MMAs of block kb into one of two TMEM buffers (leading CTA of a pair)
-//   warp 2      brings the block's scales into a ring of their own with 4-byte asynchronous copies, several blocks ahead
+//   warp 2      brings the scales into a ring of their own with 4-byte asynchronous copies, three blocks ahead, and arrives on the
+//               accumulator's barrier beside the MMAs' commit, so that the promoting warps wait once a block
 //   4 .. 19     (or 4 .. 7) promote: each reads 32 lanes x 64 columns of the buffer, scales and adds them into registers while the
 //               MMAs of block kb + 1 fill the other buffer, and at the end writes its part of C
 // Sixteen promoting warps of 64 columns hide one another's waits; eight warps of 128 columns, with 232 registers each, took 1120
@@ -50,13 +51,13 @@ struct Cfg {
     static constexpr int STAGE = X_BYTES + Y_BYTES;
     static constexpr int STAGES = TN == 256 ? 6 : 4;
     static constexpr int TMEM_COLS = 2 * TN;
-    static constexpr int D = SC == ROW ? 8 : 4;               // blocks of scales in the ring
+    static constexpr int D = 8;                               // blocks of scales in the ring
     static constexpr int SLOT = 128 + (SC == ROW ? 4 : TN);   // floats: X's rows, then Y's columns (ROW: two numbers)
     static constexpr int TURN = SWAP ? 0 : 32 * 32;           // per promoting warp: 32 rows of 32 bytes in which C is turned
     static constexpr int turn_off = STAGES * STAGE;
     static constexpr int ring_off = turn_off + EPI * TURN;
     static constexpr int bar_off = ring_off + D * SLOT * 4;
-    static constexpr int n_bars = 2 * STAGES + 4 + 2 * D;     // full, empty; accumulator full[2], free[2]; scales full, free
+    static constexpr int n_bars = 2 * STAGES + 4;             // full, empty; accumulator (and scales) full[2], accumulator free[2]
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
@@ -186,13 +187,13 @@ __device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
-// four bytes, global -> shared, asynchronously; `arrive_when_copied` arrives on `bar` once all of this thread's earlier copies landed
+// four bytes, global -> shared, asynchronously; groups of copies complete in order
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void arrive_when_copied(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int N>
 __device__ __forceinline__ void set_regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -342,7 +343,6 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         return;
     }
     const uint32_t full0 = base + C::bar_off, empty0 = full0 + S * 8, accfull0 = empty0 + S * 8, accfree0 = accfull0 + 16;
-    const uint32_t scfull0 = accfree0 + 16, scfree0 = scfull0 + D * 8;
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + C::misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + C::misc_off + 8);
     float* ring = reinterpret_cast<float*>(base_ptr + C::ring_off);
@@ -361,12 +361,8 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             mbar_init(empty0 + s * 8, 1);                     // one tcgen05.commit
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(accfull0 + b * 8, 1);
+            mbar_init(accfull0 + b * 8, 2);                   // the MMAs' commit and this CTA's scales
             mbar_init(accfree0 + b * 8, C::EPI * CG);         // promoting warps of the pair, on the leading CTA's barrier
-        }
-        for (int d = 0; d < D; ++d) {
-            mbar_init(scfull0 + d * 8, 32);                   // the lanes of warp 2
-            mbar_init(scfree0 + d * 8, C::EPI);
         }
         fence_mbar_init();
         prefetch_tmap(&tm_x);
@@ -449,15 +445,19 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             }
         } else if (warp == 2) {
             // ------------------------------------------------------------ scales; rows and columns beyond the tile take the last one's
+            // Block m's copies go into slot m % D after block m - 5 is complete on its barrier: the promoting warps have then released
+            // block m - 7 and finished block m - 8, the slot's last.  Block m - 3 is announced when its copies have landed; the wait
+            // for block m - 5 has made sure that this arrival counts for the right phase of the barrier they share.
+            static_assert(D == 8, "the distances above");
             constexpr int NY = C::TN / 32;
-            uint32_t slot = 0, ph = 0;
+            uint32_t m = 0;
             bool ok = true;
+            auto complete = [&](uint32_t n) { return warp_wait(accfull0 + (n & 1) * 8, (n >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL); };
             for (int t = unit; t < num_tiles && ok; t += units) {
                 const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
                 // offsets instead of pointers for every copy: this warp has few registers
                 const int x_last = ti.x_end - 1 - lane, y_last = ti.y_end - 1 - lane;
                 const float *xk = p.xs + lane, *yk = p.ys + lane;
-                int x_off = ti.x0, y_off = ti.y0;
                 if (p.xs_square) xk += static_cast<long long>(min(ti.x0, p.x_rows - 1) / 128) * p.kblocks - lane;      // the tile's one number
                 xk += ti.k0 * p.xs_k;
                 if constexpr (C::SC == ROW) {
@@ -466,23 +466,33 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 } else {
                     yk += ti.k0 * p.ys_k;
                 }
-                for (int kb = ti.k0; kb < ti.k1; ++kb) {
-                    if (!warp_wait(scfree0 + slot * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
-                    const uint32_t to = smem_u32(ring + slot * C::SLOT + lane);
+                for (int kb = ti.k0; kb < ti.k1; ++kb, ++m) {
+                    if (m >= 5 && !complete(m - 5)) { ok = false; break; }
+                    const uint32_t to = smem_u32(ring + (m & (D - 1)) * C::SLOT + lane);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(x_off + i * 32, x_last)));
+                    for (int i = 0; i < 4; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(ti.x0 + i * 32, x_last)));
                     if constexpr (C::SC == ROW) {
                         if (lane < 2) copy4(to + 512, yk);
                     } else {
 #pragma unroll
                         for (int i = 0; i < NY; ++i)
-                            if (i * 32 < ti.ncols) copy4(to + 512 + i * 128, yk + min(y_off + i * 32, y_last));
+                            if (i * 32 < ti.ncols) copy4(to + 512 + i * 128, yk + min(ti.y0 + i * 32, y_last));
                     }
+                    copies_commit();
                     xk += p.xs_k;
                     yk += p.ys_k;
-                    arrive_when_copied(scfull0 + slot * 8);
-                    if (++slot == D) { slot = 0; ph ^= 1; }
+                    if (m >= 3) {
+                        copies_wait<3>();
+                        __syncwarp();
+                        arrive_lane0<1>(accfull0 + ((m - 3) & 1) * 8, lane);
+                    }
                 }
+            }
+            copies_wait<0>();
+            for (uint32_t n = m < 3 ? 0 : m - 3; n < m && ok; ++n) {
+                if (n >= 2 && !complete(n - 2)) break;
+                __syncwarp();
+                arrive_lane0<1>(accfull0 + (n & 1) * 8, lane);
             }
         }
     } else {
@@ -507,30 +517,19 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             uint64_t acc[CW / 2];
 #pragma unroll
             for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
-            float s = 0.0f;
-            auto row_scale = [&](uint32_t n) {                           // of the CTA's block n
-                ok = warp_wait(scfull0 + (n & (D - 1)) * 8, (n / D) & 1, ab, DEV_TIMEOUT_FULL);
-                s = my_ring[(n & (D - 1)) * C::SLOT];
-                if constexpr (C::SC == ROW) {
-                    s *= ring[(n & (D - 1)) * C::SLOT + 128 + (col0 >> 7)];
-                    __syncwarp();
-                    arrive_lane0<1>(scfree0 + (n & (D - 1)) * 8, lane);
-                }
-            };
-            if (blocks > 0) row_scale(it);
-            for (; blocks > 0 && ok; --blocks) {
+            for (; blocks > 0; --blocks, ++it) {
                 const uint32_t buf = it & 1;
                 if (!warp_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t src = my_tmem + buf * C::TN;
-                const uint64_t ss = pair(__float_as_uint(s), __float_as_uint(s));
-                const float* cs = ring + (it & (D - 1)) * C::SLOT + 128 + col0;     // BOTH
+                const float* slot = my_ring + (it & (D - 1)) * C::SLOT;
+                uint64_t ss;
                 auto add = [&](const uint32_t (&v)[16], int c) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         uint64_t a = pair(v[i], v[i + 1]), b = pair(v[i + 2], v[i + 3]);
                         if constexpr (C::SC == BOTH) {
-                            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(cs + c + i);
+                            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(slot - r + 128 + col0 + c + i);
                             a = mul2(a, y.x);
                             b = mul2(b, y.y);
                         }
@@ -538,11 +537,18 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                         acc[(c + i) / 2 + 1] = fma2(b, ss, acc[(c + i) / 2 + 1]);
                     }
                 };
+                auto release = [&]() {                                   // the buffer's values are all in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    arrive_lane0<CG>(free_lead + buf * 8, lane);
+                };
                 if constexpr (C::SC == ROW) {
                     // 64 columns in four loads, two in flight
                     uint32_t va[16], vb[16];
                     tc_ld16(src, va);
                     tc_ld16(src + 16, vb);
+                    const float s = slot[0] * slot[128 + (col0 >> 7) - r];
+                    ss = pair(__float_as_uint(s), __float_as_uint(s));
                     tc_wait16(va);
                     tc_wait16(vb);
                     add(va, 0);
@@ -551,38 +557,25 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     tc_ld16(src + 48, vb);
                     tc_wait16(va);
                     tc_wait16(vb);
-                    tc_fence_before();
-                    __syncwarp();
-                    arrive_lane0<CG>(free_lead + buf * 8, lane);         // the buffer's values are all in registers
+                    release();
                     add(va, 32);
                     add(vb, 48);
                 } else {
                     // one in flight: the column scales want the registers
                     uint32_t v[16];
+                    if (mine > 0) tc_ld16(src, v);
+                    else release();
+                    const float s = slot[0];
+                    ss = pair(__float_as_uint(s), __float_as_uint(s));
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
-                        if (C::SWAP && c >= mine) break;
-                        tc_ld16(src + c, v);
+                        if (c >= mine) break;
+                        if (c) tc_ld16(src + c, v);
                         tc_wait16(v);
-                        if (c + 16 == CW) {
-                            tc_fence_before();
-                            __syncwarp();
-                            arrive_lane0<CG>(free_lead + buf * 8, lane);
-                        }
+                        if (c + 16 == CW || c + 16 >= mine) release();
                         add(v, c);
                     }
-                    if (C::SWAP && mine <= CW - 16) {
-                        tc_fence_before();
-                        __syncwarp();
-                        arrive_lane0<CG>(free_lead + buf * 8, lane);
-                    }
                 }
-                if constexpr (C::SC == BOTH) {
-                    __syncwarp();
-                    arrive_lane0<1>(scfree0 + (it & (D - 1)) * 8, lane);
-                }
-                ++it;
-                if (blocks > 1) row_scale(it);
             }
             if (!ok) break;
             int again = t;                                               // found anew: nothing of it has to stay in registers during the loop
@@ -643,7 +636,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         const uint64_t t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
     }
-    if (warp == 2) asm volatile("cp.async.wait_all;" ::: "memory");
+    if (warp == 2) copies_wait<0>();
     __syncwarp();
     tc_fence_before();
     // nobody leaves while its tile is read, its TMEM written or its barriers arrived on
