@@ -8,7 +8,11 @@
 // backward  normalised  dl = w (dw - sum_S w dw) on S;  otherwise  dl = p ([in S] dw - sum_S w dw);
 //           both + p (b - sum_e b p), b_e = dL E c_e / (k V^2).
 //
-// One warp owns a token; lane l holds experts l*VPL .. l*VPL + VPL - 1, so lane order is expert order and a ballot breaks ties.
+// One warp owns a token; lane l holds experts l*VPL .. l*VPL + VPL - 1.  The kernels are bound by instructions, not by memory (a token of
+// 256 experts is 512 bytes), so the selection works on 32-bit words that hold the value's order-preserving bits, cut to 22, and the
+// expert's number reversed in the other 10: all words differ, the larger word is the larger value or the lower expert, and one
+// redux.sync.max finds both.  bf16 values fit in the 22 bits; for fp32 the result is checked against the full values and rows in which
+// the cut bits decide (values within 2^-13 of each other) are selected again, slowly.
 // Sums over tokens are made in a fixed order (registers of a warp, then warps of a block, then blocks), never with floating-point
 // atomics: results do not change from run to run.
 #include <atomic>
@@ -94,6 +98,52 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// descending, by a network of compare-exchanges (19 of them for 8 words)
+template <int N>
+__device__ __forceinline__ void sort_words(uint32_t (&w)[N]) {
+    auto cx = [&](int i, int j) {
+        const uint32_t hi = max(w[i], w[j]), lo = min(w[i], w[j]);
+        w[i] = hi;
+        w[j] = lo;
+    };
+    if constexpr (N == 2) {
+        cx(0, 1);
+    } else if constexpr (N == 4) {
+        cx(0, 1); cx(2, 3); cx(0, 2); cx(1, 3); cx(1, 2);
+    } else if constexpr (N == 8) {
+        cx(0, 1); cx(2, 3); cx(4, 5); cx(6, 7);
+        cx(0, 2); cx(1, 3); cx(4, 6); cx(5, 7);
+        cx(1, 2); cx(5, 6);
+        cx(0, 4); cx(1, 5); cx(2, 6); cx(3, 7);
+        cx(2, 4); cx(3, 5);
+        cx(1, 2); cx(3, 4); cx(5, 6);
+    }
+}
+
+// k rounds on the full keys: the largest, the lowest lane that has it, the lowest of its experts that has it; lane j gets choice j
+template <int VPL>
+__device__ __noinline__ int select_slowly(uint32_t (&key)[VPL], int topk, int lane) {
+    int my_idx = -1;
+#pragma unroll 1
+    for (int j = 0; j < topk; ++j) {
+        uint32_t best = 0;
+        for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        if (top == 0) break;
+        const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+        int at = -1;
+        if (lane == owner) {
+            for (int i = VPL - 1; i >= 0; --i)
+                if (key[i] == top) at = i;
+            for (int i = 0; i < VPL; ++i)
+                if (i == at) key[i] = 0;
+        }
+        at = __shfl_sync(0xFFFFFFFFu, at, owner);
+        if (lane == j) my_idx = owner * VPL + at;
+    }
+    return my_idx;
+}
+
 __device__ __forceinline__ float loss_of(double dot, int n, int experts, int topk) {
     return n > 0 ? static_cast<float>(dot * experts / (static_cast<double>(topk) * n * n)) : 0.0f;
 }
@@ -134,17 +184,18 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
     for (long long t = static_cast<long long>(blockIdx.x) * WARPS + warp; t < p.tokens; t += static_cast<long long>(gridDim.x) * WARPS) {
         uint32_t key[VPL];
         float v[VPL];
+        const T* row = static_cast<const T*>(p.logits) + t * p.ld;
         const bool on = !p.mask || p.mask[t] != 0;
         uint32_t best = 0;
         if (on) {
-            load_row<T, VPL>(static_cast<const T*>(p.logits) + t * p.ld, lane, p.experts, p.vec != 0, v);
+            load_row<T, VPL>(row, lane, p.experts, p.vec != 0, v);
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
                 key[i] = key_of(v[i]);
                 best = max(best, key[i]);
             }
         }
-        uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
         if (top == 0) {                                    // masked, or every expert switched off
             if (lane < p.topk) {
                 p.idx[t * p.topk + lane] = -1;
@@ -165,34 +216,53 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
 #pragma unroll
         for (int i = 0; i < VPL; ++i) prob[i] += v[i] * inv;
         ++n_valid;
-        // k rounds: the largest head, the lowest lane that has it, the lowest of its experts that has it
-        int my_idx = -1;
-        uint32_t my_key = 0;
-        for (int j = 0; j < p.topk; ++j) {
-            if (j) top = __reduce_max_sync(0xFFFFFFFFu, best);
-            if (top == 0) break;                           // fewer live experts than choices
-            const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
-            int at = 0;
-            if (lane == owner) {
-                bool found = false;
-                best = 0;
+        int my_idx = -1;                                   // lane j: choice j
+        float my_val = -INFINITY;
+        uint32_t word[VPL];
 #pragma unroll
-                for (int i = 0; i < VPL; ++i) {
-                    if (!found && key[i] == top) {
-                        found = true;
-                        at = i;
-                        key[i] = 0;
-                    }
-                    best = max(best, key[i]);
-                }
+        for (int i = 0; i < VPL; ++i) word[i] = key[i] ? (key[i] & ~1023u) | static_cast<uint32_t>(1023 - lane * VPL - i) : 0u;
+        if constexpr (VPL <= 8) sort_words<VPL>(word);
+        for (int j = 0; j < p.topk; ++j) {
+            uint32_t head = word[0];
+            if constexpr (VPL > 8) {
+#pragma unroll
+                for (int i = 1; i < VPL; ++i) head = max(head, word[i]);
             }
-            at = __shfl_sync(0xFFFFFFFFu, at, owner);
-            if (lane == j) {
-                my_idx = owner * VPL + at;
-                my_key = top;
+            const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, head);
+            if (best == 0) break;                          // fewer live experts than choices
+            if (lane == j) my_idx = 1023 - static_cast<int>(best & 1023u);
+            if constexpr (VPL <= 8) {
+                const bool mine = head == best;
+#pragma unroll
+                for (int i = 0; i + 1 < VPL; ++i) word[i] = mine ? word[i + 1] : word[i];
+                word[VPL - 1] = mine ? 0u : word[VPL - 1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) word[i] = word[i] == best ? 0u : word[i];
             }
         }
-        float w = my_idx >= 0 ? expf(value_of(my_key) - mx) : 0.0f;
+        if (my_idx >= 0) my_val = to_float(row[my_idx]);
+        if constexpr (sizeof(T) == 4) {
+            // right unless the cut bits decide: the choices' full keys fall, with rising experts among equals, and as many keys of the row
+            // lie above the last choice as choices do
+            const uint32_t full = my_idx >= 0 ? key_of(my_val) : 0u;
+            const unsigned chosen = __ballot_sync(0xFFFFFFFFu, my_idx >= 0);
+            const int last = 31 - __clz(chosen);
+            const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, full, 1);
+            const int next_idx = __shfl_down_sync(0xFFFFFFFFu, my_idx, 1);
+            const bool wrong = lane < last && (full < next || (full == next && my_idx > next_idx));
+            const uint32_t low = __shfl_sync(0xFFFFFFFFu, full, last);
+            int above = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) above += key[i] > low;
+            above = __reduce_add_sync(0xFFFFFFFFu, above);
+            const int chosen_above = __popc(__ballot_sync(0xFFFFFFFFu, my_idx >= 0 && full > low));
+            if (__any_sync(0xFFFFFFFFu, wrong) || above != chosen_above) {
+                my_idx = select_slowly<VPL>(key, p.topk, lane);
+                my_val = my_idx >= 0 ? to_float(row[my_idx]) : -INFINITY;
+            }
+        }
+        float w = my_idx >= 0 ? expf(my_val - mx) : 0.0f;
         const float den = p.normalize ? warp_sum(w) : sum;
         w = my_idx >= 0 ? w / den : 0.0f;
         if (lane < p.topk) {
@@ -234,46 +304,63 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
     }
 }
 
-// Sums the blocks' partial counts and probabilities and makes the loss; one block.
-__global__ void __launch_bounds__(1024) router_finish_kernel(const FwdParams p, int blocks) {
-    __shared__ double scratch[32];
-    __shared__ double sum_p[1024];
-    __shared__ int sum_c[1024];
-    // thread (slice, e): with fewer than 1024 experts several slices of the blocks are summed side by side
-    const int slices = 1024 / p.experts;                   // >= 1
-    const int e = threadIdx.x % p.experts, slice = threadIdx.x / p.experts;
-    double s = 0;
-    int c = 0;
-    if (slice < slices) {
-        for (int b = slice; b < blocks; b += slices) {
-            s += p.part_prob[static_cast<size_t>(b) * p.experts + e];
-            c += p.part_count[static_cast<size_t>(b) * p.experts + e];
-        }
-        sum_p[threadIdx.x] = s;
-        sum_c[threadIdx.x] = c;
-    }
-    int n = 0;
-    if (threadIdx.x < 32) {
-        for (int b = threadIdx.x; b < blocks; b += 32) n += p.part_valid[b];
-        n = __reduce_add_sync(0xFFFFFFFFu, n);
-    }
-    __syncthreads();
+// Sums the blocks' partial counts and probabilities and makes the loss: one cluster of blocks, each with a share of the experts, 32
+// threads on each expert.
+constexpr int FINISH = 8;
+__global__ void __cluster_dims__(FINISH, 1, 1) __launch_bounds__(1024) router_finish_kernel(const FwdParams p, int blocks) {
+    __shared__ double sum_p[32][33];
+    __shared__ int sum_c[32][33];
+    __shared__ double dots[FINISH];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x;
     double dot = 0;
-    if (threadIdx.x < p.experts) {
-        s = 0;
-        c = 0;
-        for (int i = 0; i < slices; ++i) {
-            s += sum_p[i * p.experts + threadIdx.x];
-            c += sum_c[i * p.experts + threadIdx.x];
+    for (int e0 = rank * 32; e0 < p.experts; e0 += FINISH * 32) {
+        const int e = e0 + lane;                            // warps are slices of the blocks: consecutive experts in a load
+        double s = 0;
+        int c = 0;
+        if (e < p.experts) {
+#pragma unroll 4
+            for (int b = warp; b < blocks; b += 32) {
+                s += p.part_prob[static_cast<size_t>(b) * p.experts + e];
+                c += p.part_count[static_cast<size_t>(b) * p.experts + e];
+            }
         }
-        p.counts[threadIdx.x] = c;
-        p.prob_sum[threadIdx.x] = static_cast<float>(s);
-        dot = s * c;
+        sum_p[warp][lane] = s;
+        sum_c[warp][lane] = c;
+        __syncthreads();
+        s = sum_p[lane][warp];                              // now warp = expert, lane = slice
+        c = sum_c[lane][warp];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        c = __reduce_add_sync(0xFFFFFFFFu, c);
+        if (lane == 0 && e0 + warp < p.experts) {
+            p.counts[e0 + warp] = c;
+            p.prob_sum[e0 + warp] = static_cast<float>(s);
+            dot += s * c;
+        }
+        __syncthreads();
     }
-    dot = block_sum(dot, scratch);
-    if (threadIdx.x == 0) {
-        *p.num_valid = n;
-        *p.loss = loss_of(dot, n, p.experts, p.topk);
+    if (lane == 0) sum_p[1][warp] = dot;                    // its experts' share
+    __syncthreads();
+    if (warp == 0) {
+        dot = sum_p[1][lane];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, o);
+        if (lane == 0) {
+            const uint32_t to = map_to_cta(smem_u32(&dots[rank]), 0);
+            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(dot) : "memory");
+        }
+    }
+    cluster_sync_all();
+    if (rank == 0 && warp == 0) {
+        int n = 0;
+        for (int b = lane; b < blocks; b += 32) n += p.part_valid[b];
+        n = __reduce_add_sync(0xFFFFFFFFu, n);
+        if (lane == 0) {
+            dot = 0;
+            for (int i = 0; i < FINISH; ++i) dot += dots[i];
+            *p.num_valid = n;
+            *p.loss = loss_of(dot, n, p.experts, p.topk);
+        }
     }
 }
 
@@ -305,9 +392,8 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) router_bwd_kernel(const BwdPar
     __syncwarp();
     float b[VPL];
     {
-        const int n = *p.num_valid;
-        const float g = p.d_loss ? *p.d_loss : 0.0f;
-        const float f = n > 0 ? g * static_cast<float>(static_cast<double>(p.experts) / (static_cast<double>(p.topk) * n * n)) : 0.0f;
+        const float n = static_cast<float>(*p.num_valid), g = p.d_loss ? *p.d_loss : 0.0f;
+        const float f = n > 0.0f ? g * (static_cast<float>(p.experts) / (static_cast<float>(p.topk) * n)) / n : 0.0f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) b[i] = p.d_loss && lane * VPL + i < p.experts ? f * static_cast<float>(p.counts[lane * VPL + i]) : 0.0f;
     }
@@ -347,7 +433,7 @@ __global__ void __launch_bounds__(BWD_WARPS * 32) router_bwd_kernel(const BwdPar
                     inner = wdw;
                     dot += s;
                 }
-                if (idx >= 0) atomicAdd(&row[idx], inner);
+                if (idx >= 0) row[idx] = inner;            // a token's choices are distinct
                 __syncwarp();
             }
 #pragma unroll
@@ -585,7 +671,7 @@ extern "C" int mx8_router_topk(const void* logits, int dtype, long long ld, int 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = dtype == MX8_T_F32 ? router::dispatch_fwd<float>(p, vpl, grid, st) : router::dispatch_fwd<uint16_t>(p, vpl, grid, st);
     if (e == cudaSuccess && grid > 1) {
-        router::router_finish_kernel<<<1, 1024, 0, st>>>(p, grid);
+        router::router_finish_kernel<<<router::FINISH, 1024, 0, st>>>(p, grid);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) {

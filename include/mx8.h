@@ -272,7 +272,8 @@ MX8_API int mx8_router_topk(const void* logits, int dtype, long long ld, int tok
                             void* num_valid, void* balance_loss, void* workspace, size_t workspace_bytes, void* stream);
 
 /* d_logits [tokens][experts] (type of logits, contiguous) from the gradients of topk_weights (float [tokens][topk]) and of
- * balance_loss (float [1]); either may be NULL (zero), not both.  The other arguments are mx8_router_topk's inputs and outputs.
+ * balance_loss (float [1]); either may be NULL (zero), not both.  The other arguments are mx8_router_topk's inputs and outputs (the ids
+ * of a token that are not -1 are distinct).
  * The counts are constants, as they have no derivative.  counts and num_valid may have been summed over ranks before the call: the
  * gradient is then that of the loss over all of them.  Tokens that took no part get zeros, and entries of d_topk_weights at
  * choices with id -1 are not read. */
