@@ -6,10 +6,12 @@
 // reciprocal, one of the product (fp32, half a step of 2^-23 each), then the rounding to 3 bits that the format asks for.
 // A block that holds an infinity or NaN gets that as its scale and dequantizes to NaN.
 //
-// Bound by HBM: x is read once for both orientations.  A block of 8 warps owns a 128 x 128 tile; a warp loads 16 rows into
-// registers (lane = 4 columns, 16 loads in flight per lane), takes row maxima with redux.sync and column maxima through 4 KB of
-// shared memory; row bytes leave as 128 consecutive bytes per warp store, transposed bytes through a swizzled 16 KB tile as 16-byte
-// pieces of 128-byte rows.
+// Bound by HBM once the instructions are few: x is read once for both orientations.  A block of 8 warps owns a 128 x 128 tile.  Half a
+// warp spans a row (8 columns per lane, 16-byte loads), a lane holds 8 rows of its 8 columns, so that maxima are taken on packed
+// pairs of bf16, products on pairs of fp32 (mul.f32x2), and a lane's rows are 8 consecutive bytes of the transpose.  Row maxima by four
+// shuffles within the half warp, column maxima through 4 KB of shared memory; row bytes leave as 128 consecutive bytes per half warp, the
+// transpose through a swizzled 16 KB tile as 16-byte pieces of 128-byte rows.  The first form (4 columns x 16 rows a lane, scalar maxima
+// and products, 1700 instructions a warp) took 137 us for 16391 x 7168 gathered rows both ways, at 65 % of the issue slots.
 #include "mx8_host.cuh"
 #include "mx8_ptx.cuh"
 
@@ -38,189 +40,264 @@ struct Params {
     int vec_x, vec_q, vec_t;
 };
 
-template <typename T> struct Four;                 // four consecutive elements of a row as loaded
-template <> struct Four<uint16_t> {
-    uint32_t w[2];
-    __device__ float get(int i) const { return __uint_as_float((i & 1) ? (w[i >> 1] & 0xFFFF0000u) : (w[i >> 1] << 16)); }
-    __device__ void zero() { w[0] = w[1] = 0; }
-    __device__ void load(const uint16_t* p) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        w[0] = v.x; w[1] = v.y;
-    }
-    __device__ void set(int i, uint16_t v) { w[i >> 1] |= static_cast<uint32_t>(v) << (16 * (i & 1)); }
-};
-template <> struct Four<float> {
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+// product of two pairs of floats
+__device__ __forceinline__ void mul2(uint64_t a, uint64_t b, float& lo, float& hi) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    lo = __uint_as_float(static_cast<uint32_t>(d));
+    hi = __uint_as_float(static_cast<uint32_t>(d >> 32));
+}
+__device__ __forceinline__ uint64_t twice(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
+// the larger magnitude of two bf16 pairs, two floats; a NaN wins; the sign bits are arbitrary
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t max_f32(uint32_t a, uint32_t b) {
+    float d;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(d) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(d);
+}
+
+// eight consecutive elements of a row as loaded: WORDS words, and the magnitudes' maxima as MAXES words (bf16: a pair in each)
+template <typename T> struct Eight;
+template <> struct Eight<uint16_t> {
+    static constexpr int WORDS = 4;
     uint32_t w[4];
-    __device__ float get(int i) const { return __uint_as_float(w[i]); }
-    __device__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
-    __device__ void load(const float* p) {
+    __device__ __forceinline__ uint64_t two(int j) const { return pair(w[j] << 16, w[j] & 0xFFFF0000u); }
+    __device__ __forceinline__ void load(const uint16_t* p) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     }
-    __device__ void set(int i, float v) { w[i] = __float_as_uint(v); }
+    __device__ __forceinline__ void set(int i, uint16_t v) { w[i >> 1] |= static_cast<uint32_t>(v) << (16 * (i & 1)); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max_bf16x2(a, b); }
+};
+template <> struct Eight<float> {
+    static constexpr int WORDS = 8;
+    uint32_t w[8];
+    __device__ __forceinline__ uint64_t two(int j) const { return pair(w[2 * j], w[2 * j + 1]); }
+    __device__ __forceinline__ void load(const float* p) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p)), u = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        w[4] = u.x; w[5] = u.y; w[6] = u.z; w[7] = u.w;
+    }
+    __device__ __forceinline__ void set(int i, float v) { w[i] = __float_as_uint(v); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max_f32(a, b); }
 };
 
-__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }   // orders |v|, NaN on top
+// magnitude of a block from its maximum's bits: sign off, the floor (an unsigned comparison keeps infinities and NaN on top)
+__device__ __forceinline__ float amax_of(uint32_t bits) { return __uint_as_float(max(bits & 0x7FFFFFFFu, AMAX_FLOOR)); }
 __device__ __forceinline__ uint32_t four_bytes(float a, float b, float c, float d) { return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16); }
 
 // SQUARE: one scale for the tile; otherwise ROW / COL say which orientations have scales of their own
 template <typename T, bool ROW, bool COL, bool SQUARE>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_block128_kernel(const Params p) {
+    using E8 = Eight<T>;
+    constexpr bool BF = sizeof(T) == 2;
+    constexpr int W = E8::WORDS;
     __shared__ alignas(16) uint8_t stage[COL ? B * B : 16];
-    __shared__ uint32_t cmax[COL && !SQUARE ? WARPS * B : WARPS];
+    __shared__ alignas(16) uint32_t cmax[COL && !SQUARE ? WARPS * 16 * W : WARPS];
     __shared__ alignas(16) float cinv[B];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_e = p.tiles_m * p.tiles_n;
-    const int e = blockIdx.x / per_e, t = blockIdx.x - e * per_e;
-    const int grp = t / (GROUP_M * p.tiles_n), in_grp = t - grp * (GROUP_M * p.tiles_n);
-    const int rows_in = min(GROUP_M, p.tiles_m - grp * GROUP_M);
-    const int tm = grp * GROUP_M + in_grp % rows_in, tn = in_grp / rows_in;
-    const int m0 = tm * B + warp * ROWS, n0 = tn * B + lane * 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l16 = lane & 15;
+    // grid (GROUP_M * tiles_n, groups of tile rows, E): consecutive blocks walk down GROUP_M tile rows, then along N
+    const int e = blockIdx.z, tn = blockIdx.x / GROUP_M, tm = blockIdx.y * GROUP_M + blockIdx.x % GROUP_M;
+    if (tm >= p.tiles_m) return;
+    const int m0 = tm * B + warp * ROWS + half * 8, n0 = tn * B + l16 * 8;      // this lane's first row and column
 
-    Four<T> v[ROWS];
-    const T* x = static_cast<const T*>(p.x) + static_cast<long long>(e) * p.M * p.ldx;
-    int src = 0;
-    if (lane < ROWS) {
-        src = m0 + lane < p.M ? m0 + lane : -1;
-        if (p.row_index && src >= 0) {
-            src = p.row_index[src];
-            if (src >= p.src_rows) src = -1;
-        }
-    }
+    E8 v[8];
+    {
+        const T* x = static_cast<const T*>(p.x) + static_cast<long long>(e) * p.M * p.ldx + n0;
+        const bool whole = p.vec_x && n0 + 8 <= p.N;
+        if (!p.row_index && p.vec_x && tm * B + B <= p.M && tn * B + B <= p.N) {
+            x += static_cast<long long>(m0) * p.ldx;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        v[r].zero();
-        const int s = __shfl_sync(0xFFFFFFFFu, src, r);
-        if (s >= 0) {
-            const T* row = x + s * p.ldx + n0;
-            if (p.vec_x && n0 + 4 <= p.N) {
-                v[r].load(row);
-            } else {
+            for (int r = 0; r < 8; ++r) v[r].load(x + r * p.ldx);
+        } else {
+            int src = m0 + (lane & 7) < p.M ? m0 + (lane & 7) : -1;
+            if (p.row_index && src >= 0) {
+                src = p.row_index[src];
+                if (src >= p.src_rows) src = -1;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n0 + i < p.N) v[r].set(i, row[i]);
+            for (int r = 0; r < 8; ++r) {
+                const int s = __shfl_sync(0xFFFFFFFFu, src, r, 16);
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[r].w[i] = 0;
+                const T* row = x + s * p.ldx;
+                if (s >= 0) {
+                    if (whole) {
+                        v[r].load(row);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (n0 + i < p.N) v[r].set(i, row[i]);
+                    }
+                }
             }
         }
     }
 
-    float row_inv = 0.0f;                          // lane r < 16: reciprocal scale of row r
+    float row_inv = 0.0f;                          // lanes r and r + 8 of a half: reciprocal scale of its row r
     float tile_inv = 0.0f;
     if constexpr (SQUARE) {
-        uint32_t a = 0;
+        uint32_t a = v[0].w[0];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r)
+        for (int r = 0; r < 8; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a = max(a, mag(v[r].get(i)));
+            for (int i = 0; i < W; ++i)
+                if (r || i) a = E8::larger(a, v[r].w[i]);
+        a &= BF ? 0x7FFF7FFFu : 0x7FFFFFFFu;
+        if constexpr (BF) a = max(a & 0xFFFF0000u, a << 16);
         a = __reduce_max_sync(0xFFFFFFFFu, a);
         if (lane == 0) cmax[warp] = a;
         __syncthreads();
-        a = AMAX_FLOOR;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) a = max(a, cmax[w]);
-        tile_inv = __fdiv_rn(448.0f, __uint_as_float(a));
+        const float amax = amax_of(a);
+        tile_inv = __fdiv_rn(448.0f, amax);
         if (threadIdx.x == 0) {
-            const float s = __fdiv_rn(__uint_as_float(a), 448.0f);
+            const float s = __fdiv_rn(amax, 448.0f);
             if (ROW) p.sc[(static_cast<size_t>(e) * p.tiles_m + tm) * p.tiles_n + tn] = s;
             if (COL) p.sc_t[(static_cast<size_t>(e) * p.tiles_n + tn) * p.tiles_m + tm] = s;
         }
     } else if constexpr (ROW) {
-        uint32_t mine = AMAX_FLOOR;
+        // bf16: rows 2i and 2i + 1 share a word; then four exchanges within the half warp
+        constexpr int K = BF ? 4 : 8;
+        uint32_t m[K];
+        if constexpr (BF) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            uint32_t a = mag(v[r].get(0));
+            for (int i = 0; i < 4; ++i) {
+                uint32_t a = max_bf16x2(max_bf16x2(v[2 * i].w[0], v[2 * i].w[1]), max_bf16x2(v[2 * i].w[2], v[2 * i].w[3]));
+                uint32_t b = max_bf16x2(max_bf16x2(v[2 * i + 1].w[0], v[2 * i + 1].w[1]), max_bf16x2(v[2 * i + 1].w[2], v[2 * i + 1].w[3]));
+                m[i] = max_bf16x2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+            }
+        } else {
 #pragma unroll
-            for (int i = 1; i < 4; ++i) a = max(a, mag(v[r].get(i)));
-            a = __reduce_max_sync(0xFFFFFFFFu, a);
-            if (lane == r) mine = max(mine, a);
+            for (int r = 0; r < 8; ++r) {
+                m[r] = v[r].w[0];
+#pragma unroll
+                for (int i = 1; i < W; ++i) m[r] = max_f32(m[r], v[r].w[i]);
+            }
         }
-        row_inv = __fdiv_rn(448.0f, __uint_as_float(mine));
-        if (lane < ROWS && m0 + lane < p.M)
-            p.sc[(static_cast<size_t>(e) * p.tiles_n + tn) * p.M + m0 + lane] = __fdiv_rn(__uint_as_float(mine), 448.0f);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < K; ++i) m[i] = E8::larger(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], o));
+        uint32_t mine = m[0];
+#pragma unroll
+        for (int i = 1; i < K; ++i)
+            if (((lane & 7) >> (BF ? 1 : 0)) == i) mine = m[i];
+        if constexpr (BF) mine = (lane & 1) ? mine & 0xFFFF0000u : mine << 16;
+        const float amax = amax_of(mine);
+        row_inv = __fdiv_rn(448.0f, amax);
+        if (l16 < 8 && m0 + l16 < p.M) p.sc[(static_cast<size_t>(e) * p.tiles_n + tn) * p.M + m0 + l16] = __fdiv_rn(amax, 448.0f);
     }
     if constexpr (ROW) {
         uint8_t* q = p.q + (static_cast<long long>(e) * p.M + m0) * p.ld + n0;
+        const bool whole = p.vec_q && n0 + 8 <= p.N, inside = m0 + 8 <= p.M;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const float inv = SQUARE ? tile_inv : __shfl_sync(0xFFFFFFFFu, row_inv, r);
-            if (m0 + r >= p.M) break;
-            const uint32_t b = four_bytes(v[r].get(0) * inv, v[r].get(1) * inv, v[r].get(2) * inv, v[r].get(3) * inv);
-            if (p.vec_q && n0 + 4 <= p.N) {
-                *reinterpret_cast<uint32_t*>(q + r * p.ld) = b;
-            } else {
+        for (int r = 0; r < 8; ++r) {
+            const uint64_t inv = twice(SQUARE ? tile_inv : __shfl_sync(0xFFFFFFFFu, row_inv, r, 16));
+            float f[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n0 + i < p.N) q[r * p.ld + i] = static_cast<uint8_t>(b >> (8 * i));
+            for (int j = 0; j < 4; ++j) mul2(v[r].two(j), inv, f[2 * j], f[2 * j + 1]);
+            const uint32_t lo = four_bytes(f[0], f[1], f[2], f[3]), hi = four_bytes(f[4], f[5], f[6], f[7]);
+            if (inside || m0 + r < p.M) {
+                if (whole) {
+                    *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (n0 + i < p.N) q[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+                }
             }
+            q += p.ld;
         }
     }
     if constexpr (COL) {
-        float inv[4];
+        uint64_t inv[4];
         if constexpr (SQUARE) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) inv[i] = tile_inv;
+            for (int j = 0; j < 4; ++j) inv[j] = twice(tile_inv);
         } else {
-            uint32_t a[4] = {0, 0, 0, 0};
+            uint32_t a[W];
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r)
+            for (int i = 0; i < W; ++i) {
+                a[i] = v[0].w[i];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = max(a[i], mag(v[r].get(i)));
-            *reinterpret_cast<uint4*>(&cmax[warp * B + lane * 4]) = make_uint4(a[0], a[1], a[2], a[3]);
-            __syncthreads();
-            if (threadIdx.x < B) {
-                uint32_t m = AMAX_FLOOR;
+                for (int r = 1; r < 8; ++r) a[i] = E8::larger(a[i], v[r].w[i]);
+                a[i] = E8::larger(a[i], __shfl_xor_sync(0xFFFFFFFFu, a[i], 16));
+            }
+            if (half == 0) {
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) m = max(m, cmax[w * B + threadIdx.x]);
-                cinv[threadIdx.x] = __fdiv_rn(448.0f, __uint_as_float(m));
-                const int n = tn * B + threadIdx.x;
-                if (n < p.N) p.sc_t[(static_cast<size_t>(e) * p.tiles_m + tm) * p.N + n] = __fdiv_rn(__uint_as_float(m), 448.0f);
+                for (int i = 0; i < W; i += 4) *reinterpret_cast<uint4*>(&cmax[(warp * 16 + l16) * W + i]) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);
             }
             __syncthreads();
-            const float4 c = *reinterpret_cast<const float4*>(&cinv[lane * 4]);
-            inv[0] = c.x; inv[1] = c.y; inv[2] = c.z; inv[3] = c.w;
+            if (threadIdx.x < B) {
+                const int c = threadIdx.x;
+                uint32_t m = cmax[BF ? c >> 1 : c];
+#pragma unroll
+                for (int w = 1; w < WARPS; ++w) m = E8::larger(m, cmax[w * 16 * W + (BF ? c >> 1 : c)]);
+                if constexpr (BF) m = (c & 1) ? m & 0xFFFF0000u : m << 16;
+                const float amax = amax_of(m);
+                cinv[c] = __fdiv_rn(448.0f, amax);
+                if (tn * B + c < p.N) p.sc_t[(static_cast<size_t>(e) * p.tiles_m + tm) * p.N + tn * B + c] = __fdiv_rn(amax, 448.0f);
+            }
+            __syncthreads();
+            const ulonglong2 c0 = *reinterpret_cast<const ulonglong2*>(&cinv[l16 * 8]), c1 = *reinterpret_cast<const ulonglong2*>(&cinv[l16 * 8 + 4]);
+            inv[0] = c0.x; inv[1] = c0.y; inv[2] = c1.x; inv[3] = c1.y;
         }
-        // column c: 16-byte piece `warp` of its 128 bytes goes to slot warp ^ ((c / 4) % 8): the eight lanes of a quarter warp
-        // write, and read, eight different slots
+        // the 8-byte piece k = 2 warp + half of column c's 128 bytes lies in slot k ^ (c / 8): sixteen lanes write sixteen different slots
+        const int slot = (2 * warp + half) ^ l16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+        for (int j = 0; j < 4; ++j) {
+            float f[8], g[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                w[j] = four_bytes(v[4 * j].get(i) * inv[i], v[4 * j + 1].get(i) * inv[i], v[4 * j + 2].get(i) * inv[i], v[4 * j + 3].get(i) * inv[i]);
-            *reinterpret_cast<uint4*>(stage + (lane * 4 + i) * B + ((warp ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int r = 0; r < 8; ++r) mul2(v[r].two(j), inv[j], f[r], g[r]);
+            st_shared_v2(smem_u32(stage) + (l16 * 8 + 2 * j) * B + slot * 8, four_bytes(f[0], f[1], f[2], f[3]), four_bytes(f[4], f[5], f[6], f[7]));
+            st_shared_v2(smem_u32(stage) + (l16 * 8 + 2 * j + 1) * B + slot * 8, four_bytes(g[0], g[1], g[2], g[3]), four_bytes(g[4], g[5], g[6], g[7]));
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < ROWS / 4; ++k) {
-            const int c = warp * ROWS + k * 4 + (lane >> 3), piece = lane & 7;
+            const int c = warp * ROWS + k * 4 + (lane >> 3), piece = lane & 7, g = c >> 3;
             const int n = tn * B + c, m = tm * B + piece * 16;
             if (n >= p.N || m >= p.M) continue;
-            const uint4 w = *reinterpret_cast<const uint4*>(stage + c * B + ((piece ^ ((c >> 2) & 7)) << 4));
+            uint32_t w[4];
+            ld_shared_v4(smem_u32(stage) + c * B + ((piece ^ (g >> 1)) << 4), w[0], w[1], w[2], w[3]);
+            if (g & 1) {                               // the two 8-byte pieces of the 16 lie the other way round
+                const uint32_t a = w[0], b = w[1];
+                w[0] = w[2]; w[1] = w[3]; w[2] = a; w[3] = b;
+            }
             uint8_t* dst = p.qt + (static_cast<long long>(e) * p.N + n) * p.ld_t + m;
             if (p.vec_t && m + 16 <= p.M) {
-                *reinterpret_cast<uint4*>(dst) = w;
+                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (m + i < p.M) dst[i] = static_cast<uint8_t>(ws[i >> 2] >> (8 * (i & 3)));
+                    if (m + i < p.M) dst[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
             }
         }
     }
 }
 
+template <typename T, bool ROW, bool COL, bool SQUARE>
+static cudaError_t launch_one(const Params& p, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(GROUP_M * p.tiles_n), static_cast<unsigned>((p.tiles_m + GROUP_M - 1) / GROUP_M), static_cast<unsigned>(p.E));
+    quantize_block128_kernel<T, ROW, COL, SQUARE><<<grid, 32 * WARPS, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
 template <typename T>
 static cudaError_t launch(const Params& p, bool row, bool col, bool square, cudaStream_t st) {
-    const unsigned grid = static_cast<unsigned>(p.E) * p.tiles_m * p.tiles_n;
-    if (square) {
-        if (row && col) quantize_block128_kernel<T, true, true, true><<<grid, 32 * WARPS, 0, st>>>(p);
-        else if (row) quantize_block128_kernel<T, true, false, true><<<grid, 32 * WARPS, 0, st>>>(p);
-        else quantize_block128_kernel<T, false, true, true><<<grid, 32 * WARPS, 0, st>>>(p);
-    } else {
-        if (row && col) quantize_block128_kernel<T, true, true, false><<<grid, 32 * WARPS, 0, st>>>(p);
-        else if (row) quantize_block128_kernel<T, true, false, false><<<grid, 32 * WARPS, 0, st>>>(p);
-        else quantize_block128_kernel<T, false, true, false><<<grid, 32 * WARPS, 0, st>>>(p);
-    }
-    return cudaGetLastError();
+    if (square) return row && col ? launch_one<T, true, true, true>(p, st) : row ? launch_one<T, true, false, true>(p, st) : launch_one<T, false, true, true>(p, st);
+    return row && col ? launch_one<T, true, true, false>(p, st) : row ? launch_one<T, true, false, false>(p, st) : launch_one<T, false, true, false>(p, st);
 }
 
 }  // namespace q128
@@ -241,8 +318,8 @@ extern "C" int mx8_quantize_block128(const void* x, int dtype, int E, int M, int
     if (reinterpret_cast<uintptr_t>(x) % esize || reinterpret_cast<uintptr_t>(sc) % 4 || reinterpret_cast<uintptr_t>(sc_t) % 4 ||
         reinterpret_cast<uintptr_t>(row_index) % 4) return MX8_ERR_ALIGN;
     const long long tiles_m = (M + 127ll) / 128, tiles_n = (N + 127ll) / 128;
-    if (tiles_m * tiles_n > 0x7FFFFFFFll / E) {
-        note_cuda_error("mx8_quantize_block128", "more than 2^31 - 1 tiles of 128 x 128");
+    if (tiles_m > 65535ll * q128::GROUP_M || E > 65535) {
+        note_cuda_error("mx8_quantize_block128", "more than 65535 matrices or 67107840 rows");
         return MX8_ERR_LIMIT;
     }
     int rc = check_device_sm100();
@@ -261,8 +338,8 @@ extern "C" int mx8_quantize_block128(const void* x, int dtype, int E, int M, int
     p.qt = static_cast<uint8_t*>(fp8_t);
     p.ld_t = ld_t;
     p.sc_t = static_cast<float*>(sc_t);
-    p.vec_x = ldx % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * esize) == 0;
-    p.vec_q = ld % 4 == 0 && reinterpret_cast<uintptr_t>(fp8) % 4 == 0;
+    p.vec_x = (ldx * esize) % 16 == 0 && aligned16(x);
+    p.vec_q = ld % 8 == 0 && reinterpret_cast<uintptr_t>(fp8) % 8 == 0;
     p.vec_t = ld_t % 16 == 0 && aligned16(fp8_t);
     const cudaError_t e = dtype == MX8_T_F32 ? q128::launch<float>(p, row, col, square != 0, static_cast<cudaStream_t>(stream))
                                              : q128::launch<uint16_t>(p, row, col, square != 0, static_cast<cudaStream_t>(stream));
