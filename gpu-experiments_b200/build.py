@@ -15,6 +15,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(OUT_DIR, "libmx8.so")
 SOURCES = ["mx8_host.cu", "quantize.cu", "gemm.cu", "moe_schedule.cu", "moe_combine.cu", "moe_layer.cu", "host_pipeline.cu", "shared_expert.cu", "peak_probe.cu",
            "router.cu", "block128_quantize.cu", "block128_gemm.cu"]
+TORCH_SOURCES = ["torch_binding.cpp", "torch_block128_router.cpp"]
 HEADERS = ["mx8_host.cuh", "mx8_ptx.cuh", "mx8_qmath.cuh", os.path.join("..", "..", "include", "mx8.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
@@ -61,19 +62,32 @@ def torch_binding_path():
 
 
 def build_torch_binding(force=False, verbose=False):
-    """Compile csrc/torch_binding.cpp into the pybind11/torch module mx8/_C (links libmx8.so)."""
+    """Compile csrc/torch_*.cpp into the pybind11/torch module mx8/_C (links libmx8.so)."""
     import sysconfig
 
     from torch.utils import cpp_extension as ce
     build(force=False, verbose=verbose)
-    src = os.path.join(CSRC, "torch_binding.cpp")
     out = torch_binding_path()
-    if not (force or _stale(out, [src, os.path.join(HERE, "..", "include", "mx8.h"), LIB])):
+    hdr = os.path.join(HERE, "..", "include", "mx8.h")
+    srcs = [os.path.join(CSRC, s) for s in TORCH_SOURCES]
+    if not (force or _stale(out, srcs + [hdr, LIB])):
         return out
     inc = ce.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
     libdirs = ce.library_paths()
-    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-            src, "-o", out] + ["-I" + i for i in inc] + ["-L" + d for d in libdirs]
+    objs, running = [], []
+    for src in srcs:
+        o = os.path.join(OBJ_DIR, os.path.basename(src).replace(".cpp", ".o"))
+        objs.append(o)
+        if force or _stale(o, [src, hdr]):
+            cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H", "-c", src, "-o", o]
+                   + ["-I" + i for i in inc])
+            if verbose:
+                print(" ".join(cmd))
+            running.append((cmd, subprocess.Popen(cmd)))
+    for cmd, proc in running:
+        if proc.wait():
+            raise subprocess.CalledProcessError(proc.returncode, cmd)
+    cmd = (["g++", "-shared", "-o", out] + objs + ["-L" + d for d in libdirs]
            + ["-L" + OUT_DIR, "-lmx8", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
            + ["-Wl,-rpath," + d for d in libdirs])
     if verbose:

@@ -381,6 +381,8 @@ int device_status() {
 
 }  // namespace
 
+void bind_block128_router(pybind11::module_& m);      // torch_block128_router.cpp
+
 PYBIND11_MODULE(_C, m) {
     m.doc() = "mx8: MXFP8 quantize and block-scaled GEMM for sm_100a (host layer over the C ABI in include/mx8.h)";
     m.def("mxfp8_quantize", &mxfp8_quantize_out, "", pybind11::arg("x_bf16"), pybind11::arg("x_fp8"), pybind11::arg("x_sc"),
@@ -404,6 +406,7 @@ PYBIND11_MODULE(_C, m) {
     m.def("bwd_prologue", &bwd_prologue);
     m.def("bwd_epilogue", &bwd_epilogue);
     m.def("dispatch_mlp_swiglu_combine_bwd", &dispatch_mlp_swiglu_combine_bwd);
+    bind_block128_router(m);
     m.def("device_status", &device_status);
     m.def("version", []() { return std::string(mx8_version()); });
 }

@@ -145,6 +145,22 @@ def load():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The C++ host module (csrc/torch_*.cpp), imported on first use."""
+    global _host
+    if _host is None:
+        load()
+        try:
+            from . import _C
+        except ImportError as e:
+            raise ImportError(f"mx8._C is missing or does not load ({e}): build it with `python gpu-experiments_b200/build.py --torch`") from e
+        _host = _C
+    return _host
+
+
 def check(code, where):
     if code != OK:
         raise Mx8Error(code, where)

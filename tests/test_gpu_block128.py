@@ -177,6 +177,14 @@ def test_product_into_and_from_slices():
     check_c(c, a64[100:140], b64)
 
 
+def test_one_row_needs_no_pitch():
+    qa, sa, qb, sb, a64, b64 = operands(1, 50, 200, "square", seed=5)
+    alone = bits(qa).view(torch.float8_e4m3fn)                     # 200 bytes, contiguous
+    c = torch.empty(1, 50, device=DEV)
+    mx8.gemm_block128(alone, sa, qb, sb, c)
+    check_c(c, a64, b64)
+
+
 def test_non_finite_blocks_reach_their_rows_only():
     qa, sa, qb, sb, a64, b64 = operands(200, 300, 256, "square", seed=4)
     sa[1, 7] = float("nan")
