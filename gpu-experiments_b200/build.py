@@ -88,7 +88,7 @@ def build_torch_binding(force=False, verbose=False):
         if proc.wait():
             raise subprocess.CalledProcessError(proc.returncode, cmd)
     cmd = (["g++", "-shared", "-o", out] + objs + ["-L" + d for d in libdirs]
-           + ["-L" + OUT_DIR, "-lmx8", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           + ["-L" + OUT_DIR, "-lmx8", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
            + ["-Wl,-rpath," + d for d in libdirs])
     if verbose:
         print(" ".join(cmd))

@@ -47,50 +47,78 @@ struct FwdParams {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
 
-// lane's VPL consecutive logits; experts beyond the row's end read as -inf
+// A lane's VPL consecutive logits as they lie in memory (bf16: two to a word; a single one in the low half); experts beyond the row's
+// end are -inf.
 template <typename T, int VPL>
-__device__ __forceinline__ void load_row(const T* row, int lane, int experts, bool vec, float (&v)[VPL]) {
-    const int e0 = lane * VPL;
-    constexpr int BYTES = VPL * static_cast<int>(sizeof(T));
-    if (BYTES >= 4 && vec) {              // VPL divides the row length: a lane is whole or empty
-        if (e0 < experts) {
-            constexpr int W = BYTES >= 16 ? 4 : (BYTES / 4 > 0 ? BYTES / 4 : 1);      // words per load
-            uint32_t w[BYTES >= 4 ? BYTES / 4 : 1];
+struct Row {
+    static constexpr int BYTES = VPL * static_cast<int>(sizeof(T));
+    static constexpr int WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* row, int lane, int experts, bool vec) {
+        const int e0 = lane * VPL;
+        constexpr uint32_t NONE = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+        if (BYTES >= 4 && vec) {              // VPL divides the row length: a lane is whole or empty
             const uint8_t* src = reinterpret_cast<const uint8_t*>(row + e0);
+            if (e0 >= experts) {
 #pragma unroll
-            for (int i = 0; i < BYTES / 4; i += W) {
-                if constexpr (W == 4) {
+                for (int i = 0; i < WORDS; ++i) w[i] = NONE;
+            } else if constexpr (BYTES >= 16) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i += 4) {
                     const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + 4 * i));
                     w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
-                } else if constexpr (W == 2) {
-                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + 4 * i));
-                    w[i] = x.x; w[i + 1] = x.y;
-                } else {
-                    w[i] = __ldg(reinterpret_cast<const uint32_t*>(src + 4 * i));
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
-                else v[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+            } else if constexpr (BYTES == 8) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(src));
+                w[0] = x.x; w[1] = x.y;
+            } else {
+                w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) v[i] = -INFINITY;
+            for (int i = 0; i < VPL; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    w[i] = e0 + i < experts ? __float_as_uint(row[e0 + i]) : NONE;
+                } else {
+                    const uint32_t v = e0 + i < experts ? static_cast<uint32_t>(row[e0 + i]) : 0xFF80u;
+                    w[i / 2] = (i & 1) ? w[i / 2] | (v << 16) : v | (VPL == 1 ? 0xFF800000u : 0u);
+                }
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) v[i] = e0 + i < experts ? to_float(row[e0 + i]) : -INFINITY;
     }
-}
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return __uint_as_float((i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    }
+};
 
-// order-preserving key of a logit: 0 for -inf (switched off), NaN above everything, -0 equal to +0
+// Order-preserving bits of a logit: adding +0 makes -0 equal to +0 and every NaN the positive one, which lies above +inf; -inf gives
+// 0x007FFFFF (bf16: 0x007F), below all that is finite: words under LIVE are switched-off experts.
+constexpr uint32_t LIVE = 0x00800000u;
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t u = __float_as_uint(v + 0.0f);
-    const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return v != v ? 0xFFFFFFFFu : (u == 0xFF800000u ? 0u : k);
+    return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); }
+
+// the selection's words (see above) of a lane's experts
+template <typename T, int VPL>
+__device__ __forceinline__ void words_of(const Row<T, VPL>& row, int lane, uint32_t (&word)[VPL]) {
+    const uint32_t code = 1023u - lane * VPL;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) word[i] = (key_of(row.get(i)) & ~1023u) | (code - i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; i += 2) {
+            uint32_t w;
+            asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(row.w[i / 2]), "r"(0u));
+            w ^= ((w >> 15) & 0x00010001u) * 0x7FFFu ^ 0x80008000u;
+            word[i] = (w << 16) + (code - i);
+            if (i + 1 < VPL) word[i + 1] = (w & 0xFFFF0000u) + (code - i - 1);
+        }
+    }
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -121,23 +149,27 @@ __device__ __forceinline__ void sort_words(uint32_t (&w)[N]) {
 }
 
 // k rounds on the full keys: the largest, the lowest lane that has it, the lowest of its experts that has it; lane j gets choice j
-template <int VPL>
-__device__ __noinline__ int select_slowly(uint32_t (&key)[VPL], int topk, int lane) {
+template <typename T, int VPL>
+__device__ __noinline__ int select_slowly(const T* row, int experts, int topk, int lane) {
     int my_idx = -1;
+    uint32_t taken = 0;                                    // of this lane's experts
 #pragma unroll 1
     for (int j = 0; j < topk; ++j) {
         uint32_t best = 0;
-        for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-        if (top == 0) break;
-        const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
-        int at = -1;
-        if (lane == owner) {
-            for (int i = VPL - 1; i >= 0; --i)
-                if (key[i] == top) at = i;
-            for (int i = 0; i < VPL; ++i)
-                if (i == at) key[i] = 0;
+        int at = 0;
+#pragma unroll 1
+        for (int i = 0; i < VPL; ++i) {
+            const int e = lane * VPL + i;
+            const uint32_t k = e < experts && !((taken >> i) & 1u) ? key_of(to_float(row[e])) : 0u;
+            if (k > best) {
+                best = k;
+                at = i;
+            }
         }
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
+        if (top < LIVE) break;
+        const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
+        if (lane == owner) taken |= 1u << at;
         at = __shfl_sync(0xFFFFFFFFu, at, owner);
         if (lane == j) my_idx = owner * VPL + at;
     }
@@ -168,6 +200,7 @@ struct Shape {
 template <typename T, int VPL>
 __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(const FwdParams p) {
     constexpr int WARPS = Shape<VPL>::WARPS;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");        // the finishing kernel may be brought up beside this one
     extern __shared__ float smem[];
     float* warp_prob = smem;                                               // [WARPS][experts]
     int* count = reinterpret_cast<int*>(smem + WARPS * p.experts);         // [experts]
@@ -181,58 +214,72 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
 #pragma unroll
     for (int i = 0; i < VPL; ++i) prob[i] = 0.0f;
     int n_valid = 0;
-    for (long long t = static_cast<long long>(blockIdx.x) * WARPS + warp; t < p.tokens; t += static_cast<long long>(gridDim.x) * WARPS) {
-        uint32_t key[VPL];
-        float v[VPL];
-        const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-        const bool on = !p.mask || p.mask[t] != 0;
-        uint32_t best = 0;
-        if (on) {
-            load_row<T, VPL>(row, lane, p.experts, p.vec != 0, v);
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                key[i] = key_of(v[i]);
-                best = max(best, key[i]);
-            }
+    // the next token's logits are on their way while this one is worked on (a masked token's are fetched too, and dropped)
+    const int step = gridDim.x * WARPS;
+    int t = blockIdx.x * WARPS + warp;
+    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+    Row<T, VPL> next;
+    uint8_t next_on = 1;
+    if (t < p.tokens) {
+        next.load(row, lane, p.experts, p.vec != 0);
+        if (p.mask) next_on = p.mask[t];
+    }
+    for (; t < p.tokens; t += step, row += step * p.ld) {
+        const Row<T, VPL> in = next;
+        const bool on = next_on != 0;
+        if (p.tokens - t > step) {
+            next.load(row + step * p.ld, lane, p.experts, p.vec != 0);
+            if (p.mask) next_on = p.mask[t + step];
         }
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
-        if (top == 0) {                                    // masked, or every expert switched off
+        const size_t out = static_cast<size_t>(t) * p.topk + lane;
+        // the largest logit; bf16: the first choice's word has all of it
+        uint32_t word[VPL];
+        words_of<T, VPL>(in, lane, word);
+        uint32_t top;
+        if constexpr (sizeof(T) == 4) {
+            top = key_of(in.get(0));
+#pragma unroll
+            for (int i = 1; i < VPL; ++i) top = max(top, key_of(in.get(i)));
+            top = __reduce_max_sync(0xFFFFFFFFu, top);
+        }
+        if constexpr (VPL <= 8) sort_words<VPL>(word);
+        auto head_of = [&]() {
+            uint32_t h = word[0];
+            if constexpr (VPL > 8) {
+#pragma unroll
+                for (int i = 1; i < VPL; ++i) h = max(h, word[i]);
+            }
+            return h;
+        };
+        uint32_t best = __reduce_max_sync(0xFFFFFFFFu, head_of());
+        if constexpr (sizeof(T) == 2) top = best & 0xFFFF0000u;
+        if (!on || best < LIVE) {                          // masked, or every expert switched off
             if (lane < p.topk) {
-                p.idx[t * p.topk + lane] = -1;
-                p.weights[t * p.topk + lane] = 0.0f;
+                p.idx[out] = -1;
+                p.weights[out] = 0.0f;
             }
             if (lane == 0) p.lse[t] = -INFINITY;
             continue;
         }
-        const float mx = value_of(top);
-        float sum = 0.0f;
+        const float mx = sizeof(T) == 4 ? value_of(top) : __uint_as_float(__float_as_uint(value_of(top)) & 0xFFFF0000u);
+        float v[VPL], sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            v[i] = expf(v[i] - mx);
+            v[i] = expf(in.get(i) - mx);
             sum += v[i];
         }
         sum = warp_sum(sum);
-        const float inv = 1.0f / sum;
+        const float inv = __fdividef(1.0f, sum);
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) prob[i] += v[i] * inv;
+        for (int i = 0; i < VPL; ++i) prob[i] = fmaf(v[i], inv, prob[i]);
         ++n_valid;
         int my_idx = -1;                                   // lane j: choice j
-        float my_val = -INFINITY;
-        uint32_t word[VPL];
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) word[i] = key[i] ? (key[i] & ~1023u) | static_cast<uint32_t>(1023 - lane * VPL - i) : 0u;
-        if constexpr (VPL <= 8) sort_words<VPL>(word);
         for (int j = 0; j < p.topk; ++j) {
-            uint32_t head = word[0];
-            if constexpr (VPL > 8) {
-#pragma unroll
-                for (int i = 1; i < VPL; ++i) head = max(head, word[i]);
-            }
-            const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, head);
-            if (best == 0) break;                          // fewer live experts than choices
+            if (j) best = __reduce_max_sync(0xFFFFFFFFu, head_of());
+            if (best < LIVE) break;                        // fewer live experts than choices
             if (lane == j) my_idx = 1023 - static_cast<int>(best & 1023u);
             if constexpr (VPL <= 8) {
-                const bool mine = head == best;
+                const bool mine = word[0] == best;
 #pragma unroll
                 for (int i = 0; i + 1 < VPL; ++i) word[i] = mine ? word[i + 1] : word[i];
                 word[VPL - 1] = mine ? 0u : word[VPL - 1];
@@ -241,36 +288,35 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
                 for (int i = 0; i < VPL; ++i) word[i] = word[i] == best ? 0u : word[i];
             }
         }
-        if (my_idx >= 0) my_val = to_float(row[my_idx]);
+        float my_val = my_idx >= 0 ? to_float(row[my_idx]) : 0.0f;
         if constexpr (sizeof(T) == 4) {
             // right unless the cut bits decide: the choices' full keys fall, with rising experts among equals, and as many keys of the row
             // lie above the last choice as choices do
             const uint32_t full = my_idx >= 0 ? key_of(my_val) : 0u;
             const unsigned chosen = __ballot_sync(0xFFFFFFFFu, my_idx >= 0);
             const int last = 31 - __clz(chosen);
-            const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, full, 1);
-            const int next_idx = __shfl_down_sync(0xFFFFFFFFu, my_idx, 1);
-            const bool wrong = lane < last && (full < next || (full == next && my_idx > next_idx));
+            const uint32_t after = __shfl_down_sync(0xFFFFFFFFu, full, 1);
+            const int after_idx = __shfl_down_sync(0xFFFFFFFFu, my_idx, 1);
+            const bool wrong = lane < last && (full < after || (full == after && my_idx > after_idx));
             const uint32_t low = __shfl_sync(0xFFFFFFFFu, full, last);
             int above = 0;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) above += key[i] > low;
+            for (int i = 0; i < VPL; ++i) above += key_of(in.get(i)) > low;
             above = __reduce_add_sync(0xFFFFFFFFu, above);
             const int chosen_above = __popc(__ballot_sync(0xFFFFFFFFu, my_idx >= 0 && full > low));
             if (__any_sync(0xFFFFFFFFu, wrong) || above != chosen_above) {
-                my_idx = select_slowly<VPL>(key, p.topk, lane);
-                my_val = my_idx >= 0 ? to_float(row[my_idx]) : -INFINITY;
+                my_idx = select_slowly<T, VPL>(row, p.experts, p.topk, lane);
+                my_val = my_idx >= 0 ? to_float(row[my_idx]) : 0.0f;
             }
         }
         float w = my_idx >= 0 ? expf(my_val - mx) : 0.0f;
-        const float den = p.normalize ? warp_sum(w) : sum;
-        w = my_idx >= 0 ? w / den : 0.0f;
+        w *= p.normalize ? __fdividef(1.0f, warp_sum(w)) : inv;
         if (lane < p.topk) {
-            p.idx[t * p.topk + lane] = my_idx;
-            p.weights[t * p.topk + lane] = w;
+            p.idx[out] = my_idx;
+            p.weights[out] = my_idx >= 0 ? w : 0.0f;
             if (my_idx >= 0) atomicAdd(&count[my_idx], 1);
         }
-        if (lane == 0) p.lse[t] = mx + logf(sum);
+        if (lane == 0) p.lse[t] = mx + __logf(sum);
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
@@ -313,6 +359,8 @@ __global__ void __cluster_dims__(FINISH, 1, 1) __launch_bounds__(1024) router_fi
     __shared__ double dots[FINISH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x;
     double dot = 0;
+    // launched while the forward kernel still runs: from here on its results are there
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int e0 = rank * 32; e0 < p.experts; e0 += FINISH * 32) {
         const int e = e0 + lane;                            // warps are slices of the blocks: consecutive experts in a load
         double s = 0;
@@ -382,67 +430,76 @@ struct BwdParams {
 
 constexpr int BWD_WARPS = 8;
 
+template <int VPL>
+__host__ __device__ constexpr int bwd_blocks() { return VPL <= 8 ? 5 : VPL == 16 ? 3 : 1; }      // resident per multiprocessor
+
 template <typename T, int VPL>
-__global__ void __launch_bounds__(BWD_WARPS * 32) router_bwd_kernel(const BwdParams p) {
-    extern __shared__ float smem[];                        // per warp: a row of gradients at the chosen experts, zero elsewhere
+__global__ void __launch_bounds__(BWD_WARPS * 32, bwd_blocks<VPL>()) router_bwd_kernel(const BwdParams p) {
+    // b of every expert; per warp: gradients at the chosen experts, zero elsewhere.  Expert lane * VPL + i lies at i * 32 + lane: no two
+    // lanes of a read share a bank.
+    extern __shared__ float smem[];
+    auto place = [](int e) { return (e & (VPL - 1)) * 32 + e / VPL; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* row = smem + warp * (32 * VPL);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) row[lane + 32 * i] = 0.0f;
-    __syncwarp();
-    float b[VPL];
+    float* bs = smem;
+    float* row = smem + (warp + 1) * (32 * VPL);
     {
         const float n = static_cast<float>(*p.num_valid), g = p.d_loss ? *p.d_loss : 0.0f;
         const float f = n > 0.0f ? g * (static_cast<float>(p.experts) / (static_cast<float>(p.topk) * n)) / n : 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) b[i] = p.d_loss && lane * VPL + i < p.experts ? f * static_cast<float>(p.counts[lane * VPL + i]) : 0.0f;
+        for (int e = threadIdx.x; e < 32 * VPL; e += BWD_WARPS * 32) bs[place(e)] = p.d_loss && e < p.experts ? f * static_cast<float>(p.counts[e]) : 0.0f;
     }
-    for (long long t = static_cast<long long>(blockIdx.x) * BWD_WARPS + warp; t < p.tokens; t += static_cast<long long>(gridDim.x) * BWD_WARPS) {
-        T* out = static_cast<T*>(p.d_logits) + t * p.experts;
-        const float lse = p.lse[t];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) row[lane + 32 * i] = 0.0f;
+    __syncthreads();
+    // a token's inputs; loaded for the next token before this one's arithmetic, as nothing else hides their latency
+    struct In {
+        Row<T, VPL> v;
+        float lse, w, dw;
+        int idx;
+    };
+    const T* from = static_cast<const T*>(p.logits);
+    auto load = [&](int t, In& in) {
+        in.v.load(from + t * p.ld, lane, p.experts, p.vec != 0);
+        in.lse = p.lse[t];
+        in.idx = -1;
+        in.w = in.dw = 0.0f;
+        if (p.d_weights && lane < p.topk) {
+            const size_t at = static_cast<size_t>(t) * p.topk + lane;
+            in.idx = p.idx[at];
+            in.w = p.weights[at];
+            in.dw = p.d_weights[at];
+        }
+    };
+    const int step = gridDim.x * BWD_WARPS;
+    int t = blockIdx.x * BWD_WARPS + warp;
+    In next;
+    if (t < p.tokens) load(t, next);
+    for (; t < p.tokens; t += step) {
+        const In in = next;
+        if (p.tokens - t > step) load(t + step, next);
+        T* out = static_cast<T*>(p.d_logits) + static_cast<size_t>(t) * p.experts;
         float v[VPL];
-        if (lse == -INFINITY) {                            // took no part
+        const bool on = in.lse != -INFINITY;               // a token that took no part gets zeros, whatever its logits are
+        float dot = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) v[i] = 0.0f;
-        } else {
-            load_row<T, VPL>(static_cast<const T*>(p.logits) + t * p.ld, lane, p.experts, p.vec != 0, v);
-            float dot = 0.0f;
+        for (int i = 0; i < VPL; ++i) {
+            v[i] = on ? expf(in.v.get(i) - in.lse) : 0.0f;
+            dot += v[i] * bs[i * 32 + lane];
+        }
+        const int idx = in.idx >= 0 && in.idx < p.experts ? in.idx : -1;
+        const float w = idx >= 0 ? in.w : 0.0f, dw = idx >= 0 ? in.dw : 0.0f, wdw = w * dw;
+        dot = warp_sum(dot);
+        if (p.d_weights) {
+            const float s = warp_sum(wdw);
+            if (!p.normalize) dot += s;
+            if (idx >= 0) row[place(idx)] = p.normalize ? w * (dw - s) : wdw;      // a token's choices are distinct
+            __syncwarp();
+        }
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                v[i] = expf(v[i] - lse);
-                dot += v[i] * b[i];
-            }
-            int idx = -1;
-            float wdw = 0.0f, w = 0.0f, dw = 0.0f;
-            if (p.d_weights && lane < p.topk) {
-                idx = p.idx[t * p.topk + lane];
-                if (idx >= 0 && idx < p.experts) {
-                    w = p.weights[t * p.topk + lane];
-                    dw = p.d_weights[t * p.topk + lane];
-                    wdw = w * dw;
-                } else {
-                    idx = -1;
-                }
-            }
-            dot = warp_sum(dot);
-            float inner = 0.0f;
-            if (p.d_weights) {
-                const float s = warp_sum(wdw);
-                if (p.normalize) inner = w * (dw - s);
-                else {
-                    inner = wdw;
-                    dot += s;
-                }
-                if (idx >= 0) row[idx] = inner;            // a token's choices are distinct
-                __syncwarp();
-            }
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) v[i] = v[i] * (b[i] - dot) + (p.d_weights ? row[lane * VPL + i] : 0.0f);
-            if (p.d_weights) {
-                __syncwarp();
-                if (idx >= 0) row[idx] = 0.0f;
-                __syncwarp();
-            }
+        for (int i = 0; i < VPL; ++i) v[i] = on ? v[i] * (bs[i * 32 + lane] - dot) + (p.d_weights ? row[i * 32 + lane] : 0.0f) : 0.0f;
+        if (p.d_weights) {
+            __syncwarp();
+            if (idx >= 0) row[place(idx)] = 0.0f;
+            __syncwarp();
         }
         const int e0 = lane * VPL;
         constexpr int BYTES = VPL * static_cast<int>(sizeof(T));
@@ -574,8 +631,9 @@ static cudaError_t launch_fwd(const FwdParams& p, int grid, cudaStream_t st) {
 
 template <typename T, int VPL>
 static cudaError_t launch_bwd(const BwdParams& p, cudaStream_t st) {
-    const int need = (p.tokens + BWD_WARPS - 1) / BWD_WARPS, most = sm_count() * 8;
-    router_bwd_kernel<T, VPL><<<need < most ? need : most, BWD_WARPS * 32, sizeof(float) * BWD_WARPS * 32 * VPL, st>>>(p);
+    const int need = (p.tokens + BWD_WARPS - 1) / BWD_WARPS, most = sm_count() * bwd_blocks<VPL>();
+    const size_t smem = sizeof(float) * (BWD_WARPS + 1) * 32 * VPL;           // at most 36 KB
+    router_bwd_kernel<T, VPL><<<need < most ? need : most, BWD_WARPS * 32, smem, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -611,8 +669,8 @@ static int check_shape(const char* what, int dtype, long long ld, int tokens, in
         note_cuda_error(what, "tokens and experts positive, 1 <= topk <= experts, row pitch >= experts");
         return MX8_ERR_SIZE;
     }
-    if (experts > MAX_EXPERTS || topk > MAX_TOPK || static_cast<long long>(tokens) * topk > 0x7FFFFFFFll) {
-        note_cuda_error(what, "at most 1024 experts, 32 choices and 2^31 - 1 (token, choice) pairs");
+    if (experts > MAX_EXPERTS || topk > MAX_TOPK || static_cast<long long>(tokens) * topk > 0x7FFF0000ll) {
+        note_cuda_error(what, "at most 1024 experts, 32 choices and 2^31 - 2^16 (token, choice) pairs");
         return MX8_ERR_LIMIT;
     }
     return MX8_OK;
@@ -671,8 +729,16 @@ extern "C" int mx8_router_topk(const void* logits, int dtype, long long ld, int 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = dtype == MX8_T_F32 ? router::dispatch_fwd<float>(p, vpl, grid, st) : router::dispatch_fwd<uint16_t>(p, vpl, grid, st);
     if (e == cudaSuccess && grid > 1) {
-        router::router_finish_kernel<<<router::FINISH, 1024, 0, st>>>(p, grid);
-        e = cudaGetLastError();
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(router::FINISH);
+        cfg.blockDim = dim3(1024);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, router::router_finish_kernel, p, grid);
     }
     if (e != cudaSuccess) {
         note_cuda_error("router launch", cudaGetErrorString(e));

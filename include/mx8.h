@@ -255,7 +255,7 @@ MX8_API int mx8_transpose_bf16(const void* in, void* out, int rows, int cols, vo
 
 /* Router of the MoE layer: softmax over the experts, top-k, per-expert counts and the balance loss.
  *   logits [tokens][experts] (MX8_T_BF16 or MX8_T_F32), `ld` elements between rows; token_mask (may be NULL): one byte per token,
- *   0 = the token takes no part and its logits are not read.
+ *   0 = the token takes no part, whatever its logits are.
  * p = softmax(logits) in fp32; the topk largest logits of a token are its choices, largest first, ties to the lower expert (a NaN
  * counts as the largest value).  topk_weights = p at the choices, divided by their sum when normalize != 0.  A logit of -inf
  * switches the expert off for that token: it is never chosen; choices that a token cannot fill have id -1 and weight 0.  A token
