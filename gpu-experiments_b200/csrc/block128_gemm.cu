@@ -33,27 +33,28 @@ constexpr int MAX_GROUPS = 256;
 constexpr int DEV_BAD_GROUPS = 17;            // device status: group sizes that do not fit the operands
 constexpr int DEV_SMEM_BASE = 18;             // device status: dynamic shared memory does not start on a 1024-byte boundary
 constexpr int RED_PITCH = 129;                // floats between columns of the tile that a split adds up
-constexpr int CW = 64;                        // columns of a promoting warp
 constexpr int EPI0 = 4;                       // the first promoting warp
 
 // ROW: Y's scale is one number per 128 columns.  BOTH: it varies by column.
 enum Scales { ROW, BOTH };
 
-template <int CG_, int TN_, bool SWAP_, Scales SC_>
+template <int CG_, int SUB_, int TN_, bool SWAP_, Scales SC_>
 struct Cfg {
-    static constexpr int CG = CG_, TN = TN_;
+    static constexpr int CG = CG_, SUB = SUB_, TN = TN_;      // CTAs of a tile, 128-row parts of X in a CTA, rows of Y
     static constexpr bool SWAP = SWAP_;
     static constexpr Scales SC = SC_;
-    static constexpr int EPI = TN / CW * 4;                   // promoting warps: four lane quadrants for each 64 columns
+    static constexpr int EPI = SUB * TN / 64 * 4;             // promoting warps: 64 values a lane, in one row or in one row of each part
+    static constexpr int CW = 64 / SUB;                       // columns of a promoting warp, four lane quadrants for each
     static constexpr int THREADS = 32 * (EPI0 + EPI);
-    static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN / CG * BK;
+    static constexpr int ROWS = 128 * CG * SUB;               // rows of X of a tile
+    static constexpr int X_BYTES = SUB * 128 * BK, Y_BYTES = TN / CG * BK;
     static constexpr int Y_BOX = SWAP ? 16 : TN / CG;         // rows of Y per TMA copy: with SWAP only boxes with rows are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
-    static constexpr int STAGES = TN == 256 ? 6 : 4;
-    static constexpr int TMEM_COLS = 2 * TN;
+    static constexpr int STAGES = EPI == 16 ? (SUB == 1 ? 6 : 5) : 4;
+    static constexpr int TMEM_COLS = 2 * SUB * TN;
     static constexpr int D = 8;                               // blocks of scales in the ring
-    static constexpr int SLOT = 128 + (SC == ROW ? 4 : TN);   // floats: X's rows, then Y's columns (ROW: two numbers)
-    static constexpr int TURN = SWAP ? 0 : 32 * 32;           // per promoting warp: 32 rows of 32 bytes in which C is turned
+    static constexpr int SLOT = SUB * 128 + (SC == ROW ? 4 : TN);         // floats: X's rows, then Y's columns (ROW: two numbers)
+    static constexpr int TURN = SWAP ? 0 : (SUB == 1 ? 32 : 16) * 32;     // per promoting warp: rows of 32 bytes in which C is turned
     static constexpr int turn_off = STAGES * STAGE;
     static constexpr int ring_off = turn_off + EPI * TURN;
     static constexpr int bar_off = ring_off + D * SLOT * 4;
@@ -61,9 +62,9 @@ struct Cfg {
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
-    static constexpr int PER_SM = TN == 256 ? 1 : 2;
+    static constexpr int PER_SM = EPI == 16 ? 1 : 2;
     static_assert(dynamic * PER_SM <= 232448 - 1024 * (PER_SM - 1), "shared memory budget exceeded");
-    static_assert(TN * RED_PITCH * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
+    static_assert(SUB * TN * RED_PITCH * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
 };
 
 struct Params {
@@ -87,7 +88,7 @@ struct Params {
 };
 
 struct Tile {
-    int x0, x_end;                            // first row of X of this CTA, one past the last row of the matrix or group
+    int x0, x_end;                            // first row of X of this CTA (its second part is 128 CG rows on), one past the matrix's or group's last
     int y0, y_end, y_tma;                     // first row of Y inside its matrix, one past the tile's last, first row in the tensor map
     int ncols;                                // columns of the MMA (both CTAs together)
     int k0, k1;                               // K blocks
@@ -127,7 +128,7 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
         } else {
             o.x0 = seg[lo];
             o.x_end = seg[lo + 1];
-            tiles_x = (o.x_end - o.x0 + 128 * C::CG - 1) / (128 * C::CG);
+            tiles_x = (o.x_end - o.x0 + C::ROWS - 1) / C::ROWS;
             o.y_tma = lo * p.y_rows;
         }
     }
@@ -135,7 +136,7 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     const int in_all = t - first, per = p.group_x * p.tiles_y;
     const int grp = in_all / per, in = in_all - grp * per, n = min(p.group_x, tiles_x - grp * p.group_x);
     const int ty = in / n, tx = grp * p.group_x + in - ty * n;
-    o.x0 += (tx * C::CG + pair_rank) * 128;
+    o.x0 += tx * C::ROWS + pair_rank * 128;
     o.y0 = ty * C::TN;
     o.y_tma += o.y0;
     o.y_end = min(o.y0 + C::TN, p.y_rows);
@@ -147,24 +148,6 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     }
     return o;
 }
-
-// pairs of floats in 64-bit registers: one instruction for two columns
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float half_of(uint64_t v, int i) { return __uint_as_float(static_cast<uint32_t>(i ? v >> 32 : v)); }
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
     float v;
@@ -231,54 +214,59 @@ __device__ __forceinline__ void store_c(const Params& p, long long row, int col,
     else static_cast<uint16_t*>(p.c)[at] = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
-// One warp's 32 rows x 64 columns of C (row = lane): turned through shared memory, 32 bytes of a row at a time, so that a store covers
+// One warp's 32 rows x CW columns of C (row = lane): turned through shared memory, 32 bytes of R rows at a time, so that a store covers
 // whole sectors of rows (16 bytes per lane).  The 16-byte piece k of row r lies in slot k ^ ((r / 4) % 2): conflict-free both ways.
-__device__ __forceinline__ void write_rows(const Params& p, const uint64_t (&acc)[CW / 2], uint32_t turn, long long row0, int rows, int col0, int cols,
-                                           int lane) {
+template <int CW, int R>
+__device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[CW], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
     if (cols <= 0 || rows <= 0) return;
     const int esize = p.c_f32 ? 4 : 2, per = 32 / esize;                  // columns in 32 bytes
     uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * esize;
     const long long pitch = p.ldc * esize;
     const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0;
-    const uint32_t put = turn + lane * 32 + (((lane >> 2) & 1) << 4), get = turn + (lane >> 1) * 32 + (((lane ^ (lane >> 3)) & 1) << 4);
+    const uint32_t put = turn + (lane & (R - 1)) * 32 + (((lane >> 2) & 1) << 4), get = turn + (lane >> 1) * 32 + (((lane ^ (lane >> 3)) & 1) << 4);
 #pragma unroll
     for (int j = 0; j < CW; j += 8) {
         if (!p.c_f32 && (j & 8)) continue;
-        __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint32_t w[4];
-            if (p.c_f32) {
+        for (int r0 = 0; r0 < 32; r0 += R) {                              // the lanes with rows r0 .. r0 + R - 1
+            __syncwarp();
+            if (R == 32 || lane / R * R == r0) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(half_of(acc[j / 2 + 2 * k + i / 2], i & 1));
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t w[4];
+                    if (p.c_f32) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(acc[j + 4 * k + i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(acc[(j + 8 * k + 2 * i) % CW], acc[(j + 8 * k + 2 * i + 1) % CW]);
+                    }
+                    st_shared_v4(put ^ (k << 4), w[0], w[1], w[2], w[3]);
+                }
+            }
+            __syncwarp();
+            if (wide && cols - j >= per) {
+#pragma unroll
+                for (int i = 0; i < R / 16; ++i) {
+                    const int r = r0 + i * 16 + (lane >> 1);
+                    uint32_t w[4];
+                    ld_shared_v4(get + i * 16 * 32, w[0], w[1], w[2], w[3]);
+                    if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 1) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(half_of(acc[(j / 2 + 4 * k + i) % (CW / 2)], 0), half_of(acc[(j / 2 + 4 * k + i) % (CW / 2)], 1));
-            }
-            st_shared_v4(put ^ (k << 4), w[0], w[1], w[2], w[3]);
-        }
-        __syncwarp();
-        if (wide && cols - j >= per) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = i * 16 + (lane >> 1);
-                uint32_t w[4];
-                ld_shared_v4(get + i * 16 * 32, w[0], w[1], w[2], w[3]);
-                if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 1) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        } else {
-            // four rows at a time, a word per lane
-            const int word = lane & 7, left = cols - j - word * (4 / esize);
+                // four rows at a time, a word per lane
+                const int word = lane & 7, left = cols - j - word * (4 / esize);
 #pragma unroll 1
-            for (int r = lane >> 3; r < rows; r += 4) {
-                uint32_t w;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * 32 + (((word >> 2) ^ ((r >> 2) & 1)) << 4) + (word & 3) * 4));
-                uint8_t* to = c + r * pitch + j * esize + word * 4;
-                if (p.c_f32) {
-                    if (left >= 1) *reinterpret_cast<uint32_t*>(to) = w;
-                } else {
-                    if (left >= 1) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
-                    if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
+                for (int r = lane >> 3; r < R && r0 + r < rows; r += 4) {
+                    uint32_t w;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * 32 + (((word >> 2) ^ ((r >> 2) & 1)) << 4) + (word & 3) * 4));
+                    uint8_t* to = c + (r0 + r) * pitch + j * esize + word * 4;
+                    if (p.c_f32) {
+                        if (left >= 1) *reinterpret_cast<uint32_t*>(to) = w;
+                    } else {
+                        if (left >= 1) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
+                        if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
+                    }
                 }
             }
         }
@@ -310,7 +298,7 @@ __device__ __forceinline__ void group_prefix(const Params& p, int* seg, int lane
         end += row;
         if (end > cap) bad = true;
         const int e = static_cast<int>(min(end, static_cast<long long>(cap))), b = static_cast<int>(min(end - n, static_cast<long long>(cap)));
-        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + 128 * C::CG - 1) / (128 * C::CG) * p.tiles_y;
+        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + C::ROWS - 1) / C::ROWS * p.tiles_y;
         int tt = nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -406,7 +394,8 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                             if constexpr (CG == 2) tma_load_2d_pair(to, m, kb * BK, y, bar);
                             else tma_load_2d(to, m, kb * BK, y, bar);
                         };
-                        load(dst, &tm_x, x0);
+#pragma unroll
+                        for (int i = 0; i < C::SUB; ++i) load(dst + i * 128 * BK, &tm_x, x0 + i * 128 * CG);
 #pragma unroll
                         for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i)
                             if (i < boxes) load(dst + C::X_BYTES + i * C::Y_BOX * BK, &tm_y, y0 + i * C::Y_BOX);
@@ -430,12 +419,15 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (!warp_wait(accfree0 + buf * 8, ((it >> 1) & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE)) { ok = false; break; }
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t x = desc_sw128_lo(base + stage * C::STAGE), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
-                        const uint32_t d = tmem + buf * C::TN;
-                        tc_mma_e4m3_lo<CG, 0>(d, x, y, idesc);
-                        tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
-                        tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
-                        tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
+#pragma unroll
+                        for (int i = 0; i < C::SUB; ++i) {
+                            const uint32_t x = desc_sw128_lo(base + stage * C::STAGE + i * 128 * BK), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
+                            const uint32_t d = tmem + (buf * C::SUB + i) * C::TN;
+                            tc_mma_e4m3_lo<CG, 0>(d, x, y, idesc);
+                            tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
+                            tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
+                            tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
+                        }
                         commit<CG>(accfull0 + buf * 8, first_rank);
                         commit<CG>(empty0 + stage * 8, first_rank);
                     }
@@ -470,13 +462,13 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (m >= 5 && !complete(m - 5)) { ok = false; break; }
                     const uint32_t to = smem_u32(ring + (m & (D - 1)) * C::SLOT + lane);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(ti.x0 + i * 32, x_last)));
+                    for (int i = 0; i < 4 * C::SUB; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(ti.x0 + i * 32 + i / 4 * 128 * (CG - 1), x_last)));
                     if constexpr (C::SC == ROW) {
-                        if (lane < 2) copy4(to + 512, yk);
+                        if (lane < 2) copy4(to + C::SUB * 512, yk);
                     } else {
 #pragma unroll
                         for (int i = 0; i < NY; ++i)
-                            if (i * 32 < ti.ncols) copy4(to + 512 + i * 128, yk + min(ti.y0 + i * 32, y_last));
+                            if (i * 32 < ti.ncols) copy4(to + C::SUB * 512 + i * 128, yk + min(ti.y0 + i * 32, y_last));
                     }
                     copies_commit();
                     xk += p.xs_k;
@@ -499,6 +491,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         // ------------------------------------------------------------ promotion and C
         if constexpr (C::EPI == 16) set_regs_more<104>();
         const int ew = warp - EPI0, q = warp & 3;                        // TMEM lane quadrant
+        constexpr int CW = C::CW;
         const int col0 = (ew >> 2) * CW;
         const uint32_t turn = base + C::turn_off + ew * C::TURN;
         const uint32_t free_lead = CG == 2 ? map_to_cta(accfree0, first_rank) : accfree0;
@@ -514,41 +507,30 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 blocks = ti.k1 - ti.k0;
                 mine = ti.ncols - col0;
             }
-            uint64_t acc[CW / 2];
+            float acc[C::SUB][CW];
 #pragma unroll
-            for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < C::SUB * CW; ++i) acc[i / CW][i % CW] = 0.0f;
             for (; blocks > 0; --blocks, ++it) {
                 const uint32_t buf = it & 1;
                 if (!warp_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t src = my_tmem + buf * C::TN;
+                const uint32_t src = my_tmem + buf * (C::SUB * C::TN);
                 const float* slot = my_ring + (it & (D - 1)) * C::SLOT;
-                uint64_t ss;
-                auto add = [&](const uint32_t (&v)[16], int c) {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        uint64_t a = pair(v[i], v[i + 1]), b = pair(v[i + 2], v[i + 3]);
-                        if constexpr (C::SC == BOTH) {
-                            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(slot - r + 128 + col0 + c + i);
-                            a = mul2(a, y.x);
-                            b = mul2(b, y.y);
-                        }
-                        acc[(c + i) / 2] = fma2(a, ss, acc[(c + i) / 2]);
-                        acc[(c + i) / 2 + 1] = fma2(b, ss, acc[(c + i) / 2 + 1]);
-                    }
-                };
                 auto release = [&]() {                                   // the buffer's values are all in registers
                     tc_fence_before();
                     __syncwarp();
                     arrive_lane0<CG>(free_lead + buf * 8, lane);
                 };
+                uint32_t va[16], vb[16];
                 if constexpr (C::SC == ROW) {
                     // 64 columns in four loads, two in flight
-                    uint32_t va[16], vb[16];
                     tc_ld16(src, va);
                     tc_ld16(src + 16, vb);
                     const float s = slot[0] * slot[128 + (col0 >> 7) - r];
-                    ss = pair(__float_as_uint(s), __float_as_uint(s));
+                    auto add = [&](const uint32_t (&v)[16], int c) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[0][c + i] = fmaf(__uint_as_float(v[i]), s, acc[0][c + i]);
+                    };
                     tc_wait16(va);
                     tc_wait16(vb);
                     add(va, 0);
@@ -560,20 +542,43 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     release();
                     add(va, 32);
                     add(vb, 48);
+                } else if constexpr (C::SUB == 2) {
+                    // 32 columns of two rows: a column's scale is read once for both
+                    const float s0 = slot[0], s1 = slot[128];
+#pragma unroll
+                    for (int c = 0; c < CW; c += 16) {
+                        tc_ld16(src + c, va);
+                        tc_ld16(src + C::TN + c, vb);
+                        tc_wait16(va);
+                        tc_wait16(vb);
+                        if (c + 16 == CW) release();
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 y = *reinterpret_cast<const float4*>(slot - r + 256 + col0 + c + i);
+                            const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                acc[0][c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s0, acc[0][c + i + k]);
+                                acc[1][c + i + k] = fmaf(__uint_as_float(vb[i + k]) * ys[k], s1, acc[1][c + i + k]);
+                            }
+                        }
+                    }
                 } else {
-                    // one in flight: the column scales want the registers
-                    uint32_t v[16];
-                    if (mine > 0) tc_ld16(src, v);
-                    else release();
+                    if (mine <= 0) release();
                     const float s = slot[0];
-                    ss = pair(__float_as_uint(s), __float_as_uint(s));
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
                         if (c >= mine) break;
-                        if (c) tc_ld16(src + c, v);
-                        tc_wait16(v);
+                        tc_ld16(src + c, va);
+                        tc_wait16(va);
                         if (c + 16 == CW || c + 16 >= mine) release();
-                        add(v, c);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const float4 y = *reinterpret_cast<const float4*>(slot - r + 128 + col0 + c + i);
+                            const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) acc[0][c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s, acc[0][c + i + k]);
+                        }
                     }
                 }
             }
@@ -586,17 +591,23 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 // this CTA's MMAs are complete (its last accumulator arrived), so the stage ring is free
                 float* red = reinterpret_cast<float*>(base_ptr);
 #pragma unroll
-                for (int i = 0; i < CW; ++i)
-                    if (i < cols) red[(col0 + i) * RED_PITCH + r] = half_of(acc[i / 2], i & 1);
+                for (int k = 0; k < C::SUB; ++k)
+#pragma unroll
+                    for (int i = 0; i < CW; ++i)
+                        if (i < cols) red[(k * C::TN + col0 + i) * RED_PITCH + r] = acc[k][i];
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
                 if (ti.x0 + r < p.x_rows) {
 #pragma unroll
                     for (int i = 0; i < CW; ++i)
-                        if (i < cols) store_c(p, ti.y0 + col0 + i, ti.x0 + r, half_of(acc[i / 2], i & 1));
+                        if (i < cols) store_c(p, ti.y0 + col0 + i, ti.x0 + r, acc[0][i]);
                 }
             } else {
-                write_rows(p, acc, turn, ti.c_row + ti.x0 + q * 32, min(32, ti.x_end - ti.x0 - q * 32), ti.y0 + col0, cols, lane);
+#pragma unroll
+                for (int k = 0; k < C::SUB; ++k) {
+                    const int x0 = ti.x0 + k * 128 * CG + q * 32;
+                    write_rows<CW, C::TURN / 32>(p, acc[k], turn, ti.c_row + x0, min(32, ti.x_end - x0), ti.y0 + col0, cols, lane);
+                }
             }
         }
     }
@@ -606,7 +617,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         cluster_sync_all();
         if (warp >= EPI0 && unit < num_tiles) {
             const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-            const int ew = warp - EPI0, xn = min(128, p.x_rows - ti.x0), yn = ti.y_end - ti.y0;
+            const int ew = warp - EPI0, yn = ti.y_end - ti.y0;
             if constexpr (C::SWAP) {
                 // part k writes its share of the tile's columns (rows of C); a lane is a row of the tile (column of C)
                 const int c1 = yn * (part + 1) / p.split, r = (ew & 3) * 32 + lane;
@@ -614,17 +625,19 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     const uint32_t at = base + (c * RED_PITCH + r) * 4;
                     float s = 0.0f;
                     for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
-                    if (r < xn) store_c(p, ti.y0 + c, ti.x0 + r, s);
+                    if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + c, ti.x0 + r, s);
                 }
             } else {
                 // part k writes its share of the tile's rows; a lane is a column
-                const int r1 = min(128 * (part + 1) / p.split, xn);
-                for (int r = 128 * part / p.split + ew; r < r1; r += C::EPI) {
+                const int n = 128 * C::SUB, r1 = n * (part + 1) / p.split;
+                for (int r = n * part / p.split + ew; r < r1; r += C::EPI) {
+                    const int row = ti.x0 + r + r / 128 * 128 * (CG - 1);
+                    if (row >= ti.x_end) break;
                     for (int c = lane; c < yn; c += 32) {
-                        const uint32_t at = base + (c * RED_PITCH + r) * 4;
+                        const uint32_t at = base + ((r / 128 * C::TN + c) * RED_PITCH + r % 128) * 4;
                         float s = 0.0f;
                         for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
-                        store_c(p, ti.c_row + ti.x0 + r, ti.y0 + c, s);
+                        store_c(p, ti.c_row + row, ti.y0 + c, s);
                     }
                 }
             }
@@ -684,9 +697,9 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     p.kblocks = (a.K + BK - 1) / BK;
     p.x_rows = C::SWAP ? a.N : a.M;
     p.y_rows = C::SWAP ? a.M : a.N;
-    p.tiles_x = (p.x_rows + 128 * C::CG - 1) / (128 * C::CG);
+    p.tiles_x = (p.x_rows + C::ROWS - 1) / C::ROWS;
     p.tiles_y = (p.y_rows + C::TN - 1) / C::TN;
-    p.group_x = 16;                           // 16 tile rows walked together keep their X panels and the Y panel in L2
+    p.group_x = 16 / C::SUB;                  // 4096 rows of X walked together stay in L2 with the Y panel
     const float* bs = a.B_sc;
     p.xs = C::SWAP ? bs : a.A_sc;
     p.xs_square = C::SWAP && a.b_square;
@@ -751,13 +764,15 @@ static int split_for(long long units, long long room, int kblocks, int most) {
 
 static int run(const Args& a, cudaStream_t st) {
     const int kb = (a.K + BK - 1) / BK, sms = sm_count();
-    const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256;
-    if (a.wgrad) return launch<Cfg<2, 256, false, BOTH>>(a, 1, st);
-    if (a.groups > 0) return launch<Cfg<2, 256, false, ROW>>(a, 1, st);
+    const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256, m512 = (a.M + 511ll) / 512;
+    using Squares = Cfg<2, 1, 256, false, ROW>;
+    using Rows = Cfg<2, 2, 128, false, BOTH>;
+    using Few = Cfg<1, 1, 64, true, BOTH>;
+    if (a.wgrad) return launch<Rows>(a, 1, st);
+    if (a.groups > 0) return launch<Squares>(a, 1, st);
     // few rows: 128 weights a tile, two CTAs on a multiprocessor
-    if (a.M <= 64) return launch<Cfg<1, 64, true, BOTH>>(a, split_for(n128, 2 * sms, kb, 8), st);
-    const int split = split_for(m256 * n256, sms / 2, kb, 4);
-    return a.b_square ? launch<Cfg<2, 256, false, ROW>>(a, split, st) : launch<Cfg<2, 256, false, BOTH>>(a, split, st);
+    if (a.M <= 64) return launch<Few>(a, split_for(n128, 2 * sms, kb, 8), st);
+    return a.b_square ? launch<Squares>(a, split_for(m256 * n256, sms / 2, kb, 4), st) : launch<Rows>(a, split_for(m512 * n128, sms / 2, kb, 4), st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {
