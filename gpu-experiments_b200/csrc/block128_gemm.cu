@@ -170,6 +170,13 @@ __device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
+// 32 lanes x 8 columns at each of two addresses, and the wait for all loads
+__device__ __forceinline__ void tc_ld8x2(uint32_t t0, uint32_t t1, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(t0) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(t1) : "memory");
+}
 // four bytes, global -> shared, asynchronously; groups of copies complete in order
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -543,26 +550,34 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     add(va, 32);
                     add(vb, 48);
                 } else if constexpr (C::SUB == 2) {
-                    // 32 columns of two rows: a column's scale is read once for both
+                    // 32 columns of two rows, eight at a time; the next eight are on their way while these are added, and a column's
+                    // scale is read once for both rows
+                    tc_ld8x2(src, src + C::TN, va);
                     const float s0 = slot[0], s1 = slot[128];
+                    auto add = [&](const uint32_t (&v)[16], int c) {
 #pragma unroll
-                    for (int c = 0; c < CW; c += 16) {
-                        tc_ld16(src + c, va);
-                        tc_ld16(src + C::TN + c, vb);
-                        tc_wait16(va);
-                        tc_wait16(vb);
-                        if (c + 16 == CW) release();
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
+                        for (int i = 0; i < 8; i += 4) {
                             const float4 y = *reinterpret_cast<const float4*>(slot - r + 256 + col0 + c + i);
                             const float ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                acc[0][c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s0, acc[0][c + i + k]);
-                                acc[1][c + i + k] = fmaf(__uint_as_float(vb[i + k]) * ys[k], s1, acc[1][c + i + k]);
+                                acc[0][c + i + k] = fmaf(__uint_as_float(v[i + k]) * ys[k], s0, acc[0][c + i + k]);
+                                acc[1][c + i + k] = fmaf(__uint_as_float(v[8 + i + k]) * ys[k], s1, acc[1][c + i + k]);
                             }
                         }
-                    }
+                    };
+                    tc_wait16(va);
+                    tc_ld8x2(src + 8, src + C::TN + 8, vb);
+                    add(va, 0);
+                    tc_wait16(vb);
+                    tc_ld8x2(src + 16, src + C::TN + 16, va);
+                    add(vb, 8);
+                    tc_wait16(va);
+                    tc_ld8x2(src + 24, src + C::TN + 24, vb);
+                    add(va, 16);
+                    tc_wait16(vb);
+                    release();
+                    add(vb, 24);
                 } else {
                     if (mine <= 0) release();
                     const float s = slot[0];
