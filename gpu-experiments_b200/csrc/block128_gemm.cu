@@ -17,8 +17,9 @@
 // X = B: the weights fill the lanes and a tile has as many columns (a multiple of 16) as there are rows of A.
 // Scales that vary by lane cost a register; scales that vary by column have to reach every lane through shared memory, 128 bytes a
 // cycle, which is why squares (one scale per 128 columns) have a form of their own (ROW).
-// split > 1: `split` CTAs or pairs of one cluster share a tile, each takes a part of the K blocks, and the partial tiles are added
-// through distributed shared memory in rank order: no workspace, no atomics, the same result in every run.
+// split > 1: `split` CTAs or pairs of one cluster share a tile, each takes a part of the K blocks, and each adds up its share of the tile
+// in rank order: no workspace, no atomics, the same result in every run.  With SWAP the shares are sent by bulk copies from shared memory
+// to shared memory, otherwise each CTA reads the others' 16 bytes a lane.  (Words one by one cost 3 us read and 6 us sent for 64 rows.)
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
 #include <atomic>
 
@@ -32,16 +33,15 @@ constexpr int BK = 128;                       // bytes and elements of K per sta
 constexpr int MAX_GROUPS = 256;
 constexpr int DEV_BAD_GROUPS = 17;            // device status: group sizes that do not fit the operands
 constexpr int DEV_SMEM_BASE = 18;             // device status: dynamic shared memory does not start on a 1024-byte boundary
-constexpr int RED_PITCH = 129;                // floats between columns of the tile that a split adds up
 constexpr int EPI0 = 4;                       // the first promoting warp
 
 // ROW: Y's scale is one number per 128 columns.  BOTH: it varies by column.
 enum Scales { ROW, BOTH };
 
-template <int CG_, int SUB_, int TN_, bool SWAP_, Scales SC_>
+template <int CG_, int SUB_, int TN_, bool SWAP_, Scales SC_, bool SPLIT_>
 struct Cfg {
     static constexpr int CG = CG_, SUB = SUB_, TN = TN_;      // CTAs of a tile, 128-row parts of X in a CTA, rows of Y
-    static constexpr bool SWAP = SWAP_;
+    static constexpr bool SWAP = SWAP_, SPLIT = SPLIT_;       // SPLIT: a kernel of its own, as its code takes registers from the main loop (8192^3: 487 -> 540 us)
     static constexpr Scales SC = SC_;
     static constexpr int EPI = SUB * TN / 64 * 4;             // promoting warps: 64 values a lane, in one row or in one row of each part
     static constexpr int CW = 64 / SUB;                       // columns of a promoting warp, four lane quadrants for each
@@ -50,21 +50,25 @@ struct Cfg {
     static constexpr int X_BYTES = SUB * 128 * BK, Y_BYTES = TN / CG * BK;
     static constexpr int Y_BOX = SWAP ? 16 : TN / CG;         // rows of Y per TMA copy: with SWAP only boxes with rows are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
-    static constexpr int STAGES = EPI == 16 ? (SUB == 1 ? 6 : 5) : 4;
+    static constexpr int STAGES = EPI == 16 ? (SUB == 1 ? 6 : 5) : 3;
     static constexpr int TMEM_COLS = 2 * SUB * TN;
     static constexpr int D = 8;                               // blocks of scales in the ring
     static constexpr int SLOT = SUB * 128 + (SC == ROW ? 4 : TN);         // floats: X's rows, then Y's columns (ROW: two numbers)
-    static constexpr int TURN = SWAP ? 0 : (SUB == 1 ? 32 : 16) * 32;     // per promoting warp: rows of 32 bytes in which C is turned
-    static constexpr int turn_off = STAGES * STAGE;
+    static constexpr int TURN = SWAP || SPLIT ? 0 : 1024 / SUB;           // per promoting warp: where C is turned
+    // where a split's shares of a tile arrive with SWAP: its columns, 128 rows each, from each of 2, 4 or 8 parts
+    static constexpr int PARTS = SWAP ? TN * 128 * 4 : 0;
+    static constexpr int turn_off = STAGES * STAGE + PARTS;
     static constexpr int ring_off = turn_off + EPI * TURN;
     static constexpr int bar_off = ring_off + D * SLOT * 4;
-    static constexpr int n_bars = 2 * STAGES + 4;             // full, empty; accumulator (and scales) full[2], accumulator free[2]
+    static constexpr int n_bars = 2 * STAGES + 5;             // full, empty; accumulator (and scales) full[2], accumulator free[2]; shares
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
+    static constexpr int MAX_SPLIT = 8 / CG;                  // a cluster of eight CTAs at most
+    static constexpr int LEAST = SWAP ? 2 : 8;                // K blocks of a part
     static constexpr int PER_SM = EPI == 16 ? 1 : 2;
     static_assert(dynamic * PER_SM <= 232448 - 1024 * (PER_SM - 1), "shared memory budget exceeded");
-    static_assert(SUB * TN * RED_PITCH * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
+    static_assert(SWAP ? TN * 512 <= STAGES * STAGE : 128 * SUB * (TN + 4) * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
 };
 
 struct Params {
@@ -141,7 +145,7 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     o.y_tma += o.y0;
     o.y_end = min(o.y0 + C::TN, p.y_rows);
     o.ncols = round_cols<C::CG>(o.y_end - o.y0);
-    if (p.split > 1) {
+    if constexpr (C::SPLIT) {
         const int nk = o.k1 - o.k0, k0 = o.k0;
         o.k0 = k0 + nk * part / p.split;
         o.k1 = k0 + nk * (part + 1) / p.split;
@@ -149,11 +153,19 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     return o;
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+// contiguous bytes of this CTA's shared memory to a CTA of the cluster, counted on its barrier; 16-byte aligned
+__device__ __forceinline__ void bulk_send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // 32 lanes x 16 columns
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -221,58 +233,54 @@ __device__ __forceinline__ void store_c(const Params& p, long long row, int col,
     else static_cast<uint16_t*>(p.c)[at] = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
-// One warp's 32 rows x CW columns of C (row = lane): turned through shared memory, 32 bytes of R rows at a time, so that a store covers
-// whole sectors of rows (16 bytes per lane).  The 16-byte piece k of row r lies in slot k ^ ((r / 4) % 2): conflict-free both ways.
-template <int CW, int R>
+// One warp's 32 rows x CW columns of C (row = lane): turned through BYTES bytes of shared memory, a few rows at a time, so that a store covers
+// 64 or 128 consecutive bytes of a row (16 per lane).  The 16-byte piece k of row r lies in slot k ^ (r % pieces): conflict-free both ways.
+// (All 32 rows at once and 32 bytes of each took 3 us a tile: a store then touches 16 lines.)
+template <int CW, int BYTES, bool F32>
 __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[CW], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
-    if (cols <= 0 || rows <= 0) return;
-    const int esize = p.c_f32 ? 4 : 2, per = 32 / esize;                  // columns in 32 bytes
-    uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * esize;
-    const long long pitch = p.ldc * esize;
+    constexpr int ES = F32 ? 4 : 2, WIDE = CW * ES < 128 ? CW * ES : 128;  // bytes of a row in a pass
+    constexpr int PIECES = WIDE / 16, R = BYTES / WIDE, PER = WIDE / ES;   // 16-byte pieces of it, rows of a pass, columns of a pass
+    static_assert(R * PIECES % 32 == 0, "whole warps of pieces");
+    uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * ES;
+    const long long pitch = p.ldc * ES;
     const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0;
-    const uint32_t put = turn + (lane & (R - 1)) * 32 + (((lane >> 2) & 1) << 4), get = turn + (lane >> 1) * 32 + (((lane ^ (lane >> 3)) & 1) << 4);
+    const int my_row = lane % R, piece = lane % PIECES;
+    const uint32_t put = turn + my_row * WIDE + ((my_row % PIECES) << 4);
 #pragma unroll
-    for (int j = 0; j < CW; j += 8) {
-        if (!p.c_f32 && (j & 8)) continue;
-#pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += R) {                              // the lanes with rows r0 .. r0 + R - 1
+    for (int j = 0; j < CW; j += PER) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += R) {
             __syncwarp();
-            if (R == 32 || lane / R * R == r0) {
+            if (lane / R * R == r0) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < PIECES; ++k) {
                     uint32_t w[4];
-                    if (p.c_f32) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(acc[j + 4 * k + i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(acc[(j + 8 * k + 2 * i) % CW], acc[(j + 8 * k + 2 * i + 1) % CW]);
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F32) w[i] = __float_as_uint(acc[j + 4 * k + i]);
+                        else w[i] = pack_bf16x2(acc[j + 8 * k + 2 * i], acc[j + 8 * k + 2 * i + 1]);
                     }
                     st_shared_v4(put ^ (k << 4), w[0], w[1], w[2], w[3]);
                 }
             }
             __syncwarp();
-            if (wide && cols - j >= per) {
 #pragma unroll
-                for (int i = 0; i < R / 16; ++i) {
-                    const int r = r0 + i * 16 + (lane >> 1);
-                    uint32_t w[4];
-                    ld_shared_v4(get + i * 16 * 32, w[0], w[1], w[2], w[3]);
-                    if (r < rows) *reinterpret_cast<uint4*>(c + r * pitch + j * esize + (lane & 1) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else {
-                // four rows at a time, a word per lane
-                const int word = lane & 7, left = cols - j - word * (4 / esize);
-#pragma unroll 1
-                for (int r = lane >> 3; r < R && r0 + r < rows; r += 4) {
-                    uint32_t w;
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * 32 + (((word >> 2) ^ ((r >> 2) & 1)) << 4) + (word & 3) * 4));
-                    uint8_t* to = c + (r0 + r) * pitch + j * esize + word * 4;
-                    if (p.c_f32) {
-                        if (left >= 1) *reinterpret_cast<uint32_t*>(to) = w;
-                    } else {
-                        if (left >= 1) *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
-                        if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
+            for (int i = 0; i < R * PIECES / 32; ++i) {
+                const int r = i * (32 / PIECES) + lane / PIECES;
+                uint32_t w[4];
+                ld_shared_v4(turn + r * WIDE + ((piece ^ (r % PIECES)) << 4), w[0], w[1], w[2], w[3]);
+                uint8_t* to = c + (r0 + r) * pitch + j * ES + piece * 16;
+                const int left = cols - j - piece * (16 / ES);            // columns from this piece's first on
+                if (r0 + r >= rows || left <= 0) continue;
+                if (wide && left >= 16 / ES) {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16 / ES; ++e) {
+                        if (e < left) {
+                            if constexpr (F32) *reinterpret_cast<uint32_t*>(to + 4 * e) = w[e];
+                            else *reinterpret_cast<uint16_t*>(to + 2 * e) = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+                        }
                     }
                 }
             }
@@ -338,13 +346,14 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         return;
     }
     const uint32_t full0 = base + C::bar_off, empty0 = full0 + S * 8, accfull0 = empty0 + S * 8, accfree0 = accfull0 + 16;
+    const uint32_t shares = accfree0 + 16;                    // a split's shares have arrived (SWAP)
     volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(base_ptr + C::misc_off);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + C::misc_off + 8);
     float* ring = reinterpret_cast<float*>(base_ptr + C::ring_off);
     int* seg = reinterpret_cast<int*>(base_ptr + C::seg_off);
     const AbortCtl ab{abort_flag, p.status};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cluster = CG * p.split;                         // CTAs that share a tile
+    const int cluster = C::SPLIT ? CG * p.split : CG;         // CTAs that share a tile
     const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int pair_rank = CG == 2 ? rank & 1 : 0, part = rank / CG, first_rank = rank - pair_rank;
     const int unit = blockIdx.x / cluster, units = gridDim.x / cluster;
@@ -359,6 +368,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             mbar_init(accfull0 + b * 8, 2);                   // the MMAs' commit and this CTA's scales
             mbar_init(accfree0 + b * 8, C::EPI * CG);         // promoting warps of the pair, on the leading CTA's barrier
         }
+        mbar_init(shares, 1);
         fence_mbar_init();
         prefetch_tmap(&tm_x);
         prefetch_tmap(&tm_y);
@@ -372,6 +382,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     tc_fence_before();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync_all();
+    else if (C::SPLIT) cluster_arrive();                      // waited for before the first thing is sent
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *tmem_ptr, 0);
     const int num_tiles = p.groups > 0 ? __shfl_sync(0xFFFFFFFFu, seg[MAX_GROUPS + 1 + p.groups], 0) : p.tiles_x * p.tiles_y;
@@ -601,15 +612,22 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             int again = t;                                               // found anew: nothing of it has to stay in registers during the loop
             asm volatile("" : "+r"(again));
             const Tile ti = tile_at<C>(again, p, seg, pair_rank, part);
-            const int cols = min(CW, ti.y_end - ti.y0 - col0);            // that exist
-            if (p.split > 1) {
-                // this CTA's MMAs are complete (its last accumulator arrived), so the stage ring is free
-                float* red = reinterpret_cast<float*>(base_ptr);
-#pragma unroll
-                for (int k = 0; k < C::SUB; ++k)
+            [[maybe_unused]] const int cols = min(CW, ti.y_end - ti.y0 - col0);      // that exist
+            if constexpr (C::SPLIT) {
+                // this CTA's MMAs are complete (its last accumulator arrived): the stage ring is free
+                if constexpr (C::SWAP) {
 #pragma unroll
                     for (int i = 0; i < CW; ++i)
-                        if (i < cols) red[(k * C::TN + col0 + i) * RED_PITCH + r] = acc[k][i];
+                        if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[0][i];
+                } else {
+                    // rows of C, 16 bytes more than the columns: eight lanes' 16-byte pieces fall into different banks
+#pragma unroll
+                    for (int k = 0; k < C::SUB; ++k)
+#pragma unroll
+                        for (int i = 0; i < CW; i += 4)
+                            *reinterpret_cast<float4*>(base_ptr + ((k * 128 + r) * (C::TN + 4) + col0 + i) * 4) =
+                                make_float4(acc[k][i], acc[k][i + 1], acc[k][i + 2], acc[k][i + 3]);
+                }
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
                 if (ti.x0 + r < p.x_rows) {
@@ -621,41 +639,86 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 #pragma unroll
                 for (int k = 0; k < C::SUB; ++k) {
                     const int x0 = ti.x0 + k * 128 * CG + q * 32;
-                    write_rows<CW, C::TURN / 32>(p, acc[k], turn, ti.c_row + x0, min(32, ti.x_end - x0), ti.y0 + col0, cols, lane);
+                    const int rows = min(32, ti.x_end - x0);
+                    if (p.c_f32) write_rows<CW, C::TURN, true>(p, acc[k], turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
+                    else write_rows<CW, C::TURN, false>(p, acc[k], turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
                 }
             }
         }
     }
 
-    if (p.split > 1) {
+    if constexpr (C::SPLIT) {
         __syncwarp();
-        cluster_sync_all();
-        if (warp >= EPI0 && unit < num_tiles) {
+        // (without register shares of their own the first four warps help)
+        constexpr int W0 = C::EPI == 16 ? EPI0 : 0, WARPS = C::THREADS / 32 - W0;
+        if constexpr (C::SWAP) {
+            // part j adds up columns yn j / split .. yn (j + 1) / split of the tile (rows of C): 512 bytes each, contiguous
             const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-            const int ew = warp - EPI0, yn = ti.y_end - ti.y0;
-            if constexpr (C::SWAP) {
-                // part k writes its share of the tile's columns (rows of C); a lane is a row of the tile (column of C)
-                const int c1 = yn * (part + 1) / p.split, r = (ew & 3) * 32 + lane;
-                for (int c = yn * part / p.split + (ew >> 2); c < c1; c += C::EPI / 4) {
-                    const uint32_t at = base + (c * RED_PITCH + r) * 4;
-                    float s = 0.0f;
-                    for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
-                    if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + c, ti.x0 + r, s);
+            const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
+            fence_proxy_async_smem();                                    // the tile's words, for the copies below
+            cluster_wait();                                              // every CTA's barriers are there
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
+                for (int j = 0; j < p.split; ++j) {
+                    const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
+                    if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
                 }
-            } else {
-                // part k writes its share of the tile's rows; a lane is a column
-                const int n = 128 * C::SUB, r1 = n * (part + 1) / p.split;
-                for (int r = n * part / p.split + ew; r < r1; r += C::EPI) {
+            }
+            if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
+                const int r = (warp & 3) * 32 + lane;                    // a lane is a row of the tile (column of C)
+                const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
+                const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
+                for (int c = warp >> 2; c < mine; c += WARPS / 4) {
+                    float s = part == 0 ? own[c * 128] : in[c * 128];
+                    for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
+                    if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + first + c, ti.x0 + r, s);
+                }
+            }
+            __syncwarp();
+            cluster_arrive();                                            // this CTA has its shares: what was sent to it has been read
+            cluster_wait();
+        } else {
+            cluster_sync_all();                                          // every part's tile lies in its CTA's shared memory
+            if (warp >= W0) {
+                const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
+                // part j adds up rows n j / split .. n (j + 1) / split; a lane has four columns
+                const int w = warp - W0, yn = ti.y_end - ti.y0, n = 128 * C::SUB, r1 = n * (part + 1) / p.split, esize = p.c_f32 ? 4 : 2;
+                const bool wide = (reinterpret_cast<uintptr_t>(p.c) % (4 * esize)) == 0 && p.ldc % 4 == 0;
+                for (int r = n * part / p.split + w; r < r1; r += WARPS) {
                     const int row = ti.x0 + r + r / 128 * 128 * (CG - 1);
                     if (row >= ti.x_end) break;
-                    for (int c = lane; c < yn; c += 32) {
-                        const uint32_t at = base + ((r / 128 * C::TN + c) * RED_PITCH + r % 128) * 4;
-                        float s = 0.0f;
-                        for (int k = 0; k < p.split; ++k) s += ld_cluster(map_to_cta(at, k * CG + pair_rank));
-                        store_c(p, ti.c_row + row, ti.y0 + c, s);
+#pragma unroll
+                    for (int c = 0; c < C::TN; c += 128) {
+                        const int col = c + lane * 4;
+                        float4 v[C::MAX_SPLIT];
+#pragma unroll
+                        for (int k = 0; k < C::MAX_SPLIT; ++k)
+                            if (k < p.split) v[k] = ld_cluster4(map_to_cta(base + (r * (C::TN + 4) + col) * 4, k * CG + pair_rank));
+                        float4 s = v[0];
+#pragma unroll
+                        for (int k = 1; k < C::MAX_SPLIT; ++k)
+                            if (k < p.split) {
+                                s.x += v[k].x;
+                                s.y += v[k].y;
+                                s.z += v[k].z;
+                                s.w += v[k].w;
+                            }
+                        const long long at = (ti.c_row + row) * p.ldc + ti.y0 + col;
+                        if (wide && col + 4 <= yn) {
+                            if (p.c_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.c) + at) = s;
+                            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+                        } else {
+                            const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (col + i < yn) store_c(p, ti.c_row + row, ti.y0 + col + i, f[i]);
+                        }
                     }
                 }
             }
+            __syncwarp();
+            cluster_sync_all();                                          // nobody leaves while its tile is read
         }
     }
 
@@ -667,8 +730,9 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     if (warp == 2) copies_wait<0>();
     __syncwarp();
     tc_fence_before();
-    // nobody leaves while its tile is read, its TMEM written or its barriers arrived on
-    if (cluster > 1) cluster_sync_all(); else __syncthreads();
+    // nobody leaves a pair while its TMEM is written or its barriers are arrived on
+    if constexpr (CG == 2) cluster_sync_all();
+    else __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<CG>(tmem, C::TMEM_COLS);
@@ -696,6 +760,77 @@ static int operand_map(CUtensorMap* m, const void* base, long long rows, int K, 
     return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// what the host keeps of a kernel for each device: the status word's address and, once the shared memory limit is raised, how many of its
+// clusters can be resident at once (two threads racing here find the same)
+struct Known {
+    std::atomic<int*> status;
+    std::atomic<int> clusters[9];              // by cluster size
+};
+
+template <class C>
+static int known(Known*& k) {
+    static Known all[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) {
+        k = &all[dev & 63];
+        if (k->status.load(std::memory_order_acquire)) return MX8_OK;
+        int* status = device_status_ptr();
+        if (!status) return MX8_ERR_CUDA;
+        e = cudaFuncSetAttribute(gemm_block128_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::dynamic);
+        if (e == cudaSuccess) {
+            k->status.store(status, std::memory_order_release);
+            return MX8_OK;
+        }
+    }
+    note_cuda_error("gemm_block128 setup", cudaGetErrorString(e));
+    return MX8_ERR_CUDA;
+}
+
+template <class C>
+struct Launch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    Launch(long long clusters, int size, cudaStream_t stream) {
+        cfg.gridDim = dim3(static_cast<unsigned>(clusters * size));
+        cfg.blockDim = dim3(C::THREADS);
+        cfg.dynamicSmemBytes = C::dynamic;
+        cfg.stream = stream;
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = static_cast<unsigned>(size);
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+    }
+};
+
+// clusters of `size` CTAs that can be resident at once; 0 when that cannot be found out
+template <class C>
+static int resident(int size) {
+    Known* k = nullptr;
+    if (known<C>(k) != MX8_OK) return 0;
+    int n = k->clusters[size].load(std::memory_order_relaxed);
+    if (n == 0) {
+        Launch<C> l(sm_count() * C::PER_SM / size, size, nullptr);
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_block128_kernel<C>, &l.cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        k->clusters[size].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Parts of K, a power of two, for `units` tiles: as many as still run at once.  A part has eight K blocks at least (eight blocks of a
+// 256 x 256 tile in two parts take 11.6 us, in one 10.9; sixteen 13.2 and 14.2), for few rows two.
+template <class C>
+static int split_for(long long units, int kblocks) {
+    int s = 1;
+    while (2 * s <= C::MAX_SPLIT && 2 * s * C::LEAST <= kblocks && units <= resident<C>(2 * s * C::CG)) s *= 2;
+    return s;
+}
+
 template <class C>
 static int launch(const Args& a, int split, cudaStream_t stream) {
     CUtensorMap mx, my;
@@ -708,6 +843,8 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
         if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, 128)) != MX8_OK) return rc;
         if ((rc = operand_map(&my, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, C::Y_BOX)) != MX8_OK) return rc;
     }
+    Known* k = nullptr;
+    if ((rc = known<C>(k)) != MX8_OK) return rc;
     Params p{};
     p.kblocks = (a.K + BK - 1) / BK;
     p.x_rows = C::SWAP ? a.N : a.M;
@@ -729,14 +866,7 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     p.wgrad = a.wgrad;
     p.rows_cap = a.wgrad ? a.K : a.M;
     p.split = split;
-    p.status = device_status_ptr();
-    if (!p.status) return MX8_ERR_CUDA;
-    auto kern = gemm_block128_kernel<C>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::dynamic);
-    if (e != cudaSuccess) {
-        note_cuda_error("cudaFuncSetAttribute(gemm_block128)", cudaGetErrorString(e));
-        return MX8_ERR_CUDA;
-    }
+    p.status = k->status.load(std::memory_order_relaxed);
     // tiles that there can be: with groups every one may add a partial tile
     long long tiles = static_cast<long long>(p.tiles_x) * p.tiles_y;
     if (a.wgrad) tiles *= a.groups;
@@ -746,22 +876,11 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
         return MX8_ERR_LIMIT;
     }
     const int cluster = C::CG * split;
-    long long units = tiles;
-    const long long resident = sm_count() / C::CG * C::PER_SM;
-    if (split == 1 && units > resident) units = resident;      // persistent; a split tile needs a cluster of its own
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::dynamic;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, mx, my, p);
+    long long clusters = tiles;
+    const long long most = sm_count() / C::CG * C::PER_SM;
+    if (!C::SPLIT && clusters > most) clusters = most;         // persistent; a split tile needs a cluster of its own
+    Launch<C> l(clusters, cluster, stream);
+    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, gemm_block128_kernel<C>, mx, my, p);
     if (e != cudaSuccess) {
         note_cuda_error("gemm_block128 launch", cudaGetErrorString(e));
         return MX8_ERR_CUDA;
@@ -769,25 +888,26 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     return MX8_OK;
 }
 
-// parts of K so that `units` tiles fill `room` places; a part has two K blocks at least, a cluster eight CTAs at most
-static int split_for(long long units, long long room, int kblocks, int most) {
-    long long s = units > 0 ? room / units : 1;
-    if (s > most) s = most;
-    if (s > kblocks / 2) s = kblocks / 2;
-    return s < 1 ? 1 : static_cast<int>(s);
+// the form with a split where that pays, else the one without
+template <class Whole, class Split>
+static int launch_either(const Args& a, long long units, cudaStream_t st) {
+    const int split = split_for<Split>(units, (a.K + BK - 1) / BK);
+    return split > 1 ? launch<Split>(a, split, st) : launch<Whole>(a, 1, st);
 }
 
 static int run(const Args& a, cudaStream_t st) {
-    const int kb = (a.K + BK - 1) / BK, sms = sm_count();
     const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256, m512 = (a.M + 511ll) / 512;
-    using Squares = Cfg<2, 1, 256, false, ROW>;
-    using Rows = Cfg<2, 2, 128, false, BOTH>;
-    using Few = Cfg<1, 1, 64, true, BOTH>;
+    using Squares = Cfg<2, 1, 256, false, ROW, false>;
+    using SquaresSplit = Cfg<2, 1, 256, false, ROW, true>;
+    using Rows = Cfg<2, 2, 128, false, BOTH, false>;
+    using RowsSplit = Cfg<2, 2, 128, false, BOTH, true>;
+    using Few = Cfg<1, 1, 64, true, BOTH, false>;
+    using FewSplit = Cfg<1, 1, 64, true, BOTH, true>;
     if (a.wgrad) return launch<Rows>(a, 1, st);
     if (a.groups > 0) return launch<Squares>(a, 1, st);
     // few rows: 128 weights a tile, two CTAs on a multiprocessor
-    if (a.M <= 64) return launch<Few>(a, split_for(n128, 2 * sms, kb, 8), st);
-    return a.b_square ? launch<Squares>(a, split_for(m256 * n256, sms / 2, kb, 4), st) : launch<Rows>(a, split_for(m512 * n128, sms / 2, kb, 4), st);
+    if (a.M <= 64) return launch_either<Few, FewSplit>(a, n128, st);
+    return a.b_square ? launch_either<Squares, SquaresSplit>(a, m256 * n256, st) : launch_either<Rows, RowsSplit>(a, m512 * n128, st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {
