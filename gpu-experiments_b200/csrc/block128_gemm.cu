@@ -17,9 +17,10 @@
 // X = B: the weights fill the lanes and a tile has as many columns (a multiple of 16) as there are rows of A.
 // Scales that vary by lane cost a register; scales that vary by column have to reach every lane through shared memory, 128 bytes a
 // cycle, which is why squares (one scale per 128 columns) have a form of their own (ROW).
-// split > 1: `split` CTAs or pairs of one cluster share a tile, each takes a part of the K blocks, and each adds up its share of the tile
-// in rank order: no workspace, no atomics, the same result in every run.  With SWAP the shares are sent by bulk copies from shared memory
-// to shared memory, otherwise each CTA reads the others' 16 bytes a lane.  (Words one by one cost 3 us read and 6 us sent for 64 rows.)
+// split > 1 (with SWAP): `split` CTAs of one cluster share a tile, each takes a part of the K blocks, sends the others their shares of the
+// tile by bulk copies from shared memory to shared memory, and adds up its own in rank order: no workspace, no atomics, the same result
+// in every run.  (Words one by one took 3 us read and 6 us sent for 64 rows.)  A 256 x 256 tile has four times the words to exchange:
+// splitting it gained nothing (32 blocks: 18.8 us whole, 19.4 in two parts), and tiles of 128 x 64 serve the shapes that it could.
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
 #include <atomic>
 
@@ -54,9 +55,9 @@ struct Cfg {
     static constexpr int TMEM_COLS = 2 * SUB * TN;
     static constexpr int D = 8;                               // blocks of scales in the ring
     static constexpr int SLOT = SUB * 128 + (SC == ROW ? 4 : TN);         // floats: X's rows, then Y's columns (ROW: two numbers)
-    static constexpr int TURN = SWAP || SPLIT ? 0 : 1024 / SUB;           // per promoting warp: where C is turned
+    static constexpr int TURN = SWAP ? 0 : 1024 / SUB;           // per promoting warp: where C is turned
     // where a split's shares of a tile arrive with SWAP: its columns, 128 rows each, from each of 2, 4 or 8 parts
-    static constexpr int PARTS = SWAP ? TN * 128 * 4 : 0;
+    static constexpr int PARTS = SPLIT ? TN * 128 * 4 : 0;
     static constexpr int turn_off = STAGES * STAGE + PARTS;
     static constexpr int ring_off = turn_off + EPI * TURN;
     static constexpr int bar_off = ring_off + D * SLOT * 4;
@@ -64,11 +65,9 @@ struct Cfg {
     static constexpr int misc_off = bar_off + n_bars * 8;     // TMEM address, abort flag
     static constexpr int seg_off = misc_off + 16;             // groups: first row, first tile
     static constexpr int dynamic = seg_off + (2 * MAX_GROUPS + 2) * 4;
-    static constexpr int MAX_SPLIT = 8 / CG;                  // a cluster of eight CTAs at most
-    static constexpr int LEAST = SWAP ? 2 : 8;                // K blocks of a part
     static constexpr int PER_SM = EPI == 16 ? 1 : 2;
     static_assert(dynamic * PER_SM <= 232448 - 1024 * (PER_SM - 1), "shared memory budget exceeded");
-    static_assert(SWAP ? TN * 512 <= STAGES * STAGE : 128 * SUB * (TN + 4) * 4 <= STAGES * STAGE, "a split adds its tiles up in the stage ring");
+    static_assert(!SPLIT || (SWAP && TN * 512 <= STAGES * STAGE), "a split sends its tile from the stage ring");
 };
 
 struct Params {
@@ -153,11 +152,6 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     return o;
 }
 
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 // contiguous bytes of this CTA's shared memory to a CTA of the cluster, counted on its barrier; 16-byte aligned
 __device__ __forceinline__ void bulk_send(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src), "r"(bytes), "r"(bar)
@@ -615,19 +609,9 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             [[maybe_unused]] const int cols = min(CW, ti.y_end - ti.y0 - col0);      // that exist
             if constexpr (C::SPLIT) {
                 // this CTA's MMAs are complete (its last accumulator arrived): the stage ring is free
-                if constexpr (C::SWAP) {
 #pragma unroll
-                    for (int i = 0; i < CW; ++i)
-                        if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[0][i];
-                } else {
-                    // rows of C, 16 bytes more than the columns: eight lanes' 16-byte pieces fall into different banks
-#pragma unroll
-                    for (int k = 0; k < C::SUB; ++k)
-#pragma unroll
-                        for (int i = 0; i < CW; i += 4)
-                            *reinterpret_cast<float4*>(base_ptr + ((k * 128 + r) * (C::TN + 4) + col0 + i) * 4) =
-                                make_float4(acc[k][i], acc[k][i + 1], acc[k][i + 2], acc[k][i + 3]);
-                }
+                for (int i = 0; i < CW; ++i)
+                    if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[0][i];
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
                 if (ti.x0 + r < p.x_rows) {
@@ -649,77 +633,33 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 
     if constexpr (C::SPLIT) {
         __syncwarp();
-        // (without register shares of their own the first four warps help)
-        constexpr int W0 = C::EPI == 16 ? EPI0 : 0, WARPS = C::THREADS / 32 - W0;
-        if constexpr (C::SWAP) {
-            // part j adds up columns yn j / split .. yn (j + 1) / split of the tile (rows of C): 512 bytes each, contiguous
-            const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-            const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
-            fence_proxy_async_smem();                                    // the tile's words, for the copies below
-            cluster_wait();                                              // every CTA's barriers are there
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
-                for (int j = 0; j < p.split; ++j) {
-                    const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
-                    if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
-                }
+        // part j adds up columns yn j / split .. yn (j + 1) / split of the tile (rows of C): 512 bytes each, contiguous
+        const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
+        const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
+        fence_proxy_async_smem();                                        // the tile's words, for the copies below
+        cluster_wait();                                                  // every CTA's barriers are there
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
+            for (int j = 0; j < p.split; ++j) {
+                const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
+                if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
             }
-            if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
-                const int r = (warp & 3) * 32 + lane;                    // a lane is a row of the tile (column of C)
-                const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
-                const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
-                for (int c = warp >> 2; c < mine; c += WARPS / 4) {
-                    float s = part == 0 ? own[c * 128] : in[c * 128];
-                    for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
-                    if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + first + c, ti.x0 + r, s);
-                }
-            }
-            __syncwarp();
-            cluster_arrive();                                            // this CTA has its shares: what was sent to it has been read
-            cluster_wait();
-        } else {
-            cluster_sync_all();                                          // every part's tile lies in its CTA's shared memory
-            if (warp >= W0) {
-                const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-                // part j adds up rows n j / split .. n (j + 1) / split; a lane has four columns
-                const int w = warp - W0, yn = ti.y_end - ti.y0, n = 128 * C::SUB, r1 = n * (part + 1) / p.split, esize = p.c_f32 ? 4 : 2;
-                const bool wide = (reinterpret_cast<uintptr_t>(p.c) % (4 * esize)) == 0 && p.ldc % 4 == 0;
-                for (int r = n * part / p.split + w; r < r1; r += WARPS) {
-                    const int row = ti.x0 + r + r / 128 * 128 * (CG - 1);
-                    if (row >= ti.x_end) break;
-#pragma unroll
-                    for (int c = 0; c < C::TN; c += 128) {
-                        const int col = c + lane * 4;
-                        float4 v[C::MAX_SPLIT];
-#pragma unroll
-                        for (int k = 0; k < C::MAX_SPLIT; ++k)
-                            if (k < p.split) v[k] = ld_cluster4(map_to_cta(base + (r * (C::TN + 4) + col) * 4, k * CG + pair_rank));
-                        float4 s = v[0];
-#pragma unroll
-                        for (int k = 1; k < C::MAX_SPLIT; ++k)
-                            if (k < p.split) {
-                                s.x += v[k].x;
-                                s.y += v[k].y;
-                                s.z += v[k].z;
-                                s.w += v[k].w;
-                            }
-                        const long long at = (ti.c_row + row) * p.ldc + ti.y0 + col;
-                        if (wide && col + 4 <= yn) {
-                            if (p.c_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.c) + at) = s;
-                            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.c) + at) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
-                        } else {
-                            const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (col + i < yn) store_c(p, ti.c_row + row, ti.y0 + col + i, f[i]);
-                        }
-                    }
-                }
-            }
-            __syncwarp();
-            cluster_sync_all();                                          // nobody leaves while its tile is read
         }
+        __syncwarp();
+        if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
+            const int r = (warp & 3) * 32 + lane;                        // a lane is a row of the tile (column of C)
+            const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
+            const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
+            for (int c = warp >> 2; c < mine; c += C::THREADS / 128) {
+                float s = part == 0 ? own[c * 128] : in[c * 128];
+                for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
+                if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + first + c, ti.x0 + r, s);
+            }
+        }
+        __syncwarp();
+        cluster_arrive();                                                // this CTA has its shares: what was sent to it has been read
+        cluster_wait();
     }
 
     if (*abort_flag) {
@@ -760,11 +700,10 @@ static int operand_map(CUtensorMap* m, const void* base, long long rows, int K, 
     return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// what the host keeps of a kernel for each device: the status word's address and, once the shared memory limit is raised, how many of its
-// clusters can be resident at once (two threads racing here find the same)
+// what the host keeps of a kernel for each device: the status word's address, once the shared memory limit is raised (two threads racing here
+// find the same)
 struct Known {
     std::atomic<int*> status;
-    std::atomic<int> clusters[9];              // by cluster size
 };
 
 template <class C>
@@ -785,50 +724,6 @@ static int known(Known*& k) {
     }
     note_cuda_error("gemm_block128 setup", cudaGetErrorString(e));
     return MX8_ERR_CUDA;
-}
-
-template <class C>
-struct Launch {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    Launch(long long clusters, int size, cudaStream_t stream) {
-        cfg.gridDim = dim3(static_cast<unsigned>(clusters * size));
-        cfg.blockDim = dim3(C::THREADS);
-        cfg.dynamicSmemBytes = C::dynamic;
-        cfg.stream = stream;
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = static_cast<unsigned>(size);
-        at[0].val.clusterDim.y = 1;
-        at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-    }
-};
-
-// clusters of `size` CTAs that can be resident at once; 0 when that cannot be found out
-template <class C>
-static int resident(int size) {
-    Known* k = nullptr;
-    if (known<C>(k) != MX8_OK) return 0;
-    int n = k->clusters[size].load(std::memory_order_relaxed);
-    if (n == 0) {
-        Launch<C> l(sm_count() * C::PER_SM / size, size, nullptr);
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_block128_kernel<C>, &l.cfg) != cudaSuccess) {
-            cudaGetLastError();
-            return 0;
-        }
-        k->clusters[size].store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
-
-// Parts of K, a power of two, for `units` tiles: as many as still run at once.  A part has eight K blocks at least (eight blocks of a
-// 256 x 256 tile in two parts take 11.6 us, in one 10.9; sixteen 13.2 and 14.2), for few rows two.
-template <class C>
-static int split_for(long long units, int kblocks) {
-    int s = 1;
-    while (2 * s <= C::MAX_SPLIT && 2 * s * C::LEAST <= kblocks && units <= resident<C>(2 * s * C::CG)) s *= 2;
-    return s;
 }
 
 template <class C>
@@ -879,8 +774,19 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     long long clusters = tiles;
     const long long most = sm_count() / C::CG * C::PER_SM;
     if (!C::SPLIT && clusters > most) clusters = most;         // persistent; a split tile needs a cluster of its own
-    Launch<C> l(clusters, cluster, stream);
-    const cudaError_t e = cudaLaunchKernelEx(&l.cfg, gemm_block128_kernel<C>, mx, my, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::dynamic;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_block128_kernel<C>, mx, my, p);
     if (e != cudaSuccess) {
         note_cuda_error("gemm_block128 launch", cudaGetErrorString(e));
         return MX8_ERR_CUDA;
@@ -888,26 +794,26 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     return MX8_OK;
 }
 
-// the form with a split where that pays, else the one without
-template <class Whole, class Split>
-static int launch_either(const Args& a, long long units, cudaStream_t st) {
-    const int split = split_for<Split>(units, (a.K + BK - 1) / BK);
-    return split > 1 ? launch<Split>(a, split, st) : launch<Whole>(a, 1, st);
-}
-
 static int run(const Args& a, cudaStream_t st) {
-    const long long n128 = (a.N + 127ll) / 128, n256 = (a.N + 255ll) / 256, m256 = (a.M + 255ll) / 256, m512 = (a.M + 511ll) / 512;
     using Squares = Cfg<2, 1, 256, false, ROW, false>;
-    using SquaresSplit = Cfg<2, 1, 256, false, ROW, true>;
     using Rows = Cfg<2, 2, 128, false, BOTH, false>;
-    using RowsSplit = Cfg<2, 2, 128, false, BOTH, true>;
     using Few = Cfg<1, 1, 64, true, BOTH, false>;
     using FewSplit = Cfg<1, 1, 64, true, BOTH, true>;
     if (a.wgrad) return launch<Rows>(a, 1, st);
     if (a.groups > 0) return launch<Squares>(a, 1, st);
-    // few rows: 128 weights a tile, two CTAs on a multiprocessor
-    if (a.M <= 64) return launch_either<Few, FewSplit>(a, n128, st);
-    return a.b_square ? launch_either<Squares, SquaresSplit>(a, m256 * n256, st) : launch_either<Rows, RowsSplit>(a, m512 * n128, st);
+    // Tiles of 128 weights x 64 rows (`small` of them, two CTAs on a multiprocessor, K in several parts) for few rows, and where large tiles would
+    // leave most of the device idle.  Measured, us, small tiles against large ones: squares 256 x 2048 x 4096 (64 small tiles) 15.5 and 20.2,
+    // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks, whose large tiles
+    // are 512 x 128, 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
+    const long long small = ((a.N + 127ll) / 128) * ((a.M + 63ll) / 64), sms = sm_count();
+    const int kb = (a.K + BK - 1) / BK;
+    if (a.M <= 64 || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
+        // Parts of K: 64 x 512 x 4096 (4 small tiles) takes 20.7, 14.8, 10.8, 8.7 us in 1, 2, 4, 8 parts, 64 x 8192 x 4096 (64) 21.7, 16.5, 16.0, 24.5:
+        // clusters of eight leave multiprocessors empty, so they are taken while one CTA for each is enough.
+        const int split = kb >= 8 && small * 8 <= sms + 16 ? 8 : kb >= 4 && small * 4 <= (kb >= 8 ? 2 * sms : sms) ? 4 : kb >= 8 && small <= sms ? 2 : 1;
+        return split > 1 ? launch<FewSplit>(a, split, st) : launch<Few>(a, 1, st);
+    }
+    return a.b_square ? launch<Squares>(a, 1, st) : launch<Rows>(a, 1, st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {

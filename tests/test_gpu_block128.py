@@ -145,7 +145,8 @@ def operands(M, N, K, b, seed=0):
 @pytest.mark.parametrize("b", ["square", "rows"])
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 128, 128), (1, 520, 1040), (3, 300, 100), (16, 256, 512), (17, 129, 272), (32, 1000, 640),
                                    (33, 64, 130), (64, 512, 384), (65, 100, 200), (128, 128, 128), (128, 256, 256), (129, 257, 144), (200, 72, 1000),
-                                   (300, 1030, 520), (1000, 640, 1152), (2100, 2304, 200)])
+                                   (300, 1030, 520), (1000, 640, 1152), (2100, 2304, 200), (70, 300, 2048), (150, 1000, 1100), (64, 128, 600),
+                                   (5, 2500, 1030), (40, 20000, 260), (600, 3000, 1024)])
 def test_product(shape, b):
     M, N, K = shape
     qa, sa, qb, sb, a64, b64 = operands(M, N, K, b, seed=M + N + K)
