@@ -2,8 +2,12 @@
 //   rows     1 x 128 along N (sc [E][ceil(N/128)][M], block-major so that 128 rows' scales are consecutive),
 //   columns  128 x 1 along M, with the bytes transposed (fp8_t [E][N][M], sc_t [E][ceil(M/128)][N]),
 //   squares  128 x 128 (sc [E][ceil(M/128)][ceil(N/128)]; the transposed form has the same scales, transposed).
-// amax = largest |x| of the block, at least 2^-110; scale = amax / 448; byte = e4m3(x * (448 / amax)): one rounding of the
-// reciprocal, one of the product (fp32, half a step of 2^-23 each), then the rounding to 3 bits that the format asks for.
+// amax = largest |x| of the block, at least 2^-110; scale = amax / 448; byte = e4m3(x * 448 / amax).
+// fp32 input keeps 448 / amax in two words, its rounding error in the second: the quotient is rounded once to fp32 before the rounding to
+// 3 bits.  With one word a few bytes in a million land on the other side of a border.  bf16 input needs one word: against a border t
+// (5 bits), 448 x and t amax are integers below 2^14 times a common power of two, so a quotient that is not on the border is at least
+// 2^-14 of itself away, and the two roundings on the way are 2^-23; a quotient right on a border goes to either of its two equally near
+// neighbours, as fl(x * fl(448 / amax)) falls.  (Two words there: 95 -> 104 us at 16391 x 7168 both ways.)
 // A block that holds an infinity or NaN gets that as its scale and dequantizes to NaN.
 //
 // Bound by HBM once the instructions are few: x is read once for both orientations.  A block of 8 warps owns a 128 x 128 tile.  Half a
@@ -45,14 +49,29 @@ __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
     return d;
 }
-// product of two pairs of floats
-__device__ __forceinline__ void mul2(uint64_t a, uint64_t b, float& lo, float& hi) {
+// 448 / amax in two words: the rounded quotient and what is missing from it
+struct Inverse {
+    float hi, lo;
+};
+template <bool TWO>
+__device__ __forceinline__ Inverse inverse_of(float amax) {
+    const float hi = __fdiv_rn(448.0f, amax);
+    return {hi, TWO ? fmaf(-amax, hi, 448.0f) * (hi * (1.0f / 448.0f)) : 0.0f};         // (448 - amax hi) / amax; the difference is exact
+}
+__device__ __forceinline__ uint64_t twice(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
+// a pair of floats times a pair of inverses (two words: rounded once but for 2^-48)
+struct Inverse2 {
+    uint64_t hi, lo;
+};
+__device__ __forceinline__ Inverse2 twice(Inverse v) { return {twice(v.hi), twice(v.lo)}; }
+template <bool TWO>
+__device__ __forceinline__ void mul2(uint64_t a, const Inverse2& b, float& lo, float& hi) {
     uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    if constexpr (!TWO) asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b.hi));
+    else asm("{\n\t.reg .b64 t;\n\tmul.rn.f32x2 t, %1, %3;\n\tfma.rn.f32x2 %0, %1, %2, t;\n\t}" : "=l"(d) : "l"(a), "l"(b.hi), "l"(b.lo));
     lo = __uint_as_float(static_cast<uint32_t>(d));
     hi = __uint_as_float(static_cast<uint32_t>(d >> 32));
 }
-__device__ __forceinline__ uint64_t twice(float v) { return pair(__float_as_uint(v), __float_as_uint(v)); }
 // the larger magnitude of two bf16 pairs, two floats; a NaN wins; the sign bits are arbitrary
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -100,10 +119,11 @@ template <typename T, bool ROW, bool COL, bool SQUARE>
 __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_block128_kernel(const Params p) {
     using E8 = Eight<T>;
     constexpr bool BF = sizeof(T) == 2;
-    constexpr int W = E8::WORDS;
+    constexpr int W = E8::WORDS, IW = BF ? 2 : 4;
     __shared__ alignas(16) uint8_t stage[COL ? B * B : 16];
     __shared__ alignas(16) uint32_t cmax[COL && !SQUARE ? WARPS * 16 * W : WARPS];
-    __shared__ alignas(16) float cinv[B];
+    // inverses of the columns: those of pair j of lane l's eight at IW (16 j + l), first words, then second ones
+    __shared__ alignas(16) float cinv[COL && !SQUARE ? B * IW / 2 : 4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l16 = lane & 15;
     // grid (GROUP_M * tiles_n, groups of tile rows, E): consecutive blocks walk down GROUP_M tile rows, then along N
     const int e = blockIdx.z, tn = blockIdx.x / GROUP_M, tm = blockIdx.y * GROUP_M + blockIdx.x % GROUP_M;
@@ -143,8 +163,8 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
         }
     }
 
-    float row_inv = 0.0f;                          // lanes r and r + 8 of a half: reciprocal scale of its row r
-    float tile_inv = 0.0f;
+    Inverse row_inv = {0.0f, 0.0f};                // lanes r and r + 8 of a half: reciprocal scale of its row r
+    Inverse tile_inv = {0.0f, 0.0f};
     if constexpr (SQUARE) {
         uint32_t a = v[0].w[0];
 #pragma unroll
@@ -160,7 +180,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) a = max(a, cmax[w]);
         const float amax = amax_of(a);
-        tile_inv = __fdiv_rn(448.0f, amax);
+        tile_inv = inverse_of<!BF>(amax);
         if (threadIdx.x == 0) {
             const float s = __fdiv_rn(amax, 448.0f);
             if (ROW) p.sc[(static_cast<size_t>(e) * p.tiles_m + tm) * p.tiles_n + tn] = s;
@@ -195,7 +215,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
             if (((lane & 7) >> (BF ? 1 : 0)) == i) mine = m[i];
         if constexpr (BF) mine = (lane & 1) ? mine & 0xFFFF0000u : mine << 16;
         const float amax = amax_of(mine);
-        row_inv = __fdiv_rn(448.0f, amax);
+        row_inv = inverse_of<!BF>(amax);
         if (l16 < 8 && m0 + l16 < p.M) p.sc[(static_cast<size_t>(e) * p.tiles_n + tn) * p.M + m0 + l16] = __fdiv_rn(amax, 448.0f);
     }
     if constexpr (ROW) {
@@ -203,10 +223,10 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
         const bool whole = p.vec_q && n0 + 8 <= p.N, inside = m0 + 8 <= p.M;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const uint64_t inv = twice(SQUARE ? tile_inv : __shfl_sync(0xFFFFFFFFu, row_inv, r, 16));
+            const Inverse2 inv = twice(SQUARE ? tile_inv : Inverse{__shfl_sync(0xFFFFFFFFu, row_inv.hi, r, 16), BF ? 0.0f : __shfl_sync(0xFFFFFFFFu, row_inv.lo, r, 16)});
             float f[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mul2(v[r].two(j), inv, f[2 * j], f[2 * j + 1]);
+            for (int j = 0; j < 4; ++j) mul2<!BF>(v[r].two(j), inv, f[2 * j], f[2 * j + 1]);
             const uint32_t lo = four_bytes(f[0], f[1], f[2], f[3]), hi = four_bytes(f[4], f[5], f[6], f[7]);
             if (inside || m0 + r < p.M) {
                 if (whole) {
@@ -221,11 +241,7 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
         }
     }
     if constexpr (COL) {
-        uint64_t inv[4];
-        if constexpr (SQUARE) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) inv[j] = twice(tile_inv);
-        } else {
+        if constexpr (!SQUARE) {
             uint32_t a[W];
 #pragma unroll
             for (int i = 0; i < W; ++i) {
@@ -246,20 +262,30 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
                 for (int w = 1; w < WARPS; ++w) m = E8::larger(m, cmax[w * 16 * W + (BF ? c >> 1 : c)]);
                 if constexpr (BF) m = (c & 1) ? m & 0xFFFF0000u : m << 16;
                 const float amax = amax_of(m);
-                cinv[c] = __fdiv_rn(448.0f, amax);
+                const Inverse v = inverse_of<!BF>(amax);
+                float* to = &cinv[((c >> 1 & 3) * 16 + (c >> 3)) * IW + (c & 1)];
+                to[0] = v.hi;
+                if constexpr (!BF) to[2] = v.lo;
                 if (tn * B + c < p.N) p.sc_t[(static_cast<size_t>(e) * p.tiles_m + tm) * p.N + tn * B + c] = __fdiv_rn(amax, 448.0f);
             }
             __syncthreads();
-            const ulonglong2 c0 = *reinterpret_cast<const ulonglong2*>(&cinv[l16 * 8]), c1 = *reinterpret_cast<const ulonglong2*>(&cinv[l16 * 8 + 4]);
-            inv[0] = c0.x; inv[1] = c0.y; inv[2] = c1.x; inv[3] = c1.y;
         }
         // the 8-byte piece k = 2 warp + half of column c's 128 bytes lies in slot k ^ (c / 8): sixteen lanes write sixteen different slots
         const int slot = (2 * warp + half) ^ l16;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            Inverse2 inv;
+            if constexpr (SQUARE) {
+                inv = twice(tile_inv);
+            } else if constexpr (BF) {
+                inv = {*reinterpret_cast<const uint64_t*>(&cinv[(j * 16 + l16) * IW]), 0};
+            } else {
+                const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(&cinv[(j * 16 + l16) * IW]);
+                inv = {both.x, both.y};
+            }
             float f[8], g[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) mul2(v[r].two(j), inv[j], f[r], g[r]);
+            for (int r = 0; r < 8; ++r) mul2<!BF>(v[r].two(j), inv, f[r], g[r]);
             st_shared_v2(smem_u32(stage) + (l16 * 8 + 2 * j) * B + slot * 8, four_bytes(f[0], f[1], f[2], f[3]), four_bytes(f[4], f[5], f[6], f[7]));
             st_shared_v2(smem_u32(stage) + (l16 * 8 + 2 * j + 1) * B + slot * 8, four_bytes(g[0], g[1], g[2], g[3]), four_bytes(g[4], g[5], g[6], g[7]));
         }

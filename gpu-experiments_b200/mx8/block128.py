@@ -16,7 +16,8 @@ def quantize_block128(x, return_normal=True, return_transposed=False, *, square=
     [.., ceil(M/128), ceil(N/128)] and x_sc_t its transpose.  Outputs not requested are None.
     row_index (int32 [rows], x 2-D): row r of the output is x[row_index[r]], zeros where the index is outside x: the rows of a routing
     schedule (token = peer_token_idx // topk, -1 for padding) are gathered while they are quantized.
-    scale = amax / 448 (amax at least 2^-110), byte = e4m3(x * (448 / amax)); a block with an infinity or NaN dequantizes to NaN.
+    scale = amax / 448 (amax at least 2^-110), byte = e4m3(x * 448 / amax), the quotient rounded to float32
+    (for bfloat16 x times the rounded 448 / amax: another byte only where the quotient lies midway between two); a block with an infinity or NaN dequantizes to NaN.
     """
     return host().quantize_block128(x, return_normal, return_transposed, square, row_index)
 

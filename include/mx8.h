@@ -289,7 +289,8 @@ MX8_API int mx8_moe_bwd_topk_weights(const void* d_output, const void* combine_b
                                      int tokens, int hidden, int topk, void* stream);
 
 /* Block-128 format: E4M3 bytes with one fp32 scale per block of 128 (row blocks 1 x 128, or squares of 128 x 128), any M, N >= 1.
- * scale = amax / 448 with amax the largest |x| of the block, at least 2^-110; byte = e4m3(x * (448 / amax)).
+ * scale = amax / 448 with amax the largest |x| of the block, at least 2^-110; byte = e4m3(x * 448 / amax), the quotient
+ * rounded to fp32; for bf16 input it is x * fl(448 / amax), which differs where the quotient lies midway between two bytes.
  *   x [E][M][N] (MX8_T_BF16 or MX8_T_F32), `ldx` elements between rows (matrices M * ldx apart);
  *   row_index (may be NULL; E == 1): int32 [M], row m is x[row_index[m]], zeros when that is outside [0, src_rows);
  *   fp8 [E][M][.] with pitch `ld` bytes, sc:       row blocks [E][ceil(N/128)][M], squares [E][ceil(M/128)][ceil(N/128)];

@@ -17,35 +17,39 @@ def bits(t):
     return t.contiguous().view(torch.uint8)
 
 
-def inverse(amax):
-    """448 / amax with one rounding (a Python number divided by a tensor is reciprocal times number: two)"""
-    return torch.full_like(amax, 448.0) / amax
+def quotient(x, amax, dtype):
+    """x * 448 / amax rounded to fp32: from 64 bits, or for bf16 input as x * fl(448 / amax).  (A Python number divided by a tensor would be
+    reciprocal times number: two roundings.)"""
+    if dtype == torch.bfloat16:
+        return x * (torch.full_like(amax, 448.0) / amax)
+    return (x.double() * 448.0 / amax.double()).float()
 
 
 def quant_ref(x, square=False):
-    """x [M, N] on the CPU -> (bytes, scales) by the definition in fp32: the kernel has to give the same bits"""
+    """x [M, N] on the CPU -> (bytes, scales) by the definition: the kernel has to give the same bits"""
+    dtype = x.dtype
     M, N = x.shape
     full = torch.zeros(cdiv(M) * 128, cdiv(N) * 128)
     full[:M, :N] = x.float()
     if square:
         t = full.view(cdiv(M), 128, cdiv(N), 128)
         amax = t.abs().amax((1, 3)).clamp(min=FLOOR)
-        q = (t * inverse(amax)[:, None, :, None]).view(full.shape)[:M, :N]
+        q = quotient(t, amax[:, None, :, None], dtype).view(full.shape)[:M, :N]
         return q.to(torch.float8_e4m3fn), amax / 448.0
     t = full.view(-1, cdiv(N), 128)
     amax = t.abs().amax(2).clamp(min=FLOOR)
-    q = (t * inverse(amax)[:, :, None]).view(full.shape)[:M, :N]
+    q = quotient(t, amax[:, :, None], dtype).view(full.shape)[:M, :N]
     return q.to(torch.float8_e4m3fn), (amax / 448.0)[:M].t().contiguous()
 
 
 def check_quant(x, square=False, row_index=None):
     q, sc, qt, sct = mx8.quantize_block128(x, True, True, square=square, row_index=row_index)
     assert mx8.device_status() == 0
-    xs = x.cpu().float()
+    xs = x.cpu()
     if row_index is not None:
         i = row_index.cpu().long()
         ok = (i >= 0) & (i < xs.shape[0])
-        xs = torch.where(ok[:, None], xs[torch.where(ok, i, 0)], 0.0)
+        xs = torch.where(ok[:, None], xs[torch.where(ok, i, 0)], torch.zeros((), dtype=xs.dtype))
     mats = xs if xs.dim() == 3 else xs[None]
     lead = x.dim() == 3
     for e in range(mats.shape[0]):
@@ -53,7 +57,7 @@ def check_quant(x, square=False, row_index=None):
         for got, got_sc, ref in ((q, sc, quant_ref(mats[e], square)), (qt, sct, quant_ref(mats[e].t().contiguous(), square))):
             assert torch.equal(pick(got_sc), ref[1])
             assert torch.equal(bits(pick(got)), bits(ref[0]))
-            # and against x itself in 64 bits: half a step of 3 bits (2^-4), or of the smallest step 2^-9 of a block, plus the two
+            # and against x itself in 64 bits: half a step of 3 bits (2^-4), or of the smallest step 2^-9 of a block, plus the
             # fp32 roundings on the way
             wide = torch.repeat_interleave(torch.repeat_interleave(ref[1].double(), 128, 0), 128, 1)[:got.shape[-2], :got.shape[-1]] if square \
                 else torch.repeat_interleave(ref[1].double().t(), 128, 1)[:, :got.shape[-1]]
@@ -72,6 +76,25 @@ def make_x(*shape, seed=0, dtype=torch.bfloat16):
     x[..., 0, :] = 0.0                                            # a row of zero blocks
     x.view(-1)[::97] *= 1000.0
     return x.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("square", [False, True])
+def test_quantize_gives_the_nearest_byte(square, dtype):
+    """No byte lies nearer to x * 448 / amax than the one given.  Slack: fp32 input is rounded to fp32 first (2^-24 of the quotient); for
+    bf16 that costs nothing, only the 64 bits of this check do (2^-51)."""
+    x = make_x(513, 640, seed=31, dtype=dtype)
+    q, sc, _, _ = mx8.quantize_block128(x, True, False, square=square)
+    t = torch.zeros(640, 640, dtype=torch.float64)
+    t[:513] = x.cpu().double()
+    t = t.view(5, 128, 5, 128) if square else t.view(640, 1, 5, 128)
+    exact = (t * 448.0 / t.abs().amax((1, 3), keepdim=True).clamp(min=FLOOR)).view(640, 640)[:513]
+    table = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    table = table[~table.isnan()].unique()
+    i = torch.searchsorted(table, exact).clamp(1, len(table) - 1)
+    nearest = torch.minimum((exact - table[i - 1]).abs(), (exact - table[i]).abs())
+    slack = 2.0 ** -51 if dtype == torch.bfloat16 else 2.0 ** -24
+    assert ((q.cpu().double() - exact).abs() <= nearest + slack * exact.abs()).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
