@@ -127,7 +127,7 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
         if (p.wgrad) {
             o.k0 = seg[lo] / BK;
             o.k1 = seg[lo + 1] / BK;
-            o.c_row = static_cast<long long>(lo) * p.x_rows;
+            o.c_row = static_cast<long long>(lo) * (C::SWAP ? p.y_rows : p.x_rows);
         } else {
             o.x0 = seg[lo];
             o.x_end = seg[lo + 1];
@@ -237,7 +237,7 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[C
     static_assert(R * PIECES % 32 == 0, "whole warps of pieces");
     uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * ES;
     const long long pitch = p.ldc * ES;
-    const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0, even = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 3) == 0;
     const int my_row = lane % R, piece = lane % PIECES;
     const uint32_t put = turn + my_row * WIDE + ((my_row % PIECES) << 4);
 #pragma unroll
@@ -258,23 +258,30 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[C
                 }
             }
             __syncwarp();
+            if (wide && cols - j >= PER) {
 #pragma unroll
-            for (int i = 0; i < R * PIECES / 32; ++i) {
-                const int r = i * (32 / PIECES) + lane / PIECES;
-                uint32_t w[4];
-                ld_shared_v4(turn + r * WIDE + ((piece ^ (r % PIECES)) << 4), w[0], w[1], w[2], w[3]);
-                uint8_t* to = c + (r0 + r) * pitch + j * ES + piece * 16;
-                const int left = cols - j - piece * (16 / ES);            // columns from this piece's first on
-                if (r0 + r >= rows || left <= 0) continue;
-                if (wide && left >= 16 / ES) {
-                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
+                for (int i = 0; i < R * PIECES / 32; ++i) {
+                    const int r = i * (32 / PIECES) + lane / PIECES;
+                    uint32_t w[4];
+                    ld_shared_v4(turn + r * WIDE + ((piece ^ (r % PIECES)) << 4), w[0], w[1], w[2], w[3]);
+                    if (r0 + r < rows) *reinterpret_cast<uint4*>(c + (r0 + r) * pitch + j * ES + piece * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+                // rows that do not start on 16-byte boundaries, or end inside: a word per lane, still consecutive
+                constexpr int WORDS = WIDE / 4;
+                const int word = lane % WORDS, left = cols - j - word * (4 / ES);
 #pragma unroll
-                    for (int e = 0; e < 16 / ES; ++e) {
-                        if (e < left) {
-                            if constexpr (F32) *reinterpret_cast<uint32_t*>(to + 4 * e) = w[e];
-                            else *reinterpret_cast<uint16_t*>(to + 2 * e) = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
-                        }
+                for (int i = 0; i < R * WORDS / 32; ++i) {
+                    const int r = i * (32 / WORDS) + lane / WORDS;
+                    uint32_t w;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * WIDE + (((word >> 2) ^ (r % PIECES)) << 4) + (word & 3) * 4));
+                    uint8_t* to = c + (r0 + r) * pitch + j * ES + word * 4;
+                    if (r0 + r >= rows || left <= 0) continue;
+                    if (F32 || (even && left >= 2)) {
+                        *reinterpret_cast<uint32_t*>(to) = w;
+                    } else {
+                        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
+                        if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
                     }
                 }
             }
@@ -617,7 +624,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 if (ti.x0 + r < p.x_rows) {
 #pragma unroll
                     for (int i = 0; i < CW; ++i)
-                        if (i < cols) store_c(p, ti.y0 + col0 + i, ti.x0 + r, acc[0][i]);
+                        if (i < cols) store_c(p, ti.c_row + ti.y0 + col0 + i, ti.x0 + r, acc[0][i]);
                 }
             } else {
 #pragma unroll
@@ -654,7 +661,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             for (int c = warp >> 2; c < mine; c += C::THREADS / 128) {
                 float s = part == 0 ? own[c * 128] : in[c * 128];
                 for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
-                if (ti.x0 + r < p.x_rows) store_c(p, ti.y0 + first + c, ti.x0 + r, s);
+                if (ti.x0 + r < p.x_rows) store_c(p, ti.c_row + ti.y0 + first + c, ti.x0 + r, s);
             }
         }
         __syncwarp();
@@ -799,15 +806,14 @@ static int run(const Args& a, cudaStream_t st) {
     using Rows = Cfg<2, 2, 128, false, BOTH, false>;
     using Few = Cfg<1, 1, 64, true, BOTH, false>;
     using FewSplit = Cfg<1, 1, 64, true, BOTH, true>;
-    if (a.wgrad) return launch<Rows>(a, 1, st);
-    if (a.groups > 0) return launch<Squares>(a, 1, st);
+    if (a.groups > 0 && !a.wgrad) return launch<Squares>(a, 1, st);
     // Tiles of 128 weights x 64 rows (`small` of them, two CTAs on a multiprocessor, K in several parts) for few rows, and where large tiles would
     // leave most of the device idle.  Measured, us, small tiles against large ones: squares 256 x 2048 x 4096 (64 small tiles) 15.5 and 20.2,
     // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks, whose large tiles
     // are 512 x 128, 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
-    const long long small = ((a.N + 127ll) / 128) * ((a.M + 63ll) / 64), sms = sm_count();
-    const int kb = (a.K + BK - 1) / BK;
-    if (a.M <= 64 || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
+    const int groups = a.wgrad ? a.groups : 1, kb = (a.K + BK - 1) / BK / groups;             // blocks of K, of a group on average
+    const long long small = ((a.N + 127ll) / 128) * ((a.M + 63ll) / 64) * groups, sms = sm_count();
+    if ((a.M <= 64 && !a.wgrad) || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
         // Parts of K: 64 x 512 x 4096 (4 small tiles) takes 20.7, 14.8, 10.8, 8.7 us in 1, 2, 4, 8 parts, 64 x 8192 x 4096 (64) 21.7, 16.5, 16.0, 24.5:
         // clusters of eight leave multiprocessors empty, so they are taken while one CTA for each is enough.
         const int split = kb >= 8 && small * 8 <= sms + 16 ? 8 : kb >= 4 && small * 4 <= (kb >= 8 ? 2 * sms : sms) ? 4 : kb >= 8 && small <= sms ? 2 : 1;
