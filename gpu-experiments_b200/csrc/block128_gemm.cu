@@ -22,6 +22,7 @@
 // in every run.  (Words one by one took 3 us read and 6 us sent for 64 rows.)  A 256 x 256 tile has four times the words to exchange:
 // splitting it gained nothing (32 blocks: 18.8 us whole, 19.4 in two parts), and tiles of 128 x 64 serve the shapes that it could.
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
+#include <algorithm>
 #include <atomic>
 
 #include "mx8_host.cuh"
@@ -831,8 +832,10 @@ static int check(const char* what, const Args& a, int c_dtype) {
         note_cuda_error(what, "M, N, K positive, operand pitches multiples of 16 bytes and at least a row long, scale and C pitches at least a row long");
         return MX8_ERR_SIZE;
     }
-    if (a.groups > MAX_GROUPS || static_cast<long long>(a.groups) * a.N > 0x7FFFFFFFll) {
-        note_cuda_error(what, "more than 256 groups, or more than 2^31 - 1 rows of B");
+    // a tile's last coordinates lie beyond the operands' and have to fit an int too
+    const int most = 0x7FFFF000;
+    if (a.groups > MAX_GROUPS || a.M > most || a.K > most || std::max(a.groups, 1) * static_cast<long long>(a.N) > most) {
+        note_cuda_error(what, "more than 256 groups, or more than 2^31 - 4096 rows of A, rows of B (of all groups) or columns of either");
         return MX8_ERR_LIMIT;
     }
     if (!aligned16(a.A) || !aligned16(a.B) || reinterpret_cast<uintptr_t>(a.A_sc) % 4 || reinterpret_cast<uintptr_t>(a.B_sc) % 4 ||

@@ -344,8 +344,8 @@ extern "C" int mx8_quantize_block128(const void* x, int dtype, int E, int M, int
     if (reinterpret_cast<uintptr_t>(x) % esize || reinterpret_cast<uintptr_t>(sc) % 4 || reinterpret_cast<uintptr_t>(sc_t) % 4 ||
         reinterpret_cast<uintptr_t>(row_index) % 4) return MX8_ERR_ALIGN;
     const long long tiles_m = (M + 127ll) / 128, tiles_n = (N + 127ll) / 128;
-    if (tiles_m > 65535ll * q128::GROUP_M || E > 65535) {
-        note_cuda_error("mx8_quantize_block128", "more than 65535 matrices or 67107840 rows");
+    if (tiles_m > 65535ll * q128::GROUP_M || E > 65535 || N > 0x7FFFF000) {       // a tile's last column has to fit an int
+        note_cuda_error("mx8_quantize_block128", "more than 65535 matrices, 67107840 rows or 2^31 - 4096 columns");
         return MX8_ERR_LIMIT;
     }
     int rc = check_device_sm100();

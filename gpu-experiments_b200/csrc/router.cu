@@ -797,8 +797,8 @@ extern "C" int mx8_moe_bwd_topk_weights(const void* d_output, const void* combin
     }
     if (router::misaligned(d_output, 2) || router::misaligned(combine_buffer, 2) || router::misaligned(topk_idx, 4) ||
         router::misaligned(d_topk_weights, 4)) return MX8_ERR_ALIGN;
-    if (topk > 65535 * router::WG_K) {
-        note_cuda_error("mx8_moe_bwd_topk_weights", "more than 524280 choices per token");
+    if (topk > 65535 * router::WG_K || hidden > 0x7FFFF000) {                    // a thread's next column has to fit an int
+        note_cuda_error("mx8_moe_bwd_topk_weights", "more than 524280 choices per token or 2^31 - 4096 columns");
         return MX8_ERR_LIMIT;
     }
     int rc = check_device_sm100();

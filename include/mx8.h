@@ -306,7 +306,7 @@ MX8_API int mx8_quantize_block128(const void* x, int dtype, int E, int M, int N,
  * of two scales has to lie within the range of fp32.
  * num_groups > 0: the rows of A are those of num_groups groups back to back, group_rows[g] of them (device int32, any size >= 0),
  * B [num_groups][N][K] with squares [num_groups][ceil(N/128)][ceil(K/128)]; rows of C behind the last group are left alone.  Sizes
- * that do not fit M are cut and set the device status word.  At most 256 groups. */
+ * that do not fit M are cut and set the device status word.  At most 256 groups; M, K and the rows of B at most 2^31 - 4096. */
 MX8_API int mx8_gemm_block128(const void* A, long long lda, const void* A_sc, long long ldsa, const void* B, long long ldb,
                               const void* B_sc, long long ldsb, int b_square, void* C, long long ldc, int M, int N, int K, int c_dtype,
                               const void* group_rows, int num_groups, void* stream);

@@ -46,6 +46,7 @@ def test_bwd_topk_weights_arguments(lib):
     assert f(P, P, None, P, 0, 8, 1, None) == _lib.ERR_SIZE
     assert f(P, P, None, P, 1, 8, 524281, None) == _lib.ERR_LIMIT
     assert f(P, P, ODD, P, 1, 8, 1, None) == _lib.ERR_ALIGN
+    assert f(P, P, None, P, 1, 2 ** 31 - 8, 1, None) == _lib.ERR_LIMIT
 
 
 def test_quantize_block128_arguments(lib):
@@ -59,6 +60,7 @@ def test_quantize_block128_arguments(lib):
         assert call(**bad) == _lib.ERR_SIZE, bad
     assert call(x=ODD, dtype=1) == _lib.ERR_ALIGN and call(sc=ODD) == _lib.ERR_ALIGN
     assert call(M=2 ** 31 - 1, N=2 ** 31 - 1, ldx=2 ** 31, ld=2 ** 31) == _lib.ERR_LIMIT
+    assert call(N=2 ** 31 - 1, ldx=2 ** 31, ld=2 ** 31) == _lib.ERR_LIMIT
 
 
 def test_gemm_block128_arguments(lib):
@@ -70,6 +72,9 @@ def test_gemm_block128_arguments(lib):
     for bad in ({"M": 0}, {"N": 0}, {"K": 0}, {"lda": 120}, {"ldb": 136}, {"lda": 112}, {"ldsa": 63}, {"sq": 0, "ldsb": 63}, {"ldc": 63}):
         assert call(**bad) == _lib.ERR_SIZE, bad
     assert call(G=257, gr=P) == _lib.ERR_LIMIT
+    top, wide = 2 ** 31 - 1, 2 ** 31
+    for huge in ({"M": top, "ldsa": wide}, {"N": top, "ldc": wide, "ldsb": wide}, {"K": top, "lda": wide, "ldb": wide}, {"G": 200, "gr": P, "N": 1 << 24, "ldc": wide}):
+        assert call(**huge) == _lib.ERR_LIMIT, huge
     assert call(A=ODD) == _lib.ERR_ALIGN and call(Bsc=ODD) == _lib.ERR_ALIGN and call(C=ODD, cd=1) == _lib.ERR_ALIGN
 
     def wgrad(A=P, lda=256, ldsa=64, M=64, N=64, R=256, cd=1, gr=P, G=2):

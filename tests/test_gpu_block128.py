@@ -1,4 +1,8 @@
 """Block-128 quantizer and matrix products against plain 64-bit forms, and the MoE layer built from them and the router."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -7,6 +11,7 @@ import mx8
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 FLOOR = 2.0 ** -110
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def cdiv(a):
@@ -328,6 +333,104 @@ def test_side_stream_and_graphs_at_once():
     assert mx8.device_status() == 0
     check_c(outs[0], a64, b64)
     check_c(outs[1], c64, d64)
+
+
+@pytest.mark.parametrize("b", ["square", "rows"])
+def test_product_on_many_large_tiles(b):
+    """more K blocks than the rings hold, more tiles than one wave for neither form of the scales"""
+    qa, sa, qb, sb, a64, b64 = operands(1500, 1700, 1300, b, seed=40)
+    for c in (torch.empty(1500, 1700, device=DEV), torch.empty(1500, 1701, dtype=torch.bfloat16, device=DEV)[:, 1:]):
+        mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks=b)
+        assert mx8.device_status() == 0
+        check_c(c, a64, b64)
+
+
+@pytest.mark.parametrize("sizes", [[1280, 0, 128, 1024], [128] * 9])
+def test_weight_gradient_on_large_tiles(sizes):
+    test_weight_gradient_product(sizes, (600, 1701))
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_offsets_beyond_32_bits(m):
+    """C that spans more than 2^32 elements is written where it should be and nowhere between"""
+    N, K, pitch = 72, 260, 2 ** 32 // m + 7
+    qa, sa, qb, sb, a64, b64 = operands(m + 1, N, K, "square", seed=m)
+    store = torch.full(((m + 1) * pitch,), 2.0, dtype=torch.bfloat16, device=DEV)
+    c = store.as_strided((m + 1, N), (pitch, 1))
+    mx8.gemm_block128(qa, sa, qb, sb, c)
+    assert mx8.device_status() == 0
+    check_c(c, a64, b64)
+    c.fill_(2.0)
+    assert all(bool((part == 2.0).all()) for part in store.split(2 ** 28))
+
+
+def test_quantize_beyond_32_bits():
+    """input and transposed bytes of more than 2^32 bytes: the last rows get what they get by themselves"""
+    N = 2 ** 27 + 24
+    x = torch.empty(33, N, dtype=torch.bfloat16, device=DEV)
+    for part in x.view(-1).split(2 ** 28):
+        part.copy_(torch.arange(part.numel(), device=DEV, dtype=torch.int32) % 509 - 254)
+    q, sc, qt, sct = mx8.quantize_block128(x, True, True)
+    n0 = 2 ** 27 - 256                                             # columns from a block's start on
+    a = mx8.quantize_block128(x[:, n0:].contiguous(), True, True)
+    assert torch.equal(bits(q[:, n0:]), bits(a[0])) and torch.equal(sc[n0 // 128:], a[1])
+    assert torch.equal(bits(qt[n0:]), bits(a[2])) and torch.equal(sct[:, n0:], a[3])
+
+
+FRESH = r"""
+import sys, threading
+sys.path.insert(0, ROOT + "/gpu-experiments_b200")
+import torch
+import mx8
+torch.zeros(1, device="cuda")                    # context only: the library's first calls race, or are captured
+g = torch.Generator().manual_seed(1)
+xs = [torch.randn(80 + 300 * i, 1200, generator=g).cuda() for i in range(4)]
+ws = [torch.randn(700, 1200, generator=g).cuda() for i in range(4)]
+ls = [torch.randn(3000, 64, generator=g).cuda() for i in range(4)]
+def work(i):
+    q, s, _, _ = mx8.quantize_block128(xs[i])
+    b, t, _, _ = mx8.quantize_block128(ws[i], square=True)
+    c = mx8.gemm_block128(q, s, b, t, torch.zeros(xs[i].shape[0], 700, device="cuda"))
+    r = mx8.router_topk(ls[i], 6)
+    return [c, *r, mx8.router_topk_bwd(ls[i], r[0], r[1], r[2], r[3], r[5], r[1])]
+torch.cuda.synchronize()
+got, errors = [None] * 4, []
+if MODE == "threads":
+    barrier = threading.Barrier(4)
+    def worker(i):
+        try:
+            s = torch.cuda.Stream()
+            barrier.wait()
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    got[i] = work(i)
+                s.synchronize()
+        except Exception as e:
+            errors.append(repr(e))
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(4)]
+    for t in threads: t.start()
+    for t in threads: t.join()
+else:
+    graphs = [torch.cuda.CUDAGraph() for _ in range(4)]
+    for i in range(4):
+        with torch.cuda.graph(graphs[i]):
+            got[i] = work(i)
+    for gr in graphs * 2:
+        gr.replay()
+torch.cuda.synchronize()
+assert not errors, errors
+assert mx8.device_status() == 0
+for i in range(4):
+    for a, b in zip(got[i], work(i)):
+        assert torch.equal(a, b)
+print("FRESH_OK")
+"""
+
+
+@pytest.mark.parametrize("mode", ["threads", "capture"])
+def test_first_calls_in_threads_and_under_capture(mode):
+    r = subprocess.run([sys.executable, "-c", f"ROOT, MODE = {ROOT!r}, {mode!r}\n" + FRESH], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and "FRESH_OK" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
 
 
 # ------------------------------------------------------------------------------------------------ together

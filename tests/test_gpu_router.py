@@ -285,3 +285,26 @@ def test_repeatable_on_a_side_stream_and_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(out + (out_d,), want + (want_d,)):
         assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    """logits, and rows of the routing weights' gradient, that span more than 2^32 elements"""
+    T, E = 130, 40
+    pitch = 2 ** 32 // T + 5
+    l = torch.zeros(T * pitch, dtype=torch.bfloat16, device=DEV).as_strided((T, E), (pitch, 1))
+    l.copy_(make_logits(T, E, torch.bfloat16, 33))
+    dense = l.contiguous()
+    want, got = mx8.router_topk(dense, 4), mx8.router_topk(l, 4)
+    dw = torch.randn(T, 4, device=DEV)
+    for a, b in zip(want + (mx8.router_topk_bwd(dense, want[0], want[1], want[2], want[3], want[5], dw),),
+                    got + (mx8.router_topk_bwd(l, got[0], got[1], got[2], got[3], got[5], dw),)):
+        assert torch.equal(a, b)
+    del l
+    T, H, k = 5, 2 ** 17 + 8, 6554                                 # T k H > 2^32
+    d = torch.ones(T, H, dtype=torch.bfloat16, device=DEV)
+    c = torch.zeros(T * k, H, dtype=torch.bfloat16, device=DEV)
+    c[-1, -1] = 3.0
+    c[-k, 0] = 5.0
+    want = torch.zeros(T, k)
+    want[-1, -1], want[-1, 0] = 3.0, 5.0
+    assert torch.equal(mx8.bwd_topk_weights(d, c).cpu(), want)
