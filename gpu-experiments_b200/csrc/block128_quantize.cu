@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t four_bytes(float a, float b, float c, float 
 
 // SQUARE: one scale for the tile; otherwise ROW / COL say which orientations have scales of their own
 template <typename T, bool ROW, bool COL, bool SQUARE>
-__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_block128_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 4 : 2) quantize_block128_kernel(const Params p) {
     using E8 = Eight<T>;
     constexpr bool BF = sizeof(T) == 2;
     constexpr int W = E8::WORDS, IW = BF ? 2 : 4;
@@ -241,6 +241,11 @@ __global__ void __launch_bounds__(32 * WARPS, sizeof(T) == 2 ? 3 : 2) quantize_b
         }
     }
     if constexpr (COL) {
+        // the words are the same as before, but must not be kept in their unpacked form from the rows' products on: twice the registers
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int i = 0; i < W; ++i) asm volatile("" : "+r"(v[r].w[i]));
         if constexpr (!SQUARE) {
             uint32_t a[W];
 #pragma unroll
