@@ -40,23 +40,25 @@ constexpr int EPI0 = 4;                       // the first promoting warp
 // ROW: Y's scale is one number per 128 columns.  BOTH: it varies by column.
 enum Scales { ROW, BOTH };
 
-template <int CG_, int SUB_, int TN_, bool SWAP_, Scales SC_, bool SPLIT_>
+template <int CG_, int TN_, bool SWAP_, Scales SC_, bool SPLIT_>
 struct Cfg {
-    static constexpr int CG = CG_, SUB = SUB_, TN = TN_;      // CTAs of a tile, 128-row parts of X in a CTA, rows of Y
+    static constexpr int CG = CG_, TN = TN_;                  // CTAs of a tile, rows of Y
     static constexpr bool SWAP = SWAP_, SPLIT = SPLIT_;       // SPLIT: a kernel of its own, as its code takes registers from the main loop (8192^3: 487 -> 540 us)
     static constexpr Scales SC = SC_;
-    static constexpr int EPI = SUB * TN / 64 * 4;             // promoting warps: 64 values a lane, in one row or in one row of each part
-    static constexpr int CW = 64 / SUB;                       // columns of a promoting warp, four lane quadrants for each
+    static constexpr int EPI = TN / 64 * 4;                   // promoting warps of 32 rows x 64 columns: four lane quadrants for each 64 columns
+    static constexpr int CW = 64;
+    static constexpr bool FRAG = EPI == 16 && SC != ROW;      // values of TMEM spread over a warp as 4 rows x 16 columns of a lane
     static constexpr int THREADS = 32 * (EPI0 + EPI);
-    static constexpr int ROWS = 128 * CG * SUB;               // rows of X of a tile
-    static constexpr int X_BYTES = SUB * 128 * BK, Y_BYTES = TN / CG * BK;
+    static constexpr int ROWS = 128 * CG;                     // rows of X of a tile
+    static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN / CG * BK;
     static constexpr int Y_BOX = SWAP ? 16 : TN / CG;         // rows of Y per TMA copy: with SWAP only boxes with rows are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
-    static constexpr int STAGES = EPI == 16 ? (SUB == 1 ? 6 : 5) : 3;
-    static constexpr int TMEM_COLS = 2 * SUB * TN;
+    static constexpr int STAGES = EPI == 16 ? (CG == 2 ? 6 : 4) : 3;
+    static constexpr int TMEM_COLS = 2 * TN;
     static constexpr int D = 8;                               // blocks of scales in the ring
-    static constexpr int SLOT = SUB * 128 + (SC == ROW ? 4 : TN);         // floats: X's rows, then Y's columns (ROW: two numbers)
-    static constexpr int TURN = SWAP ? 0 : 1024 / SUB;           // per promoting warp: where C is turned
+    static constexpr int XS = 128;                            // floats of a block: X's rows,
+    static constexpr int SLOT = XS + (SC == ROW ? 4 : TN);    // then Y's columns (ROW: two numbers)
+    static constexpr int TURN = EPI == 16 ? 1024 : 0;         // per promoting warp: where C is turned
     // where a split's shares of a tile arrive with SWAP: its columns, 128 rows each, from each of 2, 4 or 8 parts
     static constexpr int PARTS = SPLIT ? TN * 128 * 4 : 0;
     static constexpr int turn_off = STAGES * STAGE + PARTS;
@@ -92,8 +94,8 @@ struct Params {
 };
 
 struct Tile {
-    int x0, x_end;                            // first row of X of this CTA (its second part is 128 CG rows on), one past the matrix's or group's last
-    int y0, y_end, y_tma;                     // first row of Y inside its matrix, one past the tile's last, first row in the tensor map
+    int x0, x_end, x_tma;                     // first row of X of this CTA inside its matrix, one past the matrix's or group's last, first row in the tensor map
+    int y0, y_end, y_tma;                     // the same for Y, y_end being the tile's
     int ncols;                                // columns of the MMA (both CTAs together)
     int k0, k1;                               // K blocks
     long long c_row;                          // first row of C of this tile's matrix
@@ -114,8 +116,8 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
     o.k1 = p.kblocks;
     o.x0 = 0;
     o.x_end = p.x_rows;
-    int first = 0, tiles_x = p.tiles_x;
-    o.y_tma = 0;
+    int first = 0, tiles_x = p.tiles_x, tiles_y = p.tiles_y, y_first = 0, y_last = p.y_rows;
+    o.x_tma = o.y_tma = 0;
     if (p.groups > 0) {
         const int* firsts = seg + MAX_GROUPS + 1;
         int lo = 0, hi = p.groups - 1;                        // last group whose first tile is <= t: the one that has tile t
@@ -129,6 +131,11 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
             o.k0 = seg[lo] / BK;
             o.k1 = seg[lo + 1] / BK;
             o.c_row = static_cast<long long>(lo) * (C::SWAP ? p.y_rows : p.x_rows);
+        } else if constexpr (C::SWAP) {
+            y_first = seg[lo];
+            y_last = seg[lo + 1];
+            tiles_y = (y_last - y_first + C::TN - 1) / C::TN;
+            o.x_tma = lo * p.x_rows;
         } else {
             o.x0 = seg[lo];
             o.x_end = seg[lo + 1];
@@ -137,13 +144,14 @@ __device__ __forceinline__ Tile tile_at(int t, const Params& p, const int* seg, 
         }
     }
     // groups of `group_x` tile rows, column-major inside, so that CTAs running together share panels in L2
-    const int in_all = t - first, per = p.group_x * p.tiles_y;
+    const int in_all = t - first, per = p.group_x * tiles_y;
     const int grp = in_all / per, in = in_all - grp * per, n = min(p.group_x, tiles_x - grp * p.group_x);
     const int ty = in / n, tx = grp * p.group_x + in - ty * n;
     o.x0 += tx * C::ROWS + pair_rank * 128;
-    o.y0 = ty * C::TN;
+    o.y0 = y_first + ty * C::TN;
+    o.x_tma += o.x0;
     o.y_tma += o.y0;
-    o.y_end = min(o.y0 + C::TN, p.y_rows);
+    o.y_end = min(o.y0 + C::TN, y_last);
     o.ncols = round_cols<C::CG>(o.y_end - o.y0);
     if constexpr (C::SPLIT) {
         const int nk = o.k1 - o.k0, k0 = o.k0;
@@ -177,12 +185,28 @@ __device__ __forceinline__ void tc_wait16(uint32_t (&r)[16]) {
                  :
                  : "memory");
 }
-// 32 lanes x 8 columns at each of two addresses, and the wait for all loads
-__device__ __forceinline__ void tc_ld8x2(uint32_t t0, uint32_t t1, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(t0) : "memory");
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(t1) : "memory");
+// 32 lanes x 8 columns, lane l of the warp getting rows l / 4 + 8 i and columns 2 (l % 4) + {0, 1}: values 2 i and 2 i + 1
+__device__ __forceinline__ void tc_ld8_frag(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr + (16u << 16)) : "memory");
+}
+__device__ __forceinline__ void tc_wait8(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) : : "memory");
+}
+// pairs of floats
+__device__ __forceinline__ uint64_t pair(float a, float b) { return static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ float first_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float second_of(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
 }
 // four bytes, global -> shared, asynchronously; groups of copies complete in order
 __device__ __forceinline__ void copy4(uint32_t dst, const float* src) {
@@ -228,27 +252,58 @@ __device__ __forceinline__ void store_c(const Params& p, long long row, int col,
     else static_cast<uint16_t*>(p.c)[at] = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
 }
 
-// One warp's 32 rows x CW columns of C (row = lane): turned through BYTES bytes of shared memory, a few rows at a time, so that a store covers
-// 64 or 128 consecutive bytes of a row (16 per lane).  The 16-byte piece k of row r lies in slot k ^ (r % pieces): conflict-free both ways.
-// (All 32 rows at once and 32 bytes of each took 3 us a tile: a store then touches 16 lines.)
-template <int CW, int BYTES, bool F32>
-__device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[CW], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
-    constexpr int ES = F32 ? 4 : 2, WIDE = CW * ES < 128 ? CW * ES : 128;  // bytes of a row in a pass
-    constexpr int PIECES = WIDE / 16, R = BYTES / WIDE, PER = WIDE / ES;   // 16-byte pieces of it, rows of a pass, columns of a pass
-    static_assert(R * PIECES % 32 == 0, "whole warps of pieces");
+// C leaves through 1 KB of shared memory of a warp, 128 bytes of eight rows at a time, so that a store covers 128 consecutive bytes of a
+// row (16 per lane).  (All 32 rows at once and 32 bytes of each took 3 us a tile: a store then touches 16 lines.)  The 16-byte piece k
+// of row r lies in slot k ^ swizzle(r), which keeps the ways in, below, and out conflict-free: the permutation sets rows that differ by
+// one apart by two slots, so that the 64-bit words of a fragment, two pieces to a row, miss each other too.
+__device__ __forceinline__ int swizzle(int r) { return ((r << 1) | (r >> 2)) & 7; }
+template <int ES>
+__device__ __forceinline__ void emit_rows(uint32_t turn, uint8_t* c, long long pitch, bool wide, bool even, int r0, int rows, int j, int cols, int lane) {
+    constexpr int PER = 128 / ES;
+    if (wide && cols - j >= PER) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = i * 4 + lane / 8, piece = lane % 8;
+            uint32_t w[4];
+            ld_shared_v4(turn + r * 128 + ((piece ^ swizzle(r)) << 4), w[0], w[1], w[2], w[3]);
+            if (r0 + r < rows) *reinterpret_cast<uint4*>(c + (r0 + r) * pitch + j * ES + piece * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+        // rows that do not start on 16-byte boundaries, or end inside: a word per lane, still consecutive
+        const int left = cols - j - lane * (4 / ES);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            uint32_t w;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * 128 + (((lane >> 2) ^ swizzle(r)) << 4) + (lane & 3) * 4));
+            uint8_t* to = c + (r0 + r) * pitch + j * ES + lane * 4;
+            if (r0 + r >= rows || left <= 0) continue;
+            if (ES == 4 || (even && left >= 2)) {
+                *reinterpret_cast<uint32_t*>(to) = w;
+            } else {
+                *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
+                if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
+            }
+        }
+    }
+}
+__device__ __forceinline__ void st_shared_b32(uint32_t a, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
+// 32 rows (one a lane) x 64 columns of C
+template <bool F32>
+__device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[64], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
+    constexpr int ES = F32 ? 4 : 2, PER = 128 / ES;
     uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * ES;
     const long long pitch = p.ldc * ES;
     const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0, even = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 3) == 0;
-    const int my_row = lane % R, piece = lane % PIECES;
-    const uint32_t put = turn + my_row * WIDE + ((my_row % PIECES) << 4);
+    const uint32_t put = turn + (lane & 7) * 128 + (swizzle(lane & 7) << 4);
 #pragma unroll
-    for (int j = 0; j < CW; j += PER) {
+    for (int j = 0; j < 64; j += PER) {
 #pragma unroll 1
-        for (int r0 = 0; r0 < rows; r0 += R) {
+        for (int r0 = 0; r0 < rows; r0 += 8) {
             __syncwarp();
-            if (lane / R * R == r0) {
+            if ((lane & ~7) == r0) {
 #pragma unroll
-                for (int k = 0; k < PIECES; ++k) {
+                for (int k = 0; k < 8; ++k) {
                     uint32_t w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -259,33 +314,35 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[C
                 }
             }
             __syncwarp();
-            if (wide && cols - j >= PER) {
+            emit_rows<ES>(turn, c, pitch, wide, even, r0, rows, j, cols, lane);
+        }
+    }
+    __syncwarp();
+}
+
+// The same from a fragment: acc[8 columns of 64][row of a lane: l / 4 + 8 i]
+template <bool F32>
+__device__ __forceinline__ void write_rows_frag(const Params& p, const uint64_t (&acc)[8][4], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
+    constexpr int ES = F32 ? 4 : 2;
+    uint8_t* c = static_cast<uint8_t*>(p.c) + (row0 * p.ldc + col0) * ES;
+    const long long pitch = p.ldc * ES;
+    const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0, even = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 3) == 0;
+    const int sw = swizzle(lane >> 2) << 4;
+    const uint32_t put = turn + (lane >> 2) * 128;
 #pragma unroll
-                for (int i = 0; i < R * PIECES / 32; ++i) {
-                    const int r = i * (32 / PIECES) + lane / PIECES;
-                    uint32_t w[4];
-                    ld_shared_v4(turn + r * WIDE + ((piece ^ (r % PIECES)) << 4), w[0], w[1], w[2], w[3]);
-                    if (r0 + r < rows) *reinterpret_cast<uint4*>(c + (r0 + r) * pitch + j * ES + piece * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            } else {
-                // rows that do not start on 16-byte boundaries, or end inside: a word per lane, still consecutive
-                constexpr int WORDS = WIDE / 4;
-                const int word = lane % WORDS, left = cols - j - word * (4 / ES);
+    for (int i = 0; i < 4; ++i) {
+        if (8 * i >= rows) break;
 #pragma unroll
-                for (int i = 0; i < R * WORDS / 32; ++i) {
-                    const int r = i * (32 / WORDS) + lane / WORDS;
-                    uint32_t w;
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(turn + r * WIDE + (((word >> 2) ^ (r % PIECES)) << 4) + (word & 3) * 4));
-                    uint8_t* to = c + (r0 + r) * pitch + j * ES + word * 4;
-                    if (r0 + r >= rows || left <= 0) continue;
-                    if (F32 || (even && left >= 2)) {
-                        *reinterpret_cast<uint32_t*>(to) = w;
-                    } else {
-                        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(w);
-                        if (left >= 2) *reinterpret_cast<uint16_t*>(to + 2) = static_cast<uint16_t>(w >> 16);
-                    }
-                }
+        for (int half = 0; half < (F32 ? 2 : 1); ++half) {
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < (F32 ? 4 : 8); ++j) {
+                const uint64_t v = acc[4 * half + j][i];
+                if constexpr (F32) asm volatile("st.shared.b64 [%0], %1;" ::"r"(put + (((2 * j + ((lane >> 1) & 1)) << 4) ^ sw) + (lane & 1) * 8), "l"(v) : "memory");
+                else st_shared_b32(put + ((j << 4) ^ sw) + (lane & 3) * 4, pack_bf16x2(first_of(v), second_of(v)));
             }
+            __syncwarp();
+            emit_rows<ES>(turn, c, pitch, wide, even, 8 * i, rows, half * 32, cols, lane);
         }
     }
     __syncwarp();
@@ -315,7 +372,7 @@ __device__ __forceinline__ void group_prefix(const Params& p, int* seg, int lane
         end += row;
         if (end > cap) bad = true;
         const int e = static_cast<int>(min(end, static_cast<long long>(cap))), b = static_cast<int>(min(end - n, static_cast<long long>(cap)));
-        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : (e - b + C::ROWS - 1) / C::ROWS * p.tiles_y;
+        int nt = g >= p.groups ? 0 : p.wgrad ? p.tiles_x * p.tiles_y : C::SWAP ? (e - b + C::TN - 1) / C::TN * p.tiles_x : (e - b + C::ROWS - 1) / C::ROWS * p.tiles_y;
         int tt = nt;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -401,7 +458,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             for (int t = unit; t < num_tiles && ok; t += units) {
                 const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
                 const int ny = ti.ncols / CG;                 // rows of Y of this CTA
-                const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x0, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y_tma + pair_rank * ny, 0);
+                const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x_tma, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y_tma + pair_rank * ny, 0);
                 const int k0 = __shfl_sync(0xFFFFFFFFu, ti.k0, 0), k1 = __shfl_sync(0xFFFFFFFFu, ti.k1, 0);
                 const int boxes = __shfl_sync(0xFFFFFFFFu, (ny + C::Y_BOX - 1) / C::Y_BOX, 0);
                 for (int kb = k0; kb < k1; ++kb) {
@@ -414,8 +471,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                             if constexpr (CG == 2) tma_load_2d_pair(to, m, kb * BK, y, bar);
                             else tma_load_2d(to, m, kb * BK, y, bar);
                         };
-#pragma unroll
-                        for (int i = 0; i < C::SUB; ++i) load(dst + i * 128 * BK, &tm_x, x0 + i * 128 * CG);
+                        load(dst, &tm_x, x0);
 #pragma unroll
                         for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i)
                             if (i < boxes) load(dst + C::X_BYTES + i * C::Y_BOX * BK, &tm_y, y0 + i * C::Y_BOX);
@@ -439,15 +495,12 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (!warp_wait(accfree0 + buf * 8, ((it >> 1) & 1) ^ 1, ab, DEV_TIMEOUT_TMEM_FREE)) { ok = false; break; }
                     tc_fence_after();
                     if (leader) {
-#pragma unroll
-                        for (int i = 0; i < C::SUB; ++i) {
-                            const uint32_t x = desc_sw128_lo(base + stage * C::STAGE + i * 128 * BK), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
-                            const uint32_t d = tmem + (buf * C::SUB + i) * C::TN;
-                            tc_mma_e4m3_lo<CG, 0>(d, x, y, idesc);
-                            tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
-                            tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
-                            tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
-                        }
+                        const uint32_t x = desc_sw128_lo(base + stage * C::STAGE), y = desc_sw128_lo(base + stage * C::STAGE + C::X_BYTES);
+                        const uint32_t d = tmem + buf * C::TN;
+                        tc_mma_e4m3_lo<CG, 0>(d, x, y, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 2, y + 2, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 4, y + 4, idesc);
+                        tc_mma_e4m3_lo<CG, 1>(d, x + 6, y + 6, idesc);
                         commit<CG>(accfull0 + buf * 8, first_rank);
                         commit<CG>(empty0 + stage * 8, first_rank);
                     }
@@ -464,13 +517,18 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             constexpr int NY = C::TN / 32;
             uint32_t m = 0;
             bool ok = true;
+            // block n's copies have landed
+            auto announce = [&](uint32_t n) {
+                __syncwarp();
+                arrive_lane0<1>(accfull0 + (n & 1) * 8, lane);
+            };
             auto complete = [&](uint32_t n) { return warp_wait(accfull0 + (n & 1) * 8, (n >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL); };
             for (int t = unit; t < num_tiles && ok; t += units) {
                 const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
                 // offsets instead of pointers for every copy: this warp has few registers
                 const int x_last = ti.x_end - 1 - lane, y_last = ti.y_end - 1 - lane;
                 const float *xk = p.xs + lane, *yk = p.ys + lane;
-                if (p.xs_square) xk += static_cast<long long>(min(ti.x0, p.x_rows - 1) / 128) * p.kblocks - lane;      // the tile's one number
+                if (p.xs_square) xk += (static_cast<long long>(ti.g) * ((p.x_rows + 127) / 128) + min(ti.x0, p.x_rows - 1) / 128) * p.kblocks - lane;      // the tile's one number
                 xk += ti.k0 * p.xs_k;
                 if constexpr (C::SC == ROW) {
                     const int nb = (p.y_rows + 127) / 128;                // lane 0, 1: the number of the tile's 128 columns
@@ -482,29 +540,27 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (m >= 5 && !complete(m - 5)) { ok = false; break; }
                     const uint32_t to = smem_u32(ring + (m & (D - 1)) * C::SLOT + lane);
 #pragma unroll
-                    for (int i = 0; i < 4 * C::SUB; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(ti.x0 + i * 32 + i / 4 * 128 * (CG - 1), x_last)));
+                    for (int i = 0; i < C::XS / 32; ++i) copy4(to + i * 128, xk + (p.xs_square ? 0 : min(ti.x0 + i * 32, x_last)));
                     if constexpr (C::SC == ROW) {
-                        if (lane < 2) copy4(to + C::SUB * 512, yk);
+                        if (lane < 2) copy4(to + C::XS * 4, yk);
                     } else {
 #pragma unroll
                         for (int i = 0; i < NY; ++i)
-                            if (i * 32 < ti.ncols) copy4(to + C::SUB * 512 + i * 128, yk + min(ti.y0 + i * 32, y_last));
+                            if (i * 32 < ti.ncols) copy4(to + C::XS * 4 + i * 128, yk + min(ti.y0 + i * 32, y_last));
                     }
                     copies_commit();
                     xk += p.xs_k;
                     yk += p.ys_k;
                     if (m >= 3) {
                         copies_wait<3>();
-                        __syncwarp();
-                        arrive_lane0<1>(accfull0 + ((m - 3) & 1) * 8, lane);
+                        announce(m - 3);
                     }
                 }
             }
             copies_wait<0>();
             for (uint32_t n = m < 3 ? 0 : m - 3; n < m && ok; ++n) {
                 if (n >= 2 && !complete(n - 2)) break;
-                __syncwarp();
-                arrive_lane0<1>(accfull0 + (n & 1) * 8, lane);
+                announce(n);
             }
         }
     } else {
@@ -519,7 +575,6 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
         const int r = q * 32 + lane;                                     // row of this CTA's tile
         uint32_t it = 0;                                                 // blocks of this CTA so far: buffer and ring slot follow from it
         bool ok = true;
-        const float* my_ring = ring + r;
         for (int t = unit; t < num_tiles && ok; t += units) {
             int blocks, mine;                                            // columns from this warp's first on; <= 0: it only takes part in the barriers
             {
@@ -527,29 +582,33 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 blocks = ti.k1 - ti.k0;
                 mine = ti.ncols - col0;
             }
-            float acc[C::SUB][CW];
+            float acc[C::FRAG ? 1 : CW];
+            uint64_t frag[8][4];                                         // FRAG: pairs of columns
 #pragma unroll
-            for (int i = 0; i < C::SUB * CW; ++i) acc[i / CW][i % CW] = 0.0f;
+            for (int i = 0; i < CW; ++i) {
+                if constexpr (!C::FRAG) acc[i] = 0.0f;
+                else if (i < 32) frag[i / 4][i % 4] = 0;
+            }
             for (; blocks > 0; --blocks, ++it) {
                 const uint32_t buf = it & 1;
                 if (!warp_wait(accfull0 + buf * 8, (it >> 1) & 1, ab, DEV_TIMEOUT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t src = my_tmem + buf * (C::SUB * C::TN);
-                const float* slot = my_ring + (it & (D - 1)) * C::SLOT;
+                const uint32_t src = my_tmem + buf * C::TN;
+                const float* slot = ring + (it & (D - 1)) * C::SLOT;
                 auto release = [&]() {                                   // the buffer's values are all in registers
                     tc_fence_before();
                     __syncwarp();
                     arrive_lane0<CG>(free_lead + buf * 8, lane);
                 };
-                uint32_t va[16], vb[16];
+                [[maybe_unused]] uint32_t va[16], vb[16];
                 if constexpr (C::SC == ROW) {
                     // 64 columns in four loads, two in flight
                     tc_ld16(src, va);
                     tc_ld16(src + 16, vb);
-                    const float s = slot[0] * slot[128 + (col0 >> 7) - r];
+                    const float s = slot[r] * slot[128 + (col0 >> 7)];
                     auto add = [&](const uint32_t (&v)[16], int c) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[0][c + i] = fmaf(__uint_as_float(v[i]), s, acc[0][c + i]);
+                        for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(v[i]), s, acc[c + i]);
                     };
                     tc_wait16(va);
                     tc_wait16(vb);
@@ -562,38 +621,32 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     release();
                     add(va, 32);
                     add(vb, 48);
-                } else if constexpr (C::SUB == 2) {
-                    // 32 columns of two rows, eight at a time; the next eight are on their way while these are added, and a column's
-                    // scale is read once for both rows
-                    tc_ld8x2(src, src + C::TN, va);
-                    const float s0 = slot[0], s1 = slot[128];
-                    auto add = [&](const uint32_t (&v)[16], int c) {
+                } else if constexpr (C::FRAG) {
+                    const float2* ys = reinterpret_cast<const float2*>(slot + C::XS + col0 + 2 * (lane & 3));
+                    float xs[4];                                         // of this lane's four rows
 #pragma unroll
-                        for (int i = 0; i < 8; i += 4) {
-                            const float4 y = *reinterpret_cast<const float4*>(slot - r + 256 + col0 + c + i);
-                            const float ys[4] = {y.x, y.y, y.z, y.w};
+                    for (int i = 0; i < 4; ++i) xs[i] = slot[q * 32 + 8 * i + (lane >> 2)];
+                    auto add = [&](const uint32_t (&v)[8], int j) {
+                        const float2 two = ys[4 * j];
+                        const uint64_t y = pair(two.x, two.y);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                acc[0][c + i + k] = fmaf(__uint_as_float(v[i + k]) * ys[k], s0, acc[0][c + i + k]);
-                                acc[1][c + i + k] = fmaf(__uint_as_float(v[8 + i + k]) * ys[k], s1, acc[1][c + i + k]);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t x = static_cast<uint64_t>(v[2 * i + 1]) << 32 | v[2 * i];
+                            frag[j][i] = fma2(mul2(x, y), pair(xs[i], xs[i]), frag[j][i]);
                         }
                     };
-                    tc_wait16(va);
-                    tc_ld8x2(src + 8, src + C::TN + 8, vb);
-                    add(va, 0);
-                    tc_wait16(vb);
-                    tc_ld8x2(src + 16, src + C::TN + 16, va);
-                    add(vb, 8);
-                    tc_wait16(va);
-                    tc_ld8x2(src + 24, src + C::TN + 24, vb);
-                    add(va, 16);
-                    tc_wait16(vb);
-                    release();
-                    add(vb, 24);
+                    uint32_t v[2][8];                                    // eight columns on their way while eight are added
+                    tc_ld8_frag(src, v[0]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        tc_wait8(v[j & 1]);
+                        if (j < 7) tc_ld8_frag(src + 8 * (j + 1), v[(j + 1) & 1]);
+                        else release();
+                        add(v[j & 1], j);
+                    }
                 } else {
                     if (mine <= 0) release();
-                    const float s = slot[0];
+                    const float s = slot[r];
 #pragma unroll
                     for (int c = 0; c < CW; c += 16) {
                         if (c >= mine) break;
@@ -602,10 +655,10 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                         if (c + 16 == CW || c + 16 >= mine) release();
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
-                            const float4 y = *reinterpret_cast<const float4*>(slot - r + 128 + col0 + c + i);
+                            const float4 y = *reinterpret_cast<const float4*>(slot + C::XS + col0 + c + i);
                             const float ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[0][c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s, acc[0][c + i + k]);
+                            for (int k = 0; k < 4; ++k) acc[c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s, acc[c + i + k]);
                         }
                     }
                 }
@@ -619,21 +672,22 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 // this CTA's MMAs are complete (its last accumulator arrived): the stage ring is free
 #pragma unroll
                 for (int i = 0; i < CW; ++i)
-                    if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[0][i];
+                    if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[i];
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
                 if (ti.x0 + r < p.x_rows) {
 #pragma unroll
                     for (int i = 0; i < CW; ++i)
-                        if (i < cols) store_c(p, ti.c_row + ti.y0 + col0 + i, ti.x0 + r, acc[0][i]);
+                        if (i < cols) store_c(p, ti.c_row + ti.y0 + col0 + i, ti.x0 + r, acc[i]);
                 }
             } else {
-#pragma unroll
-                for (int k = 0; k < C::SUB; ++k) {
-                    const int x0 = ti.x0 + k * 128 * CG + q * 32;
-                    const int rows = min(32, ti.x_end - x0);
-                    if (p.c_f32) write_rows<CW, C::TURN, true>(p, acc[k], turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
-                    else write_rows<CW, C::TURN, false>(p, acc[k], turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
+                const int x0 = ti.x0 + q * 32, rows = min(32, ti.x_end - x0);
+                if constexpr (!C::FRAG) {
+                    if (p.c_f32) write_rows<true>(p, acc, turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
+                    else write_rows<false>(p, acc, turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
+                } else {
+                    if (p.c_f32) write_rows_frag<true>(p, frag, turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
+                    else write_rows_frag<false>(p, frag, turn, ti.c_row + x0, rows, ti.y0 + col0, cols, lane);
                 }
             }
         }
@@ -641,28 +695,30 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
 
     if constexpr (C::SPLIT) {
         __syncwarp();
-        // part j adds up columns yn j / split .. yn (j + 1) / split of the tile (rows of C): 512 bytes each, contiguous
-        const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
-        const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
-        fence_proxy_async_smem();                                        // the tile's words, for the copies below
         cluster_wait();                                                  // every CTA's barriers are there
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
-            for (int j = 0; j < p.split; ++j) {
-                const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
-                if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
+        if (unit < num_tiles) {                                          // the same in the whole cluster; with groups there may be fewer tiles
+            // part j adds up columns yn j / split .. yn (j + 1) / split of the tile (rows of C): 512 bytes each, contiguous
+            const Tile ti = tile_at<C>(unit, p, seg, pair_rank, part);
+            const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
+            fence_proxy_async_smem();                                        // the tile's words, for the copies below
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
+                for (int j = 0; j < p.split; ++j) {
+                    const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
+                    if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
+                }
             }
-        }
-        __syncwarp();
-        if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
-            const int r = (warp & 3) * 32 + lane;                        // a lane is a row of the tile (column of C)
-            const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
-            const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
-            for (int c = warp >> 2; c < mine; c += C::THREADS / 128) {
-                float s = part == 0 ? own[c * 128] : in[c * 128];
-                for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
-                if (ti.x0 + r < p.x_rows) store_c(p, ti.c_row + ti.y0 + first + c, ti.x0 + r, s);
+            __syncwarp();
+            if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
+                const int r = (warp & 3) * 32 + lane;                        // a lane is a row of the tile (column of C)
+                const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
+                const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
+                for (int c = warp >> 2; c < mine; c += C::THREADS / 128) {
+                    float s = part == 0 ? own[c * 128] : in[c * 128];
+                    for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
+                    if (ti.x0 + r < p.x_rows) store_c(p, ti.c_row + ti.y0 + first + c, ti.x0 + r, s);
+                }
             }
         }
         __syncwarp();
@@ -708,6 +764,11 @@ static int operand_map(CUtensorMap* m, const void* base, long long rows, int K, 
     return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Tiles of grouped rows at the most: `across` for every `rows` of them, a partial one for every group, none without a row.
+static long long most_tiles(long long across, int M, int rows, int groups) {
+    return across * std::min<long long>(M, M / rows + groups);
+}
+
 // what the host keeps of a kernel for each device: the status word's address, once the shared memory limit is raised (two threads racing here
 // find the same)
 struct Known {
@@ -740,7 +801,7 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     const bool grouped = a.groups > 0 && !a.wgrad;
     int rc;
     if (C::SWAP) {
-        if ((rc = operand_map(&mx, a.B, a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
+        if ((rc = operand_map(&mx, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
         if ((rc = operand_map(&my, a.A, a.M, a.K, a.lda, C::Y_BOX)) != MX8_OK) return rc;
     } else {
         if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, 128)) != MX8_OK) return rc;
@@ -754,7 +815,7 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     p.y_rows = C::SWAP ? a.M : a.N;
     p.tiles_x = (p.x_rows + C::ROWS - 1) / C::ROWS;
     p.tiles_y = (p.y_rows + C::TN - 1) / C::TN;
-    p.group_x = 16 / C::SUB;                  // 4096 rows of X walked together stay in L2 with the Y panel
+    p.group_x = 16;                           // 4096 rows of X walked together stay in L2 with the Y panel
     const float* bs = a.B_sc;
     p.xs = C::SWAP ? bs : a.A_sc;
     p.xs_square = C::SWAP && a.b_square;
@@ -770,10 +831,10 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     p.rows_cap = a.wgrad ? a.K : a.M;
     p.split = split;
     p.status = k->status.load(std::memory_order_relaxed);
-    // tiles that there can be: with groups every one may add a partial tile
+    // tiles that there can be
     long long tiles = static_cast<long long>(p.tiles_x) * p.tiles_y;
     if (a.wgrad) tiles *= a.groups;
-    else if (grouped) tiles += static_cast<long long>(p.tiles_y) * a.groups;
+    else if (grouped) tiles = most_tiles(C::SWAP ? p.tiles_x : p.tiles_y, a.M, C::SWAP ? C::TN : C::ROWS, a.groups);
     if (tiles > 0x7FFFFFFFll / 16) {
         note_cuda_error("gemm_block128", "more than 2^27 tiles");
         return MX8_ERR_LIMIT;
@@ -803,24 +864,30 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
 }
 
 static int run(const Args& a, cudaStream_t st) {
-    using Squares = Cfg<2, 1, 256, false, ROW, false>;
-    using Rows = Cfg<2, 2, 128, false, BOTH, false>;
-    using Few = Cfg<1, 1, 64, true, BOTH, false>;
-    using FewSplit = Cfg<1, 1, 64, true, BOTH, true>;
-    if (a.groups > 0 && !a.wgrad) return launch<Squares>(a, 1, st);
+    using Squares = Cfg<2, 256, false, ROW, false>;
+    using Single = Cfg<1, 256, false, ROW, false>;
+    using Rows = Cfg<2, 256, false, BOTH, false>;
+    using Few = Cfg<1, 64, true, BOTH, false>;
+    using FewSplit = Cfg<1, 64, true, BOTH, true>;
     // Tiles of 128 weights x 64 rows (`small` of them, two CTAs on a multiprocessor, K in several parts) for few rows, and where large tiles would
     // leave most of the device idle.  Measured, us, small tiles against large ones: squares 256 x 2048 x 4096 (64 small tiles) 15.5 and 20.2,
-    // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks, whose large tiles
-    // are 512 x 128, 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
-    const int groups = a.wgrad ? a.groups : 1, kb = (a.K + BK - 1) / BK / groups;             // blocks of K, of a group on average
-    const long long small = ((a.N + 127ll) / 128) * ((a.M + 63ll) / 64) * groups, sms = sm_count();
-    if ((a.M <= 64 && !a.wgrad) || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
+    // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks
+    // 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
+    const bool grouped = a.groups > 0 && !a.wgrad;
+    const int matrices = a.wgrad ? a.groups : 1, kb = (a.K + BK - 1) / BK / matrices;         // blocks of K, of a group on average
+    const long long across = (a.N + 127ll) / 128, sms = sm_count();
+    const long long small = grouped ? most_tiles(across, a.M, 64, a.groups) : across * ((a.M + 63ll) / 64) * matrices;
+    if ((a.M <= 64 && a.groups == 0) || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
         // Parts of K: 64 x 512 x 4096 (4 small tiles) takes 20.7, 14.8, 10.8, 8.7 us in 1, 2, 4, 8 parts, 64 x 8192 x 4096 (64) 21.7, 16.5, 16.0, 24.5:
         // clusters of eight leave multiprocessors empty, so they are taken while one CTA for each is enough.
         const int split = kb >= 8 && small * 8 <= sms + 16 ? 8 : kb >= 4 && small * 4 <= (kb >= 8 ? 2 * sms : sms) ? 4 : kb >= 8 && small <= sms ? 2 : 1;
         return split > 1 ? launch<FewSplit>(a, split, st) : launch<Few>(a, 1, st);
     }
-    return a.b_square ? launch<Squares>(a, 1, st) : launch<Rows>(a, 1, st);
+    if (!a.b_square) return launch<Rows>(a, 1, st);
+    // Groups of fewer than 1024 rows on average: 128 rows a tile instead of the 256 of a pair, as half of a pair's last tile is empty
+    // more often than not.  The pair reads a third less from L2.  N = 2048, K = 7168, one CTA and pairs, us: 512 rows in 32 groups 87 and
+    // 132, 9001 rows 191 and 200, 16384 rows 325 and 346, 16384 rows in 8 groups 270 and 252.
+    return grouped && a.M / a.groups < 1024 ? launch<Single>(a, 1, st) : launch<Squares>(a, 1, st);
 }
 
 static int check(const char* what, const Args& a, int c_dtype) {

@@ -345,6 +345,27 @@ def test_product_on_many_large_tiles(b):
         check_c(c, a64, b64)
 
 
+@pytest.mark.parametrize("sizes,N,K", [([0, 1, 0, 130, 7, 0], 200, 1100), ([20] * 9, 700, 1100), ([20] * 8, 896, 1040), ([0, 0, 0], 130, 2048), ([64], 100, 4100),
+                                       ([1100, 0, 2200], 300, 1300), ([700, 3, 0, 129, 256, 128, 40], 600, 1300), ([0, 127, 64, 65, 0, 1], 1030, 1500)])
+def test_grouped_product_on_tiles_of_every_kind(sizes, N, K):
+    """few tiles, with K in eight, four and two parts; groups of many rows; tiles of one block and of pairs, more of them than one wave"""
+    G, cap = len(sizes), sum(sizes) + 37
+    qa, sa, _, _ = mx8.quantize_block128(make_x(cap, K, seed=cap))
+    qb, sb, _, _ = mx8.quantize_block128(make_x(G, N, K, seed=G, dtype=torch.float32) * 0.02, square=True)
+    grp = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    for store in (torch.full((cap, N), 5.0, device=DEV), torch.full((cap, N + 1), 5.0, dtype=torch.bfloat16, device=DEV)):
+        c = store[:, :N]
+        for _ in range(2):
+            mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=grp)
+        assert mx8.device_status() == 0
+        a64, at = rows64(qa, sa), 0
+        for g, n in enumerate(sizes):
+            if n:
+                check_c(c[at:at + n], a64[at:at + n], square64(qb[g], sb[g]), f"group {g}")
+            at += n
+        assert (c[at:] == 5.0).all() and (store[:, N:] == 5.0).all()
+
+
 @pytest.mark.parametrize("sizes", [[1280, 0, 128, 1024], [128] * 9])
 def test_weight_gradient_on_large_tiles(sizes):
     test_weight_gradient_product(sizes, (600, 1701))
