@@ -51,6 +51,8 @@ struct Cfg {
     static constexpr int THREADS = 32 * (EPI0 + EPI);
     static constexpr int ROWS = 128 * CG;                     // rows of X of a tile
     static constexpr int X_BYTES = 128 * BK, Y_BYTES = TN / CG * BK;
+    static constexpr bool PART = CG == 1 && !SWAP;            // tiles with few rows of X: of 32 that have none, nothing is fetched or promoted
+    static constexpr int X_BOX = PART ? 32 : 128;             // rows of X per TMA copy
     static constexpr int Y_BOX = SWAP ? 16 : TN / CG;         // rows of Y per TMA copy: with SWAP only boxes with rows are fetched
     static constexpr int STAGE = X_BYTES + Y_BYTES;
     static constexpr int STAGES = EPI == 16 ? (CG == 2 ? 6 : 4) : 3;
@@ -460,18 +462,21 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                 const int ny = ti.ncols / CG;                 // rows of Y of this CTA
                 const int x0 = __shfl_sync(0xFFFFFFFFu, ti.x_tma, 0), y0 = __shfl_sync(0xFFFFFFFFu, ti.y_tma + pair_rank * ny, 0);
                 const int k0 = __shfl_sync(0xFFFFFFFFu, ti.k0, 0), k1 = __shfl_sync(0xFFFFFFFFu, ti.k1, 0);
+                const int xboxes = C::PART ? __shfl_sync(0xFFFFFFFFu, min(4, (ti.x_end - ti.x0 + 31) / 32), 0) : 1;
                 const int boxes = __shfl_sync(0xFFFFFFFFu, (ny + C::Y_BOX - 1) / C::Y_BOX, 0);
                 for (int kb = k0; kb < k1; ++kb) {
                     if (!warp_wait(empty0 + stage * 8, ph ^ 1, ab, DEV_TIMEOUT_EMPTY)) { ok = false; break; }
                     if (leader) {
-                        const uint32_t dst = base + stage * C::STAGE, bytes = C::X_BYTES + boxes * C::Y_BOX * BK;
+                        const uint32_t dst = base + stage * C::STAGE, bytes = xboxes * C::X_BOX * BK + boxes * C::Y_BOX * BK;
                         if (CG == 1 || pair_rank == 0) mbar_arrive_expect_tx(full0 + stage * 8, CG * bytes);
                         const uint32_t bar = full_lead + stage * 8;
                         auto load = [&](uint32_t to, const CUtensorMap* m, int y) {
                             if constexpr (CG == 2) tma_load_2d_pair(to, m, kb * BK, y, bar);
                             else tma_load_2d(to, m, kb * BK, y, bar);
                         };
-                        load(dst, &tm_x, x0);
+#pragma unroll
+                        for (int i = 0; i < 128 / C::X_BOX; ++i)
+                            if (i < xboxes) load(dst + i * C::X_BOX * BK, &tm_x, x0 + i * C::X_BOX);
 #pragma unroll
                         for (int i = 0; i < C::TN / CG / C::Y_BOX; ++i)
                             if (i < boxes) load(dst + C::X_BYTES + i * C::Y_BOX * BK, &tm_y, y0 + i * C::Y_BOX);
@@ -580,7 +585,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             {
                 const Tile ti = tile_at<C>(t, p, seg, pair_rank, part);
                 blocks = ti.k1 - ti.k0;
-                mine = ti.ncols - col0;
+                mine = !C::PART || ti.x0 + q * 32 < ti.x_end ? ti.ncols - col0 : 0;
             }
             float acc[C::FRAG ? 1 : CW];
             uint64_t frag[8][4];                                         // FRAG: pairs of columns
@@ -601,7 +606,9 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     arrive_lane0<CG>(free_lead + buf * 8, lane);
                 };
                 [[maybe_unused]] uint32_t va[16], vb[16];
-                if constexpr (C::SC == ROW) {
+                if (C::PART && mine <= 0) {
+                    release();
+                } else if constexpr (C::SC == ROW) {
                     // 64 columns in four loads, two in flight
                     tc_ld16(src, va);
                     tc_ld16(src + 16, vb);
@@ -804,7 +811,7 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
         if ((rc = operand_map(&mx, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, 128)) != MX8_OK) return rc;
         if ((rc = operand_map(&my, a.A, a.M, a.K, a.lda, C::Y_BOX)) != MX8_OK) return rc;
     } else {
-        if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, 128)) != MX8_OK) return rc;
+        if ((rc = operand_map(&mx, a.A, a.M, a.K, a.lda, C::X_BOX)) != MX8_OK) return rc;
         if ((rc = operand_map(&my, a.B, grouped ? static_cast<long long>(a.groups) * a.N : a.N, a.K, a.ldb, C::Y_BOX)) != MX8_OK) return rc;
     }
     Known* k = nullptr;
