@@ -24,6 +24,7 @@
 // Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "mx8_host.cuh"
 #include "mx8_ptx.cuh"
@@ -750,6 +751,134 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
     }
 }
 
+// Single tokens: C[m][n] without tensor cores for a row or a few.  Bound by reading the weights and, for small ones, by the launch: no tensor
+// map, barrier or cluster has to be set up, which costs the tiles 4 us.  A block of up to eight warps owns four rows of B, which use each
+// value of A once it is decoded; a warp takes pieces of 512 k, 16 bytes a lane, which lie in one scale block; sums meet over the lanes
+// and then the warps in a fixed order.  E4M3 values are exact in fp16 and fma.f32.f16 adds their exact product to a float: 1.6 instructions
+// a weight for one row (decoding to floats: 2.4, 268 MB of weights in 53 instead of 44 us).  With groups a block works on one row of A
+// and looks up the row's group.
+constexpr int VEC_ROWS = 4;                   // rows of B of a block
+constexpr int VEC_K = 512;                    // k of a warp's piece
+struct VecParams {
+    const uint8_t *a, *b;
+    long long lda, ldb, ldsa, ldsb;
+    const float *sa, *sb;
+    int b_square, N, K;
+    Params c;                                 // C, its pitch and type, the groups, the status word
+};
+
+// 16 bytes of a row from k on, zeros behind the row's end (whatever lies there)
+__device__ __forceinline__ uint4 load16(const uint8_t* row, int k, int K) {
+    if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < K - k; ++i) w[i >> 2] |= static_cast<uint32_t>(row[k + i]) << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// four E4M3 bytes as halves (exact); two products of halves added to a float
+__device__ __forceinline__ void e4m3x4_to_half(uint32_t v, uint32_t (&h)[2]) {
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[0]) : "h"(static_cast<uint16_t>(v)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[1]) : "h"(static_cast<uint16_t>(v >> 16)));
+}
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+    float d;
+    asm("{\n\t.reg .f16 a0, a1, b0, b1;\n\t.reg .f32 t;\n\tmov.b32 {a0, a1}, %1;\n\tmov.b32 {b0, b1}, %2;\n\t"
+        "fma.rn.f32.f16 t, a0, b0, %3;\n\tfma.rn.f32.f16 %0, a1, b1, t;\n\t}" : "=f"(d) : "r"(a), "r"(b), "f"(c));
+    return d;
+}
+
+// the group that row m belongs to, -1 behind the last one; sizes that do not fit are cut as in group_prefix
+__device__ __forceinline__ int group_of(const Params& p, int m, int lane, bool& bad) {
+    long long row = 0;
+    int mine = -1;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+        const int raw = g0 + lane < p.groups ? p.group_rows[g0 + lane] : 0, n = max(0, min(raw, p.rows_cap));
+        bad |= raw != n;
+        long long end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xFFFFFFFFu, end, o);
+            if (lane >= o) end += u;
+        }
+        end += row;
+        bad |= end > p.rows_cap;
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, m >= end - n && m < end);
+        if (hit) mine = g0 + __ffs(hit) - 1;
+        row = __shfl_sync(0xFFFFFFFFu, end, 31);
+    }
+    return mine;
+}
+
+template <int MT, bool GROUPED>
+__global__ void __launch_bounds__(256) gemv_block128_kernel(const VecParams p) {
+    __shared__ float part[8][VEC_ROWS * MT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * VEC_ROWS, m0 = blockIdx.y * MT;
+    const int kblocks = (p.K + BK - 1) / BK;
+    long long g = 0;
+    if constexpr (GROUPED) {
+        bool bad = false;
+        g = group_of(p.c, m0, lane, bad);
+        if (bad) atomicCAS(p.c.status, 0, DEV_BAD_GROUPS);
+        if (g < 0) return;                                               // the same in the whole block
+    }
+    const int last = p.c.rows_cap - 1 - m0;                              // rows beyond it are it
+    const uint8_t *a = p.a + m0 * p.lda, *b[VEC_ROWS];
+#pragma unroll
+    for (int r = 0; r < VEC_ROWS; ++r) b[r] = p.b + (g * p.N + min(n0 + r, p.N - 1)) * p.ldb;
+    const float* sb = p.b_square ? p.sb + (g * ((p.N + BK - 1) / BK) + n0 / BK) * kblocks : p.sb + n0;
+    float acc[VEC_ROWS][MT];
+#pragma unroll
+    for (int i = 0; i < VEC_ROWS * MT; ++i) acc[i / MT][i % MT] = 0.0f;
+    for (int k = warp * VEC_K + lane * 16; k < p.K; k += static_cast<int>(blockDim.x) * 16) {
+        uint4 w[VEC_ROWS], x[MT];
+#pragma unroll
+        for (int r = 0; r < VEC_ROWS; ++r) w[r] = load16(b[r], k, p.K);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x[m] = load16(a + min(m, last) * p.lda, k, p.K);
+        const int kb = k / BK;
+        float xs[MT], ws[VEC_ROWS];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) xs[m] = p.sa[kb * p.ldsa + m0 + min(m, last)];
+#pragma unroll
+        for (int r = 0; r < VEC_ROWS; ++r) ws[r] = p.b_square ? (r ? ws[0] : sb[kb]) : sb[kb * p.ldsb + min(r, p.N - 1 - n0)];
+        float s[VEC_ROWS][MT];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto word = [i](const uint4& v) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; };
+            uint32_t xh[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) e4m3x4_to_half(word(x[m]), xh[m]);
+#pragma unroll
+            for (int r = 0; r < VEC_ROWS; ++r) {
+                uint32_t wh[2];
+                e4m3x4_to_half(word(w[r]), wh);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) s[r][m] = dot2(wh[h], xh[m][h], i || h ? s[r][m] : 0.0f);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < VEC_ROWS; ++r)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[r][m] = fmaf(s[r][m], xs[m] * ws[r], acc[r][m]);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC_ROWS * MT; ++i) {
+        float v = acc[i / MT][i % MT];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        if (lane == 0) part[warp][i] = v;
+    }
+    __syncthreads();
+    const int i = threadIdx.x;
+    if (i < VEC_ROWS * MT && n0 + i / MT < p.N && i % MT <= last) {
+        float v = part[0][i];
+        for (int w = 1; w < static_cast<int>(blockDim.x) / 32; ++w) v += part[w][i];
+        store_c(p.c, m0 + i % MT, n0 + i / MT, v);
+    }
+}
+
 struct Args {
     const void *A, *B;
     long long lda, ldb;
@@ -778,6 +907,7 @@ static long long most_tiles(long long across, int M, int rows, int groups) {
 
 // what the host keeps of a kernel for each device: the status word's address, once the shared memory limit is raised (two threads racing here
 // find the same)
+struct Vec {};                                // the kernel without tiles, among the Cfg
 struct Known {
     std::atomic<int*> status;
 };
@@ -792,7 +922,7 @@ static int known(Known*& k) {
         if (k->status.load(std::memory_order_acquire)) return MX8_OK;
         int* status = device_status_ptr();
         if (!status) return MX8_ERR_CUDA;
-        e = cudaFuncSetAttribute(gemm_block128_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::dynamic);
+        if constexpr (!std::is_same_v<C, Vec>) e = cudaFuncSetAttribute(gemm_block128_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::dynamic);
         if (e == cudaSuccess) {
             k->status.store(status, std::memory_order_release);
             return MX8_OK;
@@ -870,6 +1000,45 @@ static int launch(const Args& a, int split, cudaStream_t stream) {
     return MX8_OK;
 }
 
+static int launch_gemv(const Args& a, cudaStream_t st) {
+    VecParams p{};
+    p.a = static_cast<const uint8_t*>(a.A);
+    p.b = static_cast<const uint8_t*>(a.B);
+    p.lda = a.lda;
+    p.ldb = a.ldb;
+    p.ldsa = a.ldsa;
+    p.ldsb = a.ldsb;
+    p.sa = a.A_sc;
+    p.sb = a.B_sc;
+    p.b_square = a.b_square;
+    p.N = a.N;
+    p.K = a.K;
+    p.c.c = a.c;
+    p.c.ldc = a.ldc;
+    p.c.c_f32 = a.c_f32;
+    p.c.group_rows = a.group_rows;
+    p.c.groups = a.groups;
+    p.c.rows_cap = a.M;
+    Known* k = nullptr;
+    const int rc = known<Vec>(k);
+    if (rc != MX8_OK) return rc;
+    p.c.status = k->status.load(std::memory_order_relaxed);
+    const int warps = std::min(8, (a.K + VEC_K - 1) / VEC_K);
+    const int mt = a.groups > 0 || a.M == 1 ? 1 : a.M == 2 ? 2 : 4;
+    const dim3 grid((a.N + VEC_ROWS - 1) / VEC_ROWS, (a.M + mt - 1) / mt);
+    auto kern = a.groups > 0 ? gemv_block128_kernel<1, true>
+                : mt == 1    ? gemv_block128_kernel<1, false>
+                : mt == 2    ? gemv_block128_kernel<2, false>
+                             : gemv_block128_kernel<4, false>;
+    kern<<<grid, 32 * warps, 0, st>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        note_cuda_error("gemm_block128 launch", cudaGetErrorString(e));
+        return MX8_ERR_CUDA;
+    }
+    return MX8_OK;
+}
+
 static int run(const Args& a, cudaStream_t st) {
     using Squares = Cfg<2, 256, false, ROW, false>;
     using Single = Cfg<1, 256, false, ROW, false>;
@@ -881,6 +1050,12 @@ static int run(const Args& a, cudaStream_t st) {
     // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks
     // 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
     const bool grouped = a.groups > 0 && !a.wgrad;
+    // Single tokens, vectors against tiles (cold caches, us): N x K = 7168 x 2048, 1 row 10.2 and 14.4, 2 rows 12.3 and 14.4, 4 rows 16.4 and 15.2;
+    // 4096 x 2048, 4 rows 12.3 and 14.4, 8 rows 18.4 and 14.4; 1024 x 1024, 16 rows 8.2 and 12.3; 16384 x 16384, 1 row 61 and 68, 2 rows 68
+    // and 68.  Rows of groups share no weights: 2048 x 7168, 8 rows 38.9 and 44, 16 rows 57 and 44; 1024 x 1024, 16 rows 12.3 and 15.4, 32
+    // rows 16.4 and 14.4.
+    const long long nk = static_cast<long long>(a.N) * a.K;
+    if (!a.wgrad && (grouped ? a.M <= 8 || (a.M <= 32 && a.M * nk <= 25000000) : a.M <= 16 && (a.M - 1) * nk <= 30000000)) return launch_gemv(a, st);
     const int matrices = a.wgrad ? a.groups : 1, kb = (a.K + BK - 1) / BK / matrices;         // blocks of K, of a group on average
     const long long across = (a.N + 127ll) / 128, sms = sm_count();
     const long long small = grouped ? most_tiles(across, a.M, 64, a.groups) : across * ((a.M + 63ll) / 64) * matrices;

@@ -345,6 +345,45 @@ def test_product_on_many_large_tiles(b):
         check_c(c, a64, b64)
 
 
+@pytest.mark.parametrize("b", ["square", "rows"])
+@pytest.mark.parametrize("shape", [(1, 7, 15), (1, 5, 17), (1, 1030, 4111), (1, 130, 9000), (2, 129, 520), (3, 64, 2048), (4, 66, 513), (5, 200, 300), (16, 300, 1000),
+                                   (2, 7000, 5000), (9, 3000, 2000), (16, 2500, 900)])
+def test_single_tokens(shape, b):
+    """few rows, with rubbish behind the ends of A's and B's rows and around C; the last shapes have too many products for vectors"""
+    M, N, K = shape
+    qa, sa, qb, sb, a64, b64 = operands(M, N, K, b, seed=M + N + K)
+    pa, pb = (torch.full((t.shape[0], cdiv(K) * 128 + 16), 0x7F, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for t in (qa, qb))
+    pa[:, :K], pb[:, :K] = qa, qb
+    for dtype in (torch.bfloat16, torch.float32):
+        store = torch.full((M + 2, N + 3), 4.0, dtype=dtype, device=DEV)
+        c = store[1:M + 1, 1:N + 1]
+        mx8.gemm_block128(pa[:, :K], sa, pb[:, :K], sb, c, b_blocks=b)
+        assert mx8.device_status() == 0
+        check_c(c, a64, b64, f"{shape} {b} {dtype}")
+        c.fill_(4.0)
+        assert (store == 4.0).all()
+
+
+@pytest.mark.parametrize("sizes,cap", [([1], 1), ([0, 0, 1, 0], 2), ([2, 0, 3, 1], 8), ([0] * 40 + [1] + [0] * 30 + [4], 6), ([1] * 8, 8), ([0, 0], 3), ([5, 0, 11], 20)])
+def test_single_tokens_of_groups(sizes, cap):
+    G, N, K = len(sizes), 70, 600
+    qa, sa, _, _ = mx8.quantize_block128(make_x(cap, K, seed=cap))
+    qb, sb, _, _ = mx8.quantize_block128(make_x(G, N, K, seed=G, dtype=torch.float32) * 0.02, square=True)
+    c = torch.full((cap, N), 5.0, device=DEV)
+    mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=torch.tensor(sizes, dtype=torch.int32, device=DEV))
+    assert mx8.device_status() == 0
+    a64, at = rows64(qa, sa), 0
+    for g, n in enumerate(sizes):
+        if n:
+            check_c(c[at:at + n], a64[at:at + n], square64(qb[g], sb[g]), f"group {g}")
+        at += n
+    assert (c[at:] == 5.0).all()
+    for bad in ([cap + 1] + [0] * (G - 1), [-1] + [0] * (G - 1), [2 ** 31 - 1] * G):
+        mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=torch.tensor(bad, dtype=torch.int32, device=DEV))
+        with pytest.raises(mx8.Mx8Error):
+            mx8.device_status()
+
+
 @pytest.mark.parametrize("sizes,N,K", [([0, 1, 0, 130, 7, 0], 200, 1100), ([20] * 9, 700, 1100), ([20] * 8, 896, 1040), ([0, 0, 0], 130, 2048), ([64], 100, 4100),
                                        ([1100, 0, 2200], 300, 1300), ([700, 3, 0, 129, 256, 128, 40], 600, 1300), ([0, 127, 64, 65, 0, 1], 1030, 1500)])
 def test_grouped_product_on_tiles_of_every_kind(sizes, N, K):
