@@ -10,18 +10,23 @@
 //               accumulator's barrier beside the MMAs' commit, so that the promoting warps wait once a block
 //   4 .. 19     (or 4 .. 7) promote: each reads 32 lanes x 64 columns of the buffer, scales and adds them into registers while the
 //               MMAs of block kb + 1 fill the other buffer, and at the end writes its part of C
-// Sixteen promoting warps of 64 columns hide one another's waits; eight warps of 128 columns, with 232 registers each, took 1120
-// cycles a block, most of it in a chain of waits, against 512 of the MMAs.
+// The promotion bounds the kernel: 128 x 256 values a CTA and block take 740 cycles, of which the reads of TMEM are 256, the FMAs 256 and
+// the rest one probe of a barrier and the latency of the first read; the MMAs take 512.  Under the power limit the clock falls to 1.5 GHz.
+// 8192^3 took 848 us with one CTA a tile and 8 promoting warps, 656 with pairs, 547 with 16 warps of 64 columns that hide one
+// another's waits, 487 with the scales on the accumulator's barrier (cuBLAS in bf16 on the same device: 690 us).
 //
 // X is the operand whose rows are the lanes of TMEM, Y the one whose rows are its columns: X = A, Y = B.  For few rows of A (SWAP)
 // X = B: the weights fill the lanes and a tile has as many columns (a multiple of 16) as there are rows of A.
-// Scales that vary by lane cost a register; scales that vary by column have to reach every lane through shared memory, 128 bytes a
-// cycle, which is why squares (one scale per 128 columns) have a form of their own (ROW).
+// Scales that vary by lane cost a register; scales that vary by column would have to reach every lane through shared memory, 128 bytes a
+// cycle, 1024 cycles a block, where a lane has one row.  Squares (one scale per 128 columns) do not need them (ROW).  Where both vary,
+// the fragment loads of TMEM give a lane 4 rows x 16 columns (FRAG): 256 cycles of shared memory, at half the rate of TMEM.  Weight
+// gradients 16384 x 2048 x 7168 in 8 groups, fp32: 490 us with two rows of 32 columns a lane, 385 us so; squares would lose (253 to 290 us).
 // split > 1 (with SWAP): `split` CTAs of one cluster share a tile, each takes a part of the K blocks, sends the others their shares of the
 // tile by bulk copies from shared memory to shared memory, and adds up its own in rank order: no workspace, no atomics, the same result
 // in every run.  (Words one by one took 3 us read and 6 us sent for 64 rows.)  A 256 x 256 tile has four times the words to exchange:
 // splitting it gained nothing (32 blocks: 18.8 us whole, 19.4 in two parts), and tiles of 128 x 64 serve the shapes that it could.
-// Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups).
+// Shapes: dense; grouped (rows of A belong to groups with their own B, sizes on the device); weight gradient (K belongs to groups);
+// vectors (single tokens, a kernel of its own below).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
