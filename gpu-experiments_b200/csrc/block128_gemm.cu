@@ -304,6 +304,9 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[6
     const long long pitch = p.ldc * ES;
     const bool wide = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 15) == 0, even = ((reinterpret_cast<uintptr_t>(c) | static_cast<uintptr_t>(pitch)) & 3) == 0;
     const uint32_t put = turn + (lane & 7) * 128 + (swizzle(lane & 7) << 4);
+    uint32_t w[F32 ? 64 : 32];                               // converted once, not by the eight lanes of every pass
+#pragma unroll
+    for (int i = 0; i < (F32 ? 64 : 32); ++i) w[i] = F32 ? __float_as_uint(acc[i]) : pack_bf16x2(acc[2 * i % 64], acc[(2 * i + 1) % 64]);
 #pragma unroll
     for (int j = 0; j < 64; j += PER) {
 #pragma unroll 1
@@ -311,21 +314,49 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[6
             __syncwarp();
             if ((lane & ~7) == r0) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (F32) w[i] = __float_as_uint(acc[j + 4 * k + i]);
-                        else w[i] = pack_bf16x2(acc[j + 8 * k + 2 * i], acc[j + 8 * k + 2 * i + 1]);
-                    }
-                    st_shared_v4(put ^ (k << 4), w[0], w[1], w[2], w[3]);
-                }
+                for (int k = 0; k < 8; ++k) st_shared_v4(put ^ (k << 4), w[j / (4 / ES) + 4 * k], w[j / (4 / ES) + 4 * k + 1], w[j / (4 / ES) + 4 * k + 2], w[j / (4 / ES) + 4 * k + 3]);
             }
             __syncwarp();
             emit_rows<ES>(turn, c, pitch, wide, even, r0, rows, j, cols, lane);
         }
     }
     __syncwarp();
+}
+
+// One column of C: a lane's values are its rows.  (A branch on the type and an address of its own for every value made the code so long
+// that fetching it took 3 us of a single tile's 7.)
+__device__ __forceinline__ void put(float* to, float v) { *to = v; }
+__device__ __forceinline__ void put(uint16_t* to, float v) { *to = static_cast<uint16_t>(pack_bf16x2(v, 0.0f)); }
+// up to `left` of four values of a row, together where they can be
+__device__ __forceinline__ void put4(float* to, const float4& v, int left) {
+    if (left >= 4 && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+        *reinterpret_cast<float4*>(to) = v;
+    } else {
+        if (left > 0) to[0] = v.x;
+        if (left > 1) to[1] = v.y;
+        if (left > 2) to[2] = v.z;
+        if (left > 3) to[3] = v.w;
+    }
+}
+__device__ __forceinline__ void put4(uint16_t* to, const float4& v, int left) {
+    const uint32_t a = pack_bf16x2(v.x, v.y), b = pack_bf16x2(v.z, v.w);
+    if (left >= 4 && (reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(a, b);
+    } else {
+        if (left > 0) to[0] = static_cast<uint16_t>(a);
+        if (left > 1) to[1] = static_cast<uint16_t>(a >> 16);
+        if (left > 2) to[2] = static_cast<uint16_t>(b);
+        if (left > 3) to[3] = static_cast<uint16_t>(b >> 16);
+    }
+}
+template <class T>
+__device__ __forceinline__ void write_columns(T* to, long long pitch, const float (&acc)[64], int rows) {
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+        if (i >= rows) break;
+        put(to, acc[i]);
+        to += pitch;
+    }
 }
 
 // The same from a fragment: acc[8 columns of 64][row of a lane: l / 4 + 8 i]
@@ -688,10 +719,10 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     if (i < cols) *reinterpret_cast<float*>(base_ptr + (i * 128 + r) * 4) = acc[i];
             } else if constexpr (C::SWAP) {
                 // lanes are consecutive columns of C, registers its rows
+                const long long first = (ti.c_row + ti.y0 + col0) * p.ldc + ti.x0 + r;
                 if (ti.x0 + r < p.x_rows) {
-#pragma unroll
-                    for (int i = 0; i < CW; ++i)
-                        if (i < cols) store_c(p, ti.c_row + ti.y0 + col0 + i, ti.x0 + r, acc[i]);
+                    if (p.c_f32) write_columns(static_cast<float*>(p.c) + first, p.ldc, acc, cols);
+                    else write_columns(static_cast<uint16_t*>(p.c) + first, p.ldc, acc, cols);
                 }
             } else {
                 const int x0 = ti.x0 + q * 32, rows = min(32, ti.x_end - x0);
@@ -715,27 +746,37 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
             const int yn = ti.y_end - ti.y0, most = (yn + p.split - 1) / p.split, first = yn * part / p.split, mine = yn * (part + 1) / p.split - first;
             fence_proxy_async_smem();                                        // the tile's words, for the copies below
             __syncthreads();
-            if (threadIdx.x == 0) {
-                mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
-                for (int j = 0; j < p.split; ++j) {
-                    const int f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
-                    if (j != part && n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
-                }
+            if (threadIdx.x < p.split) {                                 // a lane for each CTA
+                const int j = threadIdx.x, f = yn * j / p.split, n = yn * (j + 1) / p.split - f;
+                if (j == part) mbar_arrive_expect_tx(shares, (p.split - 1) * mine * 512);
+                else if (n > 0) bulk_send(map_to_cta(base + S * C::STAGE + part * most * 512, j), base + f * 512, n * 512, map_to_cta(shares, j));
             }
             __syncwarp();
-            if (warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL)) {
-                const int r = (warp & 3) * 32 + lane;                        // a lane is a row of the tile (column of C)
-                const float* in = reinterpret_cast<const float*>(base_ptr + S * C::STAGE) + r;
-                const float* own = reinterpret_cast<const float*>(base_ptr) + first * 128 + r;
-                for (int c = warp >> 2; c < mine; c += C::THREADS / 128) {
-                    float s = part == 0 ? own[c * 128] : in[c * 128];
-                    for (int k = 1; k < p.split; ++k) s += k == part ? own[c * 128] : in[(k * most + c) * 128];
-                    if (ti.x0 + r < p.x_rows) store_c(p, ti.c_row + ti.y0 + first + c, ti.x0 + r, s);
+            const bool got = warp_wait(shares, 0, ab, DEV_TIMEOUT_FULL);
+            cluster_arrive();                                            // this CTA has its shares: what was sent to it has been read
+            if (got) {
+                // a warp sums a row of C, a lane four columns of it
+                const float4* in = reinterpret_cast<const float4*>(base_ptr + S * C::STAGE) + lane;
+                const float4* own = reinterpret_cast<const float4*>(base_ptr) + first * 32 + lane;
+                const int col = ti.x0 + lane * 4, left = p.x_rows - col;
+                for (int c = warp; c < mine; c += C::THREADS / 32) {
+                    float4 v[8];                                         // all parts' values are on their way together
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < p.split) v[k] = k == part ? own[c * 32] : in[(k * most + c) * 32];
+                    float4 s = v[0];
+#pragma unroll
+                    for (int k = 1; k < 8; ++k)
+                        if (k < p.split) s = make_float4(s.x + v[k].x, s.y + v[k].y, s.z + v[k].z, s.w + v[k].w);
+                    const long long to = (ti.c_row + ti.y0 + first + c) * p.ldc + col;
+                    if (p.c_f32) put4(static_cast<float*>(p.c) + to, s, left);
+                    else put4(static_cast<uint16_t*>(p.c) + to, s, left);
                 }
             }
+        } else {
+            cluster_arrive();
         }
         __syncwarp();
-        cluster_arrive();                                                // this CTA has its shares: what was sent to it has been read
         cluster_wait();
     }
 
