@@ -1091,10 +1091,11 @@ static int run(const Args& a, cudaStream_t st) {
     using Rows = Cfg<2, 256, false, BOTH, false>;
     using Few = Cfg<1, 64, true, BOTH, false>;
     using FewSplit = Cfg<1, 64, true, BOTH, true>;
-    // Tiles of 128 weights x 64 rows (`small` of them, two CTAs on a multiprocessor, K in several parts) for few rows, and where large tiles would
-    // leave most of the device idle.  Measured, us, small tiles against large ones: squares 256 x 2048 x 4096 (64 small tiles) 15.5 and 20.2,
-    // 300 x 2048 x 7168 (80) 26.5 and 29.7, 256 x 4096 x 4096 (128) 20.5 and 20.4, 256 x 2048 x 512 8.9 and 8.3; row blocks
-    // 512 x 2048 x 4096 (128) 19.2 and 30.1, 512 x 4096 x 4096 (256) 27.7 and 30.4.
+    // Tiles of 128 weights x 64 rows (`small` of them, two CTAs on a multiprocessor) for few rows, and where large tiles would leave much of
+    // the device idle: they start up faster (5 against 7 us for one block of K) and more of them run at once.  Measured, us, small tiles
+    // (in parts of K where they are taken) against large ones: squares 256 x 512 x 1024 (16 small tiles) 8.0 and 9.9, 512 x 1024 x 2048 (64)
+    // 10.9 and 13.1, 512 x 2048 (128) by 512 7.0 and 8.4, by 4096 19.4 and 19.9, 1024 x 2048 (256) by 512 8.5 and 8.6, by 1024 11.6 and 10.3,
+    // 1024 x 4096 (512) by 128 8.4 and 7.5; row blocks 1024 x 2048 x 4096 (256) 25 and 28, 1024 x 4096 x 1024 (512) 17.0 and 13.1.
     const bool grouped = a.groups > 0 && !a.wgrad;
     // Single tokens, vectors against tiles (cold caches, us): N x K = 7168 x 2048, 1 row 10.2 and 14.4, 2 rows 12.3 and 14.4, 4 rows 16.4 and 15.2;
     // 4096 x 2048, 4 rows 12.3 and 14.4, 8 rows 18.4 and 14.4; 1024 x 1024, 16 rows 8.2 and 12.3; 16384 x 16384, 1 row 61 and 68, 2 rows 68
@@ -1105,10 +1106,12 @@ static int run(const Args& a, cudaStream_t st) {
     const int matrices = a.wgrad ? a.groups : 1, kb = (a.K + BK - 1) / BK / matrices;         // blocks of K, of a group on average
     const long long across = (a.N + 127ll) / 128, sms = sm_count();
     const long long small = grouped ? most_tiles(across, a.M, 64, a.groups) : across * ((a.M + 63ll) / 64) * matrices;
-    if ((a.M <= 64 && a.groups == 0) || (a.b_square ? kb >= 8 && small * 7 <= 4 * sms : small <= 2 * sms)) {
-        // Parts of K: 64 x 512 x 4096 (4 small tiles) takes 20.7, 14.8, 10.8, 8.7 us in 1, 2, 4, 8 parts, 64 x 8192 x 4096 (64) 21.7, 16.5, 16.0, 24.5:
-        // clusters of eight leave multiprocessors empty, so they are taken while one CTA for each is enough.
-        const int split = kb >= 8 && small * 8 <= sms + 16 ? 8 : kb >= 4 && small * 4 <= (kb >= 8 ? 2 * sms : sms) ? 4 : kb >= 8 && small <= sms ? 2 : 1;
+    if ((a.M <= 64 && a.groups == 0) || small <= sms || (small <= 2 * sms && (kb <= 4 || !a.b_square))) {
+        // Parts of K, where they find multiprocessors of their own, and for a long K places beside others: 256 x 512 (16 small tiles), one part and
+        // eight: 8.5 and 8.0 us by 1024, 28.9 and 12.4 by 7168; 512 x 1024 (64), one part, two and four: 8.8, 9.0, 10.1 by 1024, 19.1, 14.4, 14.3
+        // by 4096, 29.6, 19.6, 18.3 by 7168.
+        const long long room = kb >= 32 ? 2 * sms : sms + 16;
+        const int split = kb < 8 ? 1 : small * 8 <= room ? 8 : kb < 10 ? 1 : small * 4 <= room ? 4 : small * 2 <= room ? 2 : 1;
         return split > 1 ? launch<FewSplit>(a, split, st) : launch<Few>(a, 1, st);
     }
     if (!a.b_square) return launch<Rows>(a, 1, st);

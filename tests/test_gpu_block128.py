@@ -336,6 +336,21 @@ def test_side_stream_and_graphs_at_once():
 
 
 @pytest.mark.parametrize("b", ["square", "rows"])
+@pytest.mark.parametrize("shape", [(300, 1500, 1500), (320, 1000, 1400), (200, 500, 1030), (400, 1100, 4200), (700, 1601, 640)])
+def test_product_in_parts(shape, b):
+    """small tiles with K in two, four and eight parts, two parts of a long K, and whole"""
+    qa, sa, qb, sb, a64, b64 = operands(*shape, b, seed=sum(shape))
+    c = torch.full((shape[0], shape[1] + 1), 6.0, dtype=torch.bfloat16, device=DEV)
+    mx8.gemm_block128(qa, sa, qb, sb, c[:, 1:], b_blocks=b)
+    assert mx8.device_status() == 0
+    check_c(c[:, 1:], a64, b64)
+    again = torch.empty(shape[0], shape[1], device=DEV)
+    mx8.gemm_block128(qa, sa, qb, sb, again, b_blocks=b)
+    check_c(again, a64, b64)
+    assert (c[:, 0] == 6.0).all()
+
+
+@pytest.mark.parametrize("b", ["square", "rows"])
 def test_product_on_many_large_tiles(b):
     """more K blocks than the rings hold, more tiles than one wave for neither form of the scales"""
     qa, sa, qb, sb, a64, b64 = operands(1500, 1700, 1300, b, seed=40)
@@ -385,7 +400,9 @@ def test_single_tokens_of_groups(sizes, cap):
 
 
 @pytest.mark.parametrize("sizes,N,K", [([0, 1, 0, 130, 7, 0], 200, 1100), ([20] * 9, 700, 1100), ([20] * 8, 896, 1040), ([0, 0, 0], 130, 2048), ([64], 100, 4100),
-                                       ([1100, 0, 2200], 300, 1300), ([700, 3, 0, 129, 256, 128, 40], 600, 1300), ([0, 127, 64, 65, 0, 1], 1030, 1500)])
+                                       ([1100, 0, 2200], 300, 1300), ([700, 3, 0, 129, 256, 128, 40], 600, 1300), ([0, 127, 64, 65, 0, 1], 1030, 1500),
+                                       ([20] * 9, 384, 1500), ([20] * 9, 700, 1500), ([700, 3, 0, 129, 256, 128, 40], 1030, 1300), ([0, 127, 64, 65, 0, 1], 2100, 1500),
+                                       ([700, 3, 0, 129, 256, 128, 40], 2100, 272), ([1500, 1300], 1030, 272)])
 def test_grouped_product_on_tiles_of_every_kind(sizes, N, K):
     """few tiles, with K in eight, four and two parts; groups of many rows; tiles of one block and of pairs, more of them than one wave"""
     G, cap = len(sizes), sum(sizes) + 37
