@@ -51,11 +51,10 @@ int dim(int64_t n, const char* name) {
 // past the dispatcher: half the time of at::empty
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device dev) { return at::detail::empty_cuda(shape, type, dev, std::nullopt); }
 
-// a vector of four-byte elements inside an allocation, from its `first`-th on
-at::Tensor part_of(const at::Tensor& whole, int64_t first, int64_t n, at::ScalarType type) {
+// a tensor inside an allocation, from its `first`-th element on (past the dispatcher too)
+at::Tensor part_of(const at::Tensor& whole, int64_t first, at::IntArrayRef shape, at::IntArrayRef strides, at::ScalarType type) {
     at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
-    t.unsafeGetTensorImpl()->set_storage_offset(first);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides, first);
     return t;
 }
 
@@ -113,8 +112,8 @@ py::tuple router_topk(const at::Tensor& logits, int64_t topk, bool normalize, co
     at::Tensor idx = empty({l.T, width}, I32, l.dev), weights = empty({l.T, width}, F32, l.dev), lse = empty({l.T}, F32, l.dev), ws;
     // the few words for the experts come from one allocation: an allocation is 0.6 us of the host's
     const at::Tensor words = empty({2 * static_cast<int64_t>(l.E) + 2}, I32, l.dev);
-    at::Tensor counts = part_of(words, 0, l.E, I32), prob_sum = part_of(words, l.E, l.E, F32), num_valid = part_of(words, 2 * l.E, 1, I32),
-               loss = part_of(words, 2 * l.E + 1, 1, F32);
+    at::Tensor counts = part_of(words, 0, {l.E}, {1}, I32), prob_sum = part_of(words, l.E, {l.E}, {1}, F32), num_valid = part_of(words, 2 * l.E, {1}, {1}, I32),
+               loss = part_of(words, 2 * l.E + 1, {1}, {1}, F32);
     const size_t need = mx8_router_topk_workspace_bytes(l.T, l.E);
     if (need) ws = empty({static_cast<int64_t>(need)}, U8, l.dev);
     check(mx8_router_topk(logits.data_ptr(), l.type, l.ld, l.T, l.E, k, normalize, mask, idx.data_ptr(), weights.data_ptr(), lse.data_ptr(),
@@ -158,7 +157,8 @@ at::Tensor bwd_topk_weights(const at::Tensor& d_output, const at::Tensor& combin
 at::Tensor bytes_out(at::Device dev, bool batched, int64_t E, int64_t rows, int64_t cols) {
     const int64_t pitch = pad16(cols);
     at::Tensor t = batched ? empty({E, rows, pitch}, FP8, dev) : empty({rows, pitch}, FP8, dev);
-    return pitch == cols ? t : t.narrow(-1, 0, cols);
+    if (pitch == cols) return t;
+    return batched ? part_of(t, 0, {E, rows, cols}, {rows * pitch, pitch, 1}, FP8) : part_of(t, 0, {rows, cols}, {pitch, 1}, FP8);
 }
 
 py::tuple quantize_block128(const at::Tensor& x, bool normal, bool transposed, bool square, const OptTensor& row_index) {
