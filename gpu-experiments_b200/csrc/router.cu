@@ -148,28 +148,28 @@ __device__ __forceinline__ void sort_words(uint32_t (&w)[N]) {
     }
 }
 
-// k rounds on the full keys: the largest, the lowest lane that has it, the lowest of its experts that has it; lane j gets choice j
-template <typename T, int VPL>
-__device__ __noinline__ int select_slowly(const T* row, int experts, int topk, int lane) {
+// k rounds on the full keys: the largest, the lowest lane that has it, the lowest of its experts that has it; lane j gets choice j.  From the
+// registers: with 512 experts two tokens in a hundred come here, and reading the row again every round took 10 us for one.
+template <int VPL>
+__device__ __forceinline__ int select_slowly(const Row<float, VPL>& in, int topk, int lane) {
     int my_idx = -1;
-    uint32_t taken = 0;                                    // of this lane's experts
+    uint32_t key[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = key_of(in.get(i));
 #pragma unroll 1
     for (int j = 0; j < topk; ++j) {
-        uint32_t best = 0;
+        uint32_t best = key[0];
         int at = 0;
-#pragma unroll 1
-        for (int i = 0; i < VPL; ++i) {
-            const int e = lane * VPL + i;
-            const uint32_t k = e < experts && !((taken >> i) & 1u) ? key_of(to_float(row[e])) : 0u;
-            if (k > best) {
-                best = k;
-                at = i;
-            }
+#pragma unroll
+        for (int i = 1; i < VPL; ++i) {
+            at = key[i] > best ? i : at;
+            best = max(best, key[i]);
         }
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best);
         if (top < LIVE) break;
         const int owner = __ffs(__ballot_sync(0xFFFFFFFFu, best == top)) - 1;
-        if (lane == owner) taken |= 1u << at;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) key[i] = lane == owner && i == at ? 0u : key[i];
         at = __shfl_sync(0xFFFFFFFFu, at, owner);
         if (lane == j) my_idx = owner * VPL + at;
     }
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
             above = __reduce_add_sync(0xFFFFFFFFu, above);
             const int chosen_above = __popc(__ballot_sync(0xFFFFFFFFu, my_idx >= 0 && full > low));
             if (__any_sync(0xFFFFFFFFu, wrong) || above != chosen_above) {
-                my_idx = select_slowly<T, VPL>(row, p.experts, p.topk, lane);
+                my_idx = select_slowly<VPL>(in, p.topk, lane);
                 my_val = my_idx >= 0 ? to_float(row[my_idx]) : 0.0f;
             }
         }

@@ -81,6 +81,20 @@ def test_ties_go_to_the_lower_expert(dtype):
     check_forward(flat, 8, True)
 
 
+@pytest.mark.parametrize("shape", [(70, 512, 8), (33, 1000, 5), (40, 64, 6), (10, 8, 8), (5, 130, 32), (200, 33, 1)])
+def test_close_float32_values_are_told_apart(shape):
+    """logits of a few last bits' difference, many equal, some experts off: the order is that of the full values, ties to the lower expert"""
+    T, E, k = shape
+    g = torch.Generator().manual_seed(T)
+    l = 1.0 + torch.randint(0, 40, (T, E), generator=g).float() * 2.0 ** -23
+    l = torch.where(torch.rand(T, E, generator=g) < 0.1, -l, l)
+    l = torch.where(torch.rand(T, E, generator=g) < 0.2, float("-inf"), l)
+    idx = mx8.router_topk(l.to(DEV), k)[0].cpu()
+    order = torch.sort(l, dim=1, descending=True, stable=True)
+    want = torch.where(order.values[:, :k] == float("-inf"), -1, order.indices[:, :k]).to(torch.int32)
+    assert torch.equal(idx, want)
+
+
 def test_masks_switched_off_experts_and_lowest_values():
     l = make_logits(200, 64, torch.float32, 2)
     l[5] = NEG                                                 # nothing left
