@@ -323,8 +323,6 @@ __device__ __forceinline__ void write_rows(const Params& p, const float (&acc)[6
     __syncwarp();
 }
 
-// One column of C: a lane's values are its rows.  (A branch on the type and an address of its own for every value made the code so long
-// that fetching it took 3 us of a single tile's 7.)
 __device__ __forceinline__ void put(float* to, float v) { *to = v; }
 __device__ __forceinline__ void put(uint16_t* to, float v) { *to = static_cast<uint16_t>(pack_bf16x2(v, 0.0f)); }
 // up to `left` of four values of a row, together where they can be
@@ -349,6 +347,8 @@ __device__ __forceinline__ void put4(uint16_t* to, const float4& v, int left) {
         if (left > 3) to[3] = static_cast<uint16_t>(b >> 16);
     }
 }
+// One column of C: a lane's values are its rows.  (A branch on the type and an address of its own for every value made the code so long
+// that fetching it took 3 us of a single tile's 7.)
 template <class T>
 __device__ __forceinline__ void write_columns(T* to, long long pitch, const float (&acc)[64], int rows) {
 #pragma unroll
@@ -359,7 +359,7 @@ __device__ __forceinline__ void write_columns(T* to, long long pitch, const floa
     }
 }
 
-// The same from a fragment: acc[8 columns of 64][row of a lane: l / 4 + 8 i]
+// 32 rows x 64 columns from a fragment: acc[8 columns of 64][row of a lane: l / 4 + 8 i]
 template <bool F32>
 __device__ __forceinline__ void write_rows_frag(const Params& p, const uint64_t (&acc)[8][4], uint32_t turn, long long row0, int rows, int col0, int cols, int lane) {
     constexpr int ES = F32 ? 4 : 2;

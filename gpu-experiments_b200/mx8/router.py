@@ -17,7 +17,7 @@ def router_topk(logits, topk, *, normalize=True, token_mask=None):
     cannot be filled, and all of a token that takes no part, have id -1 (no rank owns it, `schedule` skips it) and weight 0.
     lse [T] float32 is saved for the backward; counts int32 [E]; prob_sum float32 [E]; num_valid int32 [1];
     balance_loss float32 [1] = E / (topk num_valid^2) sum_e counts[e] prob_sum[e]: 1 for an even spread.
-    At most 1024 experts and 32 choices."""
+    At most 1024 experts and 32 choices.  The words for the experts, and in small calls all outputs, share an allocation."""
     return host().router_topk(logits, topk, normalize, token_mask)
 
 
