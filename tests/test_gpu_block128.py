@@ -427,6 +427,30 @@ def test_weight_gradient_on_large_tiles(sizes):
     test_weight_gradient_product(sizes, (600, 1701))
 
 
+@pytest.mark.parametrize("sizes,mn", [([4096, 128], (64, 100)), ([0, 2944, 128], (130, 257)), ([1408] * 12, (100, 500)), ([128, 0, 8064], (200, 129))])
+def test_weight_gradient_in_parts(sizes, mn):
+    """few tiles, groups with fewer blocks than there are parts of K"""
+    test_weight_gradient_product(sizes, mn)
+
+
+def test_small_and_large_tiles_on_two_streams():
+    a = operands(3000, 2100, 700, "square", seed=50)
+    b = operands(64, 512, 4096, "square", seed=51)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for rep in range(4):
+        for st, ops in zip(streams, (a, b)):
+            with torch.cuda.stream(st):
+                outs.append(mx8.gemm_block128(*ops[:4], torch.empty(ops[0].shape[0], ops[2].shape[0], device=DEV)))
+    torch.cuda.synchronize()
+    assert mx8.device_status() == 0
+    for i, c in enumerate(outs):
+        if i < 2:
+            check_c(c, *(a, b)[i][4:])
+        else:
+            assert torch.equal(c, outs[i % 2])
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_offsets_beyond_32_bits(m):
     """C that spans more than 2^32 elements is written where it should be and nowhere between"""
