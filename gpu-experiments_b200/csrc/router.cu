@@ -359,6 +359,8 @@ __global__ void __cluster_dims__(FINISH, 1, 1) __launch_bounds__(1024) router_fi
     __shared__ double dots[FINISH];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x;
     double dot = 0;
+    // rank 0's shared memory may be written once its block is known to run: every block arrives here, and waits before it stores
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // launched while the forward kernel still runs: from here on its results are there
     asm volatile("griddepcontrol.wait;" ::: "memory");
     int n = 0;                                              // the tokens that took part
@@ -392,6 +394,7 @@ __global__ void __cluster_dims__(FINISH, 1, 1) __launch_bounds__(1024) router_fi
     }
     if (lane == 0) sum_p[1][warp] = dot;                    // its experts' share
     __syncthreads();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp == 0) {
         dot = sum_p[1][lane];
 #pragma unroll

@@ -322,3 +322,16 @@ def test_offsets_beyond_32_bits():
     want = torch.zeros(T, k)
     want[-1, -1], want[-1, 0] = 3.0, 5.0
     assert torch.equal(mx8.bwd_topk_weights(d, c).cpu(), want)
+
+
+@pytest.mark.parametrize("E", [1, 33, 256, 257, 1000])
+def test_balance_loss_of_many_launches_in_a_row(E):
+    """the finishing kernel's blocks start at any time beside the forward kernels of a full stream: the loss is that of the returned sums"""
+    k = min(E, 5)
+    l = make_logits(700, E, torch.float32, E)
+    outs = [mx8.router_topk(l + float(i), k) for i in range(200)]
+    torch.cuda.synchronize()
+    for _, _, _, counts, prob, n, loss in outs:
+        want = float((counts.double() * prob.double()).sum()) * E / (k * 700.0 ** 2)
+        # prob_sum and the loss are rounded to fp32, half a step each
+        assert int(n) == 700 and int(counts.sum()) == 700 * k and abs(float(loss) - want) <= 2.0 ** -23 * want
