@@ -10,7 +10,8 @@
 // blackwell-ultra/022-moe-dispatch-mlp-swiglu-combine-mxfp8-bw.cu:830-922.
 //
 // epilogue: out[t] = bf16( y_shared[t] + sum_j w[t][j] * combine[t*topk + j] ), fp32, products and
-// sums rounded separately, j ascending, so the result does not depend on the launch shape.
+// sums rounded separately, j ascending, so the result does not depend on the launch shape.  A choice that the
+// router could not fill has weight 0 and a row that no rank wrote: with weight 0 an infinity or NaN counts as 0.
 // Replaces fwd_epilogue_kernel, blackwell-ultra/022-…-mxfp8-bw.cu:2789-2856.
 #include <atomic>
 
@@ -155,7 +156,10 @@ __global__ void __launch_bounds__(256) epilogue_kernel(EpilogueParams p) {
             float v[8];
             unpack8(reinterpret_cast<const uint4*>(p.combine)[(static_cast<size_t>(t) * p.topk + j) * n16 + c], v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = __fadd_rn(acc[i], __fmul_rn(v[i], w));   // no fused multiply-add
+            for (int i = 0; i < 8; ++i) {
+                const float t = __fmul_rn(v[i], w);                                       // no fused multiply-add
+                acc[i] = __fadd_rn(acc[i], w == 0.0f && t != t ? 0.0f : t);
+            }
         }
         uint4 o;
         o.x = pack_bf16x2(acc[0], acc[1]);

@@ -80,7 +80,9 @@ def combine(y_routed, schedule_peer_rank, schedule_peer_token_idx, num_tokens, c
 
 def fwd_epilogue(y_shared, combine_buffer, topk_weights):
     """fwd_epilogue(y_shared, combine_buffer, topk_weights) -> output
-    (blackwell-ultra/022-…-mxfp8-bw.cu:2842-2856, bound at :3029-3030).  y_shared may be None."""
+    (blackwell-ultra/022-…-mxfp8-bw.cu:2842-2856, bound at :3029-3030).  y_shared may be None.  A choice of weight 0
+    contributes nothing, whatever its row holds: `combine` does not write the rows of choices without an expert (id -1
+    of `router_topk`), which need not be cleared."""
     lib = _lib.load()
     T, k = topk_weights.shape
     H = combine_buffer.shape[1]

@@ -14,7 +14,8 @@ def router_topk(logits, topk, *, normalize=True, token_mask=None):
     logits [T, E], bf16 or float32.  p = softmax(logits) in float32; topk_idx int32 [T, topk] are the largest logits of a token, largest
     first, ties to the lower expert; topk_weights float32 [T, topk] is p there, divided by its sum over the choices when `normalize`.
     token_mask (bool [T]): False for a token that takes no part.  A logit of -inf switches an expert off for its token.  Choices that
-    cannot be filled, and all of a token that takes no part, have id -1 (no rank owns it, `schedule` skips it) and weight 0.
+    cannot be filled, and all of a token that takes no part, have id -1 (no rank owns it, `schedule` skips it, `combine` leaves its row as it
+    was) and weight 0 (`fwd_epilogue` adds nothing for it).
     lse [T] float32 is saved for the backward; counts int32 [E]; prob_sum float32 [E]; num_valid int32 [1];
     balance_loss float32 [1] = E / (topk num_valid^2) sum_e counts[e] prob_sum[e]: 1 for an even spread.
     At most 1024 experts and 32 choices.  The words for the experts, and in small calls all outputs, share an allocation."""

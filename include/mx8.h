@@ -139,7 +139,9 @@ MX8_API int mx8_moe_combine(const void* y_routed, const void* peer_rank, const v
                             int capacity, int hidden, void* const* combine_ptrs, int world, long long combine_rows, void* stream);
 
 /* out[t] = bf16( y_shared[t] + sum_j topk_weights[t][j] * combine_buffer[t*topk + j] ); y_shared may be
- * NULL (no shared expert).  topk_weights float32 [tokens][topk]; the other tensors bf16.
+ * NULL (no shared expert).  topk_weights float32 [tokens][topk]; the other tensors bf16.  A choice of weight 0
+ * contributes nothing, whatever its row holds: mx8_moe_combine does not write the rows of choices without an expert
+ * (id -1), which therefore need not be cleared.
  * Replaces fwd_epilogue, blackwell-ultra/022-…-mxfp8-bw.cu:2789-2856. */
 MX8_API int mx8_moe_fwd_epilogue(const void* y_shared, const void* combine_buffer, const void* topk_weights, void* out,
                                  int tokens, int hidden, int topk, void* stream);

@@ -335,3 +335,33 @@ def test_balance_loss_of_many_launches_in_a_row(E):
         want = float((counts.double() * prob.double()).sum()) * E / (k * 700.0 ** 2)
         # prob_sum and the loss are rounded to fp32, half a step each
         assert int(n) == 700 and int(counts.sum()) == 700 * k and abs(float(loss) - want) <= 2.0 ** -23 * want
+
+
+@pytest.mark.parametrize("H,k", [(8, 1), (264, 3), (1024, 8)])
+def test_rows_of_choices_without_an_expert_do_not_reach_the_output(H, k):
+    """combine leaves the rows of ids -1 as they were: NaN, infinities or an earlier step's values there change nothing, a NaN of a
+    live choice stays one"""
+    T, E = 40, 16
+    l = make_logits(T, E, torch.float32, H)
+    l[3, 1:] = NEG                                                 # one live expert
+    mask = torch.arange(T, device=DEV) < 35
+    idx, w, _, _, _, _, _ = mx8.router_topk(l, k, token_mask=mask)
+    g = torch.Generator().manual_seed(k)
+    buf = torch.randn(T * k, H, generator=g).to(torch.bfloat16).to(DEV)
+    y = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    dead = (idx < 0).reshape(-1)
+    assert int(dead.sum()) == 5 * k + k - 1
+    clean = buf.masked_fill(dead[:, None], 0.0)
+    for shared in (y, None):
+        want = mx8.fwd_epilogue(shared, clean, w)
+        for bad in (float("nan"), float("inf"), float("-inf"), 3e38):
+            assert torch.equal(mx8.fwd_epilogue(shared, buf.masked_fill(dead[:, None], bad), w), want)
+    assert torch.equal(want[35:], torch.zeros_like(want[35:]))
+    live = clean.clone()
+    live[0, 0] = float("nan")
+    out = mx8.fwd_epilogue(None, live, w)
+    assert torch.isnan(out[0, 0]) and int(torch.isnan(out).sum()) == 1
+    # a finite row times 0 keeps the zero's sign, as before
+    one = torch.full((1, 8), -1.0, dtype=torch.bfloat16, device=DEV)
+    zero = torch.full((1, 8), -0.0, dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(mx8.fwd_epilogue(zero, one, torch.zeros(1, 1, device=DEV)).view(torch.int16), zero.view(torch.int16))
