@@ -269,12 +269,18 @@ at::Tensor bwd_prologue(const at::Tensor& d_output, const at::Tensor& topk_weigh
     return d_output;   // == d_y_shared; the combine buffer is filled in place
 }
 
-at::Tensor bwd_epilogue(const at::Tensor& d_x_shared, const at::Tensor& d_x_routed_buffer) {
+at::Tensor bwd_epilogue(const at::Tensor& d_x_shared, const at::Tensor& d_x_routed_buffer, const std::optional<at::Tensor>& topk_idx) {
     c10::cuda::CUDAGuard guard(d_x_shared.device());
     const int64_t T = d_x_shared.size(0), H = d_x_shared.size(1), k = d_x_routed_buffer.size(0) / T;
+    const void* ids = nullptr;
+    if (topk_idx.has_value() && topk_idx->defined()) {
+        TORCH_CHECK(topk_idx->device() == d_x_shared.device() && topk_idx->scalar_type() == at::kInt && topk_idx->is_contiguous() && topk_idx->numel() == T * k,
+                    "topk_idx int32 [tokens, topk]");
+        ids = topk_idx->data_ptr();
+    }
     at::Tensor d_x = at::empty_like(d_x_shared);
-    check(mx8_moe_bwd_epilogue(dptr(d_x_shared, "d_x_shared", T * H), dptr(d_x_routed_buffer, "d_x_routed_buffer", T * k * H),
-                               d_x.data_ptr(), static_cast<int>(T), static_cast<int>(H), static_cast<int>(k), stream()),
+    check(mx8_moe_bwd_epilogue_ids(dptr(d_x_shared, "d_x_shared", T * H), dptr(d_x_routed_buffer, "d_x_routed_buffer", T * k * H), ids,
+                                   d_x.data_ptr(), static_cast<int>(T), static_cast<int>(H), static_cast<int>(k), stream()),
           "bwd_epilogue");
     return d_x;
 }
@@ -404,7 +410,7 @@ PYBIND11_MODULE(_C, m) {
           pybind11::arg("macrobatch_size") = 0, pybind11::arg("minibatch_size") = 0);
     m.def("fwd_epilogue", &fwd_epilogue, "", pybind11::arg("y_shared"), pybind11::arg("combine_buffer"), pybind11::arg("topk_weights"));
     m.def("bwd_prologue", &bwd_prologue);
-    m.def("bwd_epilogue", &bwd_epilogue);
+    m.def("bwd_epilogue", &bwd_epilogue, "", pybind11::arg("d_x_shared"), pybind11::arg("d_x_routed_buffer"), pybind11::arg("topk_idx") = std::nullopt);
     m.def("dispatch_mlp_swiglu_combine_bwd", &dispatch_mlp_swiglu_combine_bwd);
     bind_block128_router(m);
     m.def("device_status", &device_status);

@@ -244,25 +244,29 @@ def bwd_prologue(d_output, topk_weights, d_combine_buffer):
     return d_output
 
 
-def bwd_epilogue(d_x_shared, d_x_routed_buffer):
+def bwd_epilogue(d_x_shared, d_x_routed_buffer, topk_idx=None):
     """bwd_epilogue(d_x_shared, d_x_routed_buffer) -> d_x = d_x_shared + sum over the topk rows of every
     token (blackwell-ultra/022-…-mxfp8-bw.cu:2982-2993).  d_x_shared may be None; then its shape is taken
-    from `d_x_routed_buffer` and the `tokens` it was built for must divide its rows (pass topk via shape)."""
+    from `d_x_routed_buffer` and the `tokens` it was built for must divide its rows (pass topk via shape).
+    topk_idx (an addition; int32 [T, topk] of `router_topk`): rows of choices with a negative id, which `combine` does not
+    write, add nothing, whatever they hold.  Without it such rows have to be cleared before every backward."""
     raise_if = d_x_shared is None
     if raise_if:
         raise ValueError("bwd_epilogue needs d_x_shared (use bwd_epilogue_routed for the routed part alone)")
-    return bwd_epilogue_routed(d_x_shared, d_x_routed_buffer, d_x_routed_buffer.shape[0] // d_x_shared.shape[0])
+    return bwd_epilogue_routed(d_x_shared, d_x_routed_buffer, d_x_routed_buffer.shape[0] // d_x_shared.shape[0], topk_idx)
 
 
-def bwd_epilogue_routed(d_x_shared, d_x_routed_buffer, topk):
+def bwd_epilogue_routed(d_x_shared, d_x_routed_buffer, topk, topk_idx=None):
+    """`bwd_epilogue` with the number of choices given, so that d_x_shared may be None."""
     lib = _lib.load()
     H = d_x_routed_buffer.shape[1]
     T = d_x_routed_buffer.shape[0] // topk
     d_x = torch.empty(T, H, dtype=torch.bfloat16, device=d_x_routed_buffer.device)
     with torch.cuda.device(d_x.device):
-        _lib.check(lib.mx8_moe_bwd_epilogue(
+        _lib.check(lib.mx8_moe_bwd_epilogue_ids(
             _chk(d_x_shared, "d_x_shared", (torch.bfloat16,), (T, H)) if d_x_shared is not None else None,
-            _chk(d_x_routed_buffer, "d_x_routed_buffer", (torch.bfloat16,), (T * topk, H)), d_x.data_ptr(), T, H, topk,
+            _chk(d_x_routed_buffer, "d_x_routed_buffer", (torch.bfloat16,), (T * topk, H)),
+            _chk(topk_idx, "topk_idx", (torch.int32,), (T, topk)) if topk_idx is not None else None, d_x.data_ptr(), T, H, topk,
             _stream()), "bwd_epilogue")
     return d_x
 

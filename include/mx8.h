@@ -200,6 +200,11 @@ MX8_API int mx8_moe_bwd_prologue(const void* d_output, const void* topk_weights,
 MX8_API int mx8_moe_bwd_epilogue(const void* d_x_shared, const void* d_x_routed_buffer, void* d_x, int tokens, int hidden,
                                  int topk, void* stream);
 
+/* The same for a routing with ids: rows of choices whose id in topk_idx (int32 [tokens][topk], may be NULL) is negative, which
+ * mx8_moe_combine does not write, add nothing, whatever they hold.  Without ids such rows have to be cleared before every backward. */
+MX8_API int mx8_moe_bwd_epilogue_ids(const void* d_x_shared, const void* d_x_routed_buffer, const void* topk_idx, void* d_x, int tokens,
+                                     int hidden, int topk, void* stream);
+
 /* Expert-parallel MoE routing schedule for the calling rank (int32 everywhere).
  *   topk_all [world][tokens][topk]: global expert ids chosen by every rank's tokens;
  *   this rank owns experts [rank*num_local_experts, (rank+1)*num_local_experts).

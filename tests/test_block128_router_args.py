@@ -100,3 +100,10 @@ def test_no_device_means_error_not_fallback(lib):
         mx8.gemm_block128(torch.zeros(4, 16, dtype=torch.float8_e4m3fn), *[torch.zeros(1)] * 4)
     with pytest.raises(ValueError):
         mx8.bwd_topk_weights(torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 8, dtype=torch.bfloat16))
+
+
+def test_bwd_epilogue_with_ids_arguments(lib):
+    f = lib.mx8_moe_bwd_epilogue_ids
+    assert f(None, None, P, P, 1, 8, 1, None) == _lib.ERR_ARG and f(None, P, P, None, 1, 8, 1, None) == _lib.ERR_ARG
+    assert f(None, P, P, P, 0, 8, 1, None) == _lib.ERR_ARG and f(None, P, P, P, 1, 12, 1, None) == _lib.ERR_SHAPE
+    assert f(None, P, ODD, P, 1, 8, 1, None) == _lib.ERR_ALIGN and f(ODD, P, None, P, 1, 8, 1, None) == _lib.ERR_ALIGN

@@ -365,3 +365,31 @@ def test_rows_of_choices_without_an_expert_do_not_reach_the_output(H, k):
     one = torch.full((1, 8), -1.0, dtype=torch.bfloat16, device=DEV)
     zero = torch.full((1, 8), -0.0, dtype=torch.bfloat16, device=DEV)
     assert torch.equal(mx8.fwd_epilogue(zero, one, torch.zeros(1, 1, device=DEV)).view(torch.int16), zero.view(torch.int16))
+
+
+def test_gradients_of_choices_without_an_expert_are_not_summed():
+    """the backward's combine leaves the rows of ids -1 as they were; the sum over a token's rows skips them when it has the ids"""
+    T, E, H, k = 40, 16, 264, 3
+    l = make_logits(T, E, torch.float32, 1)
+    l[3, 1:] = NEG
+    idx = mx8.router_topk(l, k, token_mask=torch.arange(T, device=DEV) < 35)[0]
+    g = torch.Generator().manual_seed(k)
+    shared = torch.randn(T, H, generator=g).to(torch.bfloat16).to(DEV)
+    buf = torch.randn(T * k, H, generator=g).to(torch.bfloat16).to(DEV)        # an earlier step's values in the dead rows
+    dead = (idx < 0).reshape(-1, 1)
+    clean = buf.masked_fill(dead, 0.0)
+    want = mx8.bwd_epilogue(shared, clean)
+    terms = torch.cat([shared[:, None], clean.view(T, k, H)], 1).double()
+    # k + 1 terms added in fp32, then half a step of bf16
+    assert ((want.double() - terms.sum(1)).abs() <= 2.0 ** -8 * terms.sum(1).abs() + 2.0 ** -22 * terms.abs().sum(1)).all()
+    assert not torch.equal(mx8.bwd_epilogue(shared, buf), want)
+    from mx8 import _C
+    for held in (buf, buf.masked_fill(dead, float("nan"))):
+        assert torch.equal(mx8.bwd_epilogue(shared, held, idx), want)
+        assert torch.equal(_C.bwd_epilogue(shared, held, idx), want)
+        assert torch.equal(mx8.bwd_epilogue_routed(None, held, k, idx), mx8.bwd_epilogue_routed(None, clean, k))
+    for bad in (idx.long(), idx[:5].contiguous(), idx.cpu()):
+        with pytest.raises(ValueError):
+            mx8.bwd_epilogue(shared, buf, bad)
+        with pytest.raises(RuntimeError):
+            _C.bwd_epilogue(shared, buf, bad)
