@@ -627,9 +627,11 @@ template <typename T, int VPL>
 static cudaError_t launch_fwd(const FwdParams& p, int grid, cudaStream_t st) {
     constexpr int WARPS = Shape<VPL>::WARPS;
     const size_t smem = sizeof(float) * (WARPS + 1) * static_cast<size_t>(p.experts);
+    constexpr int MOST = static_cast<int>(sizeof(float)) * (WARPS + 1) * 32 * VPL;
     auto kern = router_fwd_kernel<T, VPL>;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if constexpr (MOST > 40 * 1024) {
+        // what the kernel can need at most, not this call's own: another thread may be between its attribute and its launch
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
         if (e != cudaSuccess) return e;
     }
     kern<<<grid, WARPS * 32, smem, st>>>(p);

@@ -393,3 +393,38 @@ def test_gradients_of_choices_without_an_expert_are_not_summed():
             mx8.bwd_epilogue(shared, buf, bad)
         with pytest.raises(RuntimeError):
             _C.bwd_epilogue(shared, buf, bad)
+
+
+def test_calls_of_different_widths_in_threads():
+    """host threads through the C ABI, which holds no lock of Python's: all of 513 to 1024 experts share a kernel and its limits"""
+    import threading
+    lib, failed = mx8.load(), []
+    widths = (1024, 520, 1000, 700)
+    held = {E: (make_logits(4, E, torch.float32, E), make_logits(4, E, torch.bfloat16, E)) for E in widths}
+    barrier = threading.Barrier(len(widths))
+    got = {}
+
+    def worker(E):
+        s = torch.cuda.Stream()
+        out = [torch.empty(4, 8, dtype=torch.int32, device=DEV), torch.empty(4, 8, device=DEV), torch.empty(4, device=DEV),
+               torch.empty(E, dtype=torch.int32, device=DEV), torch.empty(E, device=DEV), torch.empty(1, dtype=torch.int32, device=DEV), torch.empty(1, device=DEV)]
+        ptrs = [t.data_ptr() for t in out]
+        barrier.wait()
+        for i in range(20000):
+            rc = lib.mx8_router_topk(held[E][i & 1].data_ptr(), 1 - (i & 1), E, 4, E, 8, 1, None, *ptrs, None, 0, s.cuda_stream)
+            if rc:
+                failed.append((E, i, rc, lib.mx8_last_cuda_error()))
+                break
+        s.synchronize()
+        got[E] = out
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=worker, args=(E,)) for E in widths]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for E in widths:
+        for a, b in zip(got[E], mx8.router_topk(held[E][1], 8)):
+            assert torch.equal(a, b)
