@@ -109,21 +109,29 @@ py::tuple router_topk(const at::Tensor& logits, int64_t topk, bool normalize, co
     const void* mask = vec(token_mask, "token_mask", at::kBool, {l.T}, l.dev);
     const int k = topk < INT_MIN ? INT_MIN : topk > INT_MAX ? INT_MAX : static_cast<int>(topk);
     const int64_t width = k < 1 || k > l.E || k > 32 ? 1 : k;                  // refused below
-    // the few words for the experts, and in small calls all outputs, come from one allocation (an allocation is 0.6 us of the host's), each
-    // starting where an allocation of its own could
+    // the few words for the experts, and in small calls all outputs, come from one allocation of each type (an allocation is 0.6 us of the
+    // host's), each starting where an allocation of its own could.  Not from one for both types: torch.save refuses tensors of different
+    // types on one storage.
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
-    const int64_t pairs = l.T * width, own = 2 * up(l.E) + 256, rest = 2 * up(pairs) + up(l.T);
-    const bool small = rest <= 16384;
-    const at::Tensor words = empty({small ? own + rest : own}, I32, l.dev);
-    int64_t next = 0;
-    const auto take = [&](int64_t rows, int64_t cols, bool matrix, at::ScalarType type) {
-        const int64_t at = next;
-        next += up(rows * cols);
-        return matrix ? part_of(words, at, {rows, cols}, {cols, 1}, type) : part_of(words, at, {rows}, {1}, type);
+    const int64_t pairs = l.T * width;
+    const bool small = 2 * up(pairs) + up(l.T) <= 16384;
+    struct Words {
+        at::Tensor all;
+        at::ScalarType type;
+        int64_t next = 0;
     };
-    at::Tensor counts = take(l.E, 1, false, I32), prob_sum = take(l.E, 1, false, F32), num_valid = take(1, 1, false, I32), loss = take(1, 1, false, F32);
-    at::Tensor idx = small ? take(l.T, width, true, I32) : empty({l.T, width}, I32, l.dev), weights = small ? take(l.T, width, true, F32) : empty({l.T, width}, F32, l.dev),
-               lse = small ? take(l.T, 1, false, F32) : empty({l.T}, F32, l.dev), ws;
+    Words ints{empty({up(l.E) + 128 + (small ? up(pairs) : 0)}, I32, l.dev), I32}, floats{empty({up(l.E) + 128 + (small ? up(pairs) + up(l.T) : 0)}, F32, l.dev), F32};
+    const auto vector = [&](Words& w, int64_t n) {
+        w.next += up(n);
+        return part_of(w.all, w.next - up(n), {n}, {1}, w.type);
+    };
+    const auto matrix = [&](Words& w) {                                        // [T, width]
+        w.next += up(pairs);
+        return part_of(w.all, w.next - up(pairs), {l.T, width}, {width, 1}, w.type);
+    };
+    at::Tensor counts = vector(ints, l.E), prob_sum = vector(floats, l.E), num_valid = vector(ints, 1), loss = vector(floats, 1);
+    at::Tensor idx = small ? matrix(ints) : empty({l.T, width}, I32, l.dev), weights = small ? matrix(floats) : empty({l.T, width}, F32, l.dev),
+               lse = small ? vector(floats, l.T) : empty({l.T}, F32, l.dev), ws;
     const size_t need = mx8_router_topk_workspace_bytes(l.T, l.E);
     if (need) ws = empty({static_cast<int64_t>(need)}, U8, l.dev);
     check(mx8_router_topk(logits.data_ptr(), l.type, l.ld, l.T, l.E, k, normalize, mask, idx.data_ptr(), weights.data_ptr(), lse.data_ptr(),

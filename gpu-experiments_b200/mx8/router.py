@@ -18,7 +18,8 @@ def router_topk(logits, topk, *, normalize=True, token_mask=None):
     was) and weight 0 (`fwd_epilogue` adds nothing for it).
     lse [T] float32 is saved for the backward; counts int32 [E]; prob_sum float32 [E]; num_valid int32 [1];
     balance_loss float32 [1] = E / (topk num_valid^2) sum_e counts[e] prob_sum[e]: 1 for an even spread.
-    At most 1024 experts and 32 choices.  The words for the experts, and in small calls all outputs, share an allocation."""
+    At most 1024 experts and 32 choices.  counts and num_valid, prob_sum and balance_loss, and in small calls all outputs of a type share
+    a storage (saving one of them saves its storage; `clone` it to keep it alone)."""
     return host().router_topk(logits, topk, normalize, token_mask)
 
 

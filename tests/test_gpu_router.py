@@ -428,3 +428,21 @@ def test_calls_of_different_widths_in_threads():
     for E in widths:
         for a, b in zip(got[E], mx8.router_topk(held[E][1], 8)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [3, 2000])
+def test_outputs_can_be_saved_together(T):
+    """in calls whose outputs share allocations and in those where they do not; what is saved is what was there"""
+    import io
+    import itertools
+    l = make_logits(T, 64, torch.float32, T)
+    out = mx8.router_topk(l, 4)
+    for group in list(itertools.combinations(out, 2)) + [out]:
+        f = io.BytesIO()
+        torch.save(list(group), f)
+        f.seek(0)
+        for a, b in zip(torch.load(f), group):
+            assert a.dtype == b.dtype and torch.equal(a, b)
+    # no two of them overlap, and each starts on a 512-byte boundary
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in out)
+    assert all(a % 512 == 0 for a, _ in spans) and all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
