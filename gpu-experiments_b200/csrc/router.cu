@@ -13,8 +13,8 @@
 // expert's number reversed in the other 10: all words differ, the larger word is the larger value or the lower expert, and one
 // redux.sync.max finds both.  bf16 values fit in the 22 bits; for fp32 the result is checked against the full values and rows in which
 // the cut bits decide (values within 2^-13 of each other) are selected again, slowly.
-// Sums over tokens are made in a fixed order (registers of a warp, then warps of a block, then blocks), never with floating-point
-// atomics: results do not change from run to run.
+// Sums over tokens are made in a fixed order (registers of a warp, then warps of a block, both in 32 bits, then blocks in 64), never with
+// floating-point atomics: results do not change from run to run.
 #include <atomic>
 
 #include "mx8_host.cuh"
@@ -224,6 +224,16 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
         next.load(row, lane, p.experts, p.vec != 0);
         if (p.mask) next_on = p.mask[t];
     }
+    // the logarithms of 32 tokens are taken together, a lane each: lane n % 32 holds those of the warp's n-th token
+    int n = 0;
+    float lse_max = 0.0f, lse_sum = 1.0f;
+    auto keep_lse = [&](float mx, float sum) {
+        if (lane == (n & 31)) {
+            lse_max = mx;
+            lse_sum = sum;
+        }
+        if ((++n & 31) == 0) p.lse[t - (31 - lane) * step] = lse_max + logf(lse_sum);
+    };
     for (; t < p.tokens; t += step, row += step * p.ld) {
         const Row<T, VPL> in = next;
         const bool on = next_on != 0;
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
                 p.idx[out] = -1;
                 p.weights[out] = 0.0f;
             }
-            if (lane == 0) p.lse[t] = -INFINITY;
+            keep_lse(-INFINITY, 1.0f);
             continue;
         }
         const float mx = sizeof(T) == 4 ? value_of(top) : __uint_as_float(__float_as_uint(value_of(top)) & 0xFFFF0000u);
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
             sum += v[i];
         }
         sum = warp_sum(sum);
-        const float inv = __fdividef(1.0f, sum);
+        const float inv = __frcp_rn(sum);                  // rounded once; a weight is off by this rounding and its own
 #pragma unroll
         for (int i = 0; i < VPL; ++i) prob[i] = fmaf(v[i], inv, prob[i]);
         ++n_valid;
@@ -310,14 +320,15 @@ __global__ void __launch_bounds__(Shape<VPL>::WARPS * 32) router_fwd_kernel(cons
             }
         }
         float w = my_idx >= 0 ? expf(my_val - mx) : 0.0f;
-        w *= p.normalize ? __fdividef(1.0f, warp_sum(w)) : inv;
+        w *= p.normalize ? __frcp_rn(warp_sum(w)) : inv;
         if (lane < p.topk) {
             p.idx[out] = my_idx;
             p.weights[out] = my_idx >= 0 ? w : 0.0f;
             if (my_idx >= 0) atomicAdd(&count[my_idx], 1);
         }
-        if (lane == 0) p.lse[t] = mx + __logf(sum);
+        keep_lse(mx, sum);
     }
+    if (lane < (n & 31)) p.lse[t - ((n & 31) - lane) * step] = lse_max + logf(lse_sum);
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
         if (lane * VPL + i < p.experts) warp_prob[warp * p.experts + lane * VPL + i] = prob[i];

@@ -446,3 +446,18 @@ def test_outputs_can_be_saved_together(T):
     # no two of them overlap, and each starts on a 512-byte boundary
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in out)
     assert all(a % 512 == 0 for a, _ in spans) and all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_equal_logits_give_correctly_rounded_values(dtype):
+    """exp(0) is 1 and E ones add up exactly, so that a weight is one division, rounded once, and lse the logarithm of an integer (logf: one
+    step of 2^-23 of its binade)"""
+    for E in [*range(1, 40), *range(41, 1024, 17), 1023, 1024]:
+        k = min(E, 1 + E % 32)
+        flat = torch.zeros(2, E, dtype=dtype, device=DEV)
+        for normalize, n in ((True, k), (False, E)):
+            out = mx8.router_topk(flat, k, normalize=normalize)
+            assert (out[1].cpu() == torch.full((2, k), 1.0 / n, dtype=torch.float64).float()).all(), (E, k, normalize)
+        want = torch.tensor(float(E), dtype=torch.float64).log()
+        step = 2.0 ** (float(want.log2().floor()) - 23) if E > 1 else 0.0
+        assert ((out[2].cpu().double() - want).abs() <= step).all(), E
