@@ -126,6 +126,21 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// three sums over the warp at once: lanes first divide the sums among themselves, nine exchanges instead of fifteen
+__device__ __forceinline__ void warp_sums(float& a, float& b, float& c, int lane) {
+    const bool h = lane & 16, q = lane & 8;
+    float x = h ? b : a, z = c;
+    x += __shfl_xor_sync(0xFFFFFFFFu, h ? a : b, 16);                      // lanes 0 - 15: a, 16 - 31: b
+    z += __shfl_xor_sync(0xFFFFFFFFu, z, 16);
+    float u = q ? z : x;
+    u += __shfl_xor_sync(0xFFFFFFFFu, q ? x : z, 8);                       // lanes 8 - 15 and 24 - 31: c
+#pragma unroll
+    for (int o = 4; o; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+    a = __shfl_sync(0xFFFFFFFFu, u, 0);
+    b = __shfl_sync(0xFFFFFFFFu, u, 16);
+    c = __shfl_sync(0xFFFFFFFFu, u, 8);
+}
+
 // descending, by a network of compare-exchanges (19 of them for 8 words)
 template <int N>
 __device__ __forceinline__ void sort_words(uint32_t (&w)[N]) {
@@ -497,23 +512,28 @@ __global__ void __launch_bounds__(BWD_WARPS * 32, bwd_blocks<VPL>()) router_bwd_
         T* out = static_cast<T*>(p.d_logits) + static_cast<size_t>(t) * p.experts;
         float v[VPL];
         const bool on = in.lse != -INFINITY;               // a token that took no part gets zeros, whatever its logits are
-        float dot = 0.0f;
+        // lse is rounded, which makes all of the token's exponentials too large or too small by up to |lse| 2^-24: what counts is their
+        // share of their own sum
+        float dot = 0.0f, sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             v[i] = on ? expf(in.v.get(i) - in.lse) : 0.0f;
             dot += v[i] * b[i];
+            sum += v[i];
         }
         const int idx = in.idx >= 0 && in.idx < p.experts ? in.idx : -1;
         const float w = idx >= 0 ? in.w : 0.0f, dw = idx >= 0 ? in.dw : 0.0f, wdw = w * dw;
-        dot = warp_sum(dot);
+        float s = wdw;
+        warp_sums(dot, sum, s, lane);
+        const float inv = __frcp_rn(sum);
+        dot *= inv;
         if (p.d_weights) {
-            const float s = warp_sum(wdw);
             if (!p.normalize) dot += s;
             if (idx >= 0) row[place(idx)] = p.normalize ? w * (dw - s) : wdw;      // a token's choices are distinct
             __syncwarp();
         }
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) v[i] = on ? v[i] * (b[i] - dot) + (p.d_weights ? row[i * 32 + lane] : 0.0f) : 0.0f;
+        for (int i = 0; i < VPL; ++i) v[i] = on ? v[i] * fmaf(b[i], inv, -dot * inv) + (p.d_weights ? row[i * 32 + lane] : 0.0f) : 0.0f;
         if (p.d_weights) {
             __syncwarp();
             if (idx >= 0) row[place(idx)] = 0.0f;

@@ -461,3 +461,21 @@ def test_equal_logits_give_correctly_rounded_values(dtype):
         want = torch.tensor(float(E), dtype=torch.float64).log()
         step = 2.0 ** (float(want.log2().floor()) - 23) if E > 1 else 0.0
         assert ((out[2].cpu().double() - want).abs() <= step).all(), E
+
+
+@pytest.mark.parametrize("shift", [0.0, 1000.0, -1000.0, 30000.0])
+@pytest.mark.parametrize("shape", [(300, 64, 4), (40, 1000, 8), (7, 5, 2), (100, 256, 8)])
+def test_backward_of_shifted_logits(shape, shift):
+    """the rounding of a large lse does not reach the gradient: it is that of 64 bits, and a token's gradients add up to nothing"""
+    T, E, k = shape
+    logits = make_logits(T, E, torch.float32, T) + shift                       # the rounded sums are the logits of both sides
+    g = torch.Generator().manual_seed(E)
+    dw, dl = torch.randn(T, k, generator=g).to(DEV), torch.tensor([3.0], device=DEV)
+    for normalize in (True, False):
+        idx, w, lse, counts, _, n, _ = mx8.router_topk(logits, k, normalize=normalize)
+        got = mx8.router_topk_bwd(logits, idx, w, lse, counts, n, dw, dl, normalize=normalize).cpu().double()
+        want, size = bwd_ref(logits, idx.cpu().long(), normalize, counts.cpu(), int(n), k, dw, dl)
+        assert ((got - want).abs() <= 4 * P_TOL * size + 2.0 ** -120).all()
+        # the sum that is subtracted is off by its E / 32 + 5 additions and two products, every gradient by three roundings, 1 / sum by one,
+        # all of 2^-24 and of terms that add up to at most twice `size`
+        assert (got.sum(1, keepdim=True).abs() <= (E / 32 + 16) * 2.0 ** -23 * size).all()
