@@ -1,7 +1,8 @@
 // Matrix product of the block-128 format for sm_100a:
 //   C[i][j] = sum_kb sa[kb][i] * sb(kb, j) * sum_{k in block kb} A[i][k] * B[j][k],   A, B E4M3, scales fp32, C bf16 or fp32.
 // The scales are no powers of two and belong to 128 values of k, so the tensor core sums one block at a time (four
-// tcgen05.mma.kind::f8f6f4 of K = 32 into TMEM, fp32) and registers add the blocks up: acc += scale * partial, one rounding each.
+// tcgen05.mma.kind::f8f6f4 of K = 32 into TMEM, fp32) and registers add the blocks up: acc += (sa * sb) * partial, the scales' product
+// rounded once and the fused addition once, in every form.
 //
 // A CTA, or a pair of CTAs on one tile (cta_group::2), holds 128 rows of X each and TN rows of Y:
 //   warp 0      streams operand tiles with TMA (128-byte swizzle) into a ring of stages
@@ -670,23 +671,26 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     float xs[4];                                         // of this lane's four rows
 #pragma unroll
                     for (int i = 0; i < 4; ++i) xs[i] = slot[q * 32 + 8 * i + (lane >> 2)];
-                    auto add = [&](const uint32_t (&v)[8], int j) {
-                        const float2 two = ys[4 * j];
+                    // the scales' product first: it is in range, a sum times one of them may not be
+                    auto add = [&](const uint32_t (&v)[8], int j, const float2& two) {
                         const uint64_t y = pair(two.x, two.y);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const uint64_t x = static_cast<uint64_t>(v[2 * i + 1]) << 32 | v[2 * i];
-                            frag[j][i] = fma2(mul2(x, y), pair(xs[i], xs[i]), frag[j][i]);
+                            frag[j][i] = fma2(x, mul2(y, pair(xs[i], xs[i])), frag[j][i]);
                         }
                     };
                     uint32_t v[2][8];                                    // eight columns on their way while eight are added
                     tc_ld8_frag(src, v[0]);
+                    float2 two = ys[0];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
+                        const float2 now = two;
+                        if (j < 7) two = ys[4 * (j + 1)];
                         tc_wait8(v[j & 1]);
                         if (j < 7) tc_ld8_frag(src + 8 * (j + 1), v[(j + 1) & 1]);
                         else release();
-                        add(v[j & 1], j);
+                        add(v[j & 1], j, now);
                     }
                 } else {
                     if (mine <= 0) release();
@@ -702,7 +706,7 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                             const float4 y = *reinterpret_cast<const float4*>(slot + C::XS + col0 + c + i);
                             const float ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[c + i + k] = fmaf(__uint_as_float(va[i + k]) * ys[k], s, acc[c + i + k]);
+                            for (int k = 0; k < 4; ++k) acc[c + i + k] = fmaf(__uint_as_float(va[i + k]), ys[k] * s, acc[c + i + k]);
                         }
                     }
                 }

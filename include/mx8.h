@@ -310,7 +310,7 @@ MX8_API int mx8_quantize_block128(const void* x, int dtype, int E, int M, int N,
 /* C[M][N] = dequant(A) . dequant(B)^T on block-128 operands, fp32 sums.  A [M][K] with row blocks: A_sc [ceil(K/128)][M], `ldsa` floats
  * between K blocks.  B [N][K]: squares (b_square != 0, B_sc [ceil(N/128)][ceil(K/128)]) or row blocks (B_sc [ceil(K/128)][N], pitch
  * ldsb).  lda, ldb: bytes between rows, multiples of 16 (K need not be one); C bf16 or float, `ldc` elements between rows.  The product
- * of two scales has to lie within the range of fp32.
+ * of two scales, which every form takes first, has to lie within the range of fp32; either alone may be as large or small as fp32 allows.
  * num_groups > 0: the rows of A are those of num_groups groups back to back, group_rows[g] of them (device int32, any size >= 0),
  * B [num_groups][N][K] with squares [num_groups][ceil(N/128)][ceil(K/128)]; rows of C behind the last group are left alone.  Sizes
  * that do not fit M are cut and set the device status word.  At most 256 groups; M, K and the rows of B at most 2^31 - 4096. */

@@ -611,3 +611,34 @@ def test_moe_layer_forward_and_backward_from_the_router_to_the_weight_gradients(
             assert (d_down[e] == 0).all()
         at += m
     assert mx8.device_status() == 0
+
+
+@pytest.mark.parametrize("shape,b", [((2, 64, 256), "rows"), ((9, 3000, 2000), "rows"), ((100, 100, 256), "rows"), ((100, 100, 256), "square"), ((100, 100, 2048), "rows"),
+                                     ((100, 100, 2048), "square"), ((1500, 1700, 256), "rows"), ((1500, 1700, 256), "square")])
+def test_scales_whose_product_alone_is_in_range(shape, b):
+    """one scale far above 1 and the other far below: their product is taken first in every form, so that no block's sum overflows or
+    loses bits on the way.  Sums of 448 * 448 are exact in fp32 up to the 24 bits of 49 * K, and every block adds two roundings."""
+    M, N, K = shape
+    a = torch.full((M, 16 * ((K + 15) // 16)), 448.0, device=DEV).to(torch.float8_e4m3fn)[:, :K]
+    w = torch.full((N, a.stride(0)), 448.0, device=DEV).to(torch.float8_e4m3fn)[:, :K]
+    for sx, sy in ((1e-30, 1e33), (1e33, 1e-30), (1e37, 1e-37), (1e-37, 1e37), (1e-36, 1e2)):
+        sa = torch.full((cdiv(K), M), sx, device=DEV)
+        sb = torch.full((cdiv(K), N) if b == "rows" else (cdiv(N), cdiv(K)), sy, device=DEV)
+        c = torch.empty(M, N, device=DEV)
+        mx8.gemm_block128(a, sa, w, sb, c, b_blocks=b)
+        want = K * 448.0 ** 2 * float(sa[0, 0].double() * sb[0, 0].double())
+        assert ((c.double() / want - 1).abs() <= (2 * cdiv(K) + 1) * 2.0 ** -24).all(), (sx, sy)
+
+
+def test_scales_whose_product_alone_is_in_range_in_weight_gradients():
+    for M, N, R in ((100, 100, 256), (600, 1701, 1280)):
+        a, w = (torch.full((rows, R), 448.0, device=DEV).to(torch.float8_e4m3fn) for rows in (M, N))
+        grp = torch.tensor([128, 0, R - 128], dtype=torch.int32, device=DEV)
+        for sx, sy in ((1e-30, 1e33), (1e33, 1e-30), (1e37, 1e-37)):
+            sa, sb = torch.full((R // 128, M), sx, device=DEV), torch.full((R // 128, N), sy, device=DEV)
+            c = torch.empty(3, M, N, device=DEV)
+            mx8.gemm_block128_wgrad(a, sa, w, sb, c, grp)
+            one = 448.0 ** 2 * float(sa[0, 0].double() * sb[0, 0].double())
+            assert (c[1] == 0).all()
+            for g, rows in ((0, 128), (2, R - 128)):
+                assert ((c[g].double() / (rows * one) - 1).abs() <= (rows // 64 + 1) * 2.0 ** -24).all()
