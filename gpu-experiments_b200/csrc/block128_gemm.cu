@@ -40,8 +40,8 @@ namespace g128 {
 
 constexpr int BK = 128;                       // bytes and elements of K per stage: one scale block
 constexpr int MAX_GROUPS = 256;
-constexpr int DEV_BAD_GROUPS = 17;            // device status: group sizes that do not fit the operands
-constexpr int DEV_SMEM_BASE = 18;             // device status: dynamic shared memory does not start on a 1024-byte boundary
+constexpr int DEV_BAD_GROUPS = MX8_DEV_INPUT_GROUPS;      // device status: group sizes that do not fit the operands
+constexpr int DEV_SMEM_BASE = MX8_DEV_SMEM_BASE;          // device status: dynamic shared memory does not start on a 1024-byte boundary
 constexpr int EPI0 = 4;                       // the first promoting warp
 
 // ROW: Y's scale is one number per 128 columns.  BOTH: it varies by column.

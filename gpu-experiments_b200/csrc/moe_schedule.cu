@@ -29,7 +29,7 @@ namespace moe {
 
 constexpr int PAD = 256;
 constexpr int THREADS = 1024;
-constexpr int DEV_MOE_CAPACITY = 16;   // device status: schedule does not fit `capacity`
+constexpr int DEV_MOE_CAPACITY = MX8_DEV_INPUT_CAPACITY;   // device status: schedule does not fit `capacity`
 
 struct SchedParams {
     const int* topk;        // [world][tokens][topk]

@@ -9,7 +9,7 @@
 
 namespace mx8 {
 
-// Device-side status codes recorded when a bounded wait gives up (0 = healthy).
+// Device-side status codes recorded when a bounded wait gives up (0 = healthy): MX8_DEV_* of include/mx8.h, which lists the others too.
 enum : int {
     DEV_OK = 0,
     DEV_TIMEOUT_FULL = 1,      // consumer waited for a TMA-filled stage

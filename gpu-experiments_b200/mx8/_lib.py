@@ -10,6 +10,10 @@ OK, ERR_ARG, ERR_SHAPE, ERR_ALIGN, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE_TIMEOUT
 SCALE_RCEIL, SCALE_FLOOR = 0, 1
 C_BF16, C_F32, C_MXFP8 = 0, 1, 2
 T_BF16, T_F32 = 0, 1
+# the device status word (MX8_DEV_* of include/mx8.h)
+DEV_WORDS = {1: "a wait for operands expired", 2: "a wait for room in shared memory expired", 3: "a wait for an accumulator expired",
+             4: "a wait for an accumulator's readers expired", 8: "the self-test's wait expired", 16: "a schedule does not fit its capacity",
+             17: "group sizes do not fit the operands", 18: "shared memory does not start on a 1024-byte boundary"}
 
 # every symbol include/mx8.h declares, with its ctypes signature
 _vp, _i = ctypes.c_void_p, ctypes.c_int

@@ -221,13 +221,15 @@ def kernel_transpose(A, A_fp8, A_sc):
 
 def device_status():
     """Synchronize the current stream and return the device status word (0 = healthy); raises
-    Mx8Error if a kernel's bounded wait expired."""
+    Mx8Error if a kernel's bounded wait expired or an input on the device did not fit.  The error's `word` is the word."""
     import ctypes
     lib = _lib.load()
     v = ctypes.c_int(0)
     rc = lib.mx8_device_status(ctypes.byref(v), _stream())
     if rc != _lib.OK:
-        raise Mx8Error(rc, f"device_status (device word = {v.value})")
+        err = Mx8Error(rc, f"device_status (device word = {v.value}: {_lib.DEV_WORDS.get(v.value, 'unknown')})")
+        err.word = v.value
+        raise err
     return v.value
 
 

@@ -41,9 +41,21 @@ enum {
     MX8_ERR_ALIGN = 3,          /* a pointer is not 16-byte aligned                         */
     MX8_ERR_CUDA = 4,           /* a CUDA runtime / driver call failed (mx8_last_cuda_error) */
     MX8_ERR_UNSUPPORTED = 5,    /* device is not compute capability 10.x                    */
-    MX8_ERR_DEVICE_TIMEOUT = 6, /* a kernel's bounded wait expired (mx8_device_status)      */
+    MX8_ERR_DEVICE_TIMEOUT = 6, /* a kernel recorded a failure: a bounded wait expired, or an input did not fit (mx8_device_status) */
     MX8_ERR_LIMIT = 7,          /* problem exceeds a built-in size limit (mx8_last_cuda_error has the text) */
     MX8_ERR_SIZE = 8            /* sizes or pitches do not fit the call (mx8_last_cuda_error has the text) */
+};
+
+/* what mx8_device_status can find in the device status word (0 = healthy) */
+enum {
+    MX8_DEV_TIMEOUT_FULL = 1,      /* a bounded wait expired: for operands on their way to shared memory     */
+    MX8_DEV_TIMEOUT_EMPTY = 2,     /* ... for room in shared memory                                           */
+    MX8_DEV_TIMEOUT_TMEM_FULL = 3, /* ... for a finished accumulator                                          */
+    MX8_DEV_TIMEOUT_TMEM_FREE = 4, /* ... for an accumulator to be read out                                   */
+    MX8_DEV_TIMEOUT_SELFTEST = 8,  /* ... in mx8_selftest_bounded_wait, on purpose                            */
+    MX8_DEV_INPUT_CAPACITY = 16,   /* input: a schedule does not fit its capacity (mx8_moe_schedule)          */
+    MX8_DEV_INPUT_GROUPS = 17,     /* input: group sizes do not fit the operands (mx8_gemm_block128, _wgrad)  */
+    MX8_DEV_SMEM_BASE = 18         /* a kernel's shared memory does not start on a 1024-byte boundary; C was not written */
 };
 
 /* scale rounding */
@@ -218,7 +230,7 @@ MX8_API int mx8_moe_bwd_epilogue_ids(const void* d_x_shared, const void* d_x_rou
  * overwritten: with mx8_moe_schedule_scratch_bytes(...) bytes the schedule is a counting sort that reads
  * the routing table twice; with at least num_local_experts*(world+1) ints it still works, scanning the
  * table once per local expert; less is MX8_ERR_LIMIT.  capacity is a multiple of 256; a schedule that
- * does not fit sets the device status word (mx8_device_status) instead of trapping.
+ * does not fit sets the device status word (MX8_DEV_INPUT_CAPACITY, mx8_device_status) instead of trapping.
  * Replaces scheduler::schedule, blackwell-ultra/022-moe-dispatch-mlp-swiglu-combine-mxfp8-bw.cu:149-183. */
 MX8_API size_t mx8_moe_schedule_scratch_bytes(int world, int tokens, int topk, int num_local_experts);
 MX8_API int mx8_moe_schedule(const void* topk_all, int world, int tokens, int topk, int num_local_experts,
@@ -313,14 +325,14 @@ MX8_API int mx8_quantize_block128(const void* x, int dtype, int E, int M, int N,
  * of two scales, which every form takes first, has to lie within the range of fp32; either alone may be as large or small as fp32 allows.
  * num_groups > 0: the rows of A are those of num_groups groups back to back, group_rows[g] of them (device int32, any size >= 0),
  * B [num_groups][N][K] with squares [num_groups][ceil(N/128)][ceil(K/128)]; rows of C behind the last group are left alone.  Sizes
- * that do not fit M are cut and set the device status word.  At most 256 groups; M, K and the rows of B at most 2^31 - 4096. */
+ * that do not fit M are cut and set the device status word (MX8_DEV_INPUT_GROUPS).  At most 256 groups; M, K and the rows of B at most 2^31 - 4096. */
 MX8_API int mx8_gemm_block128(const void* A, long long lda, const void* A_sc, long long ldsa, const void* B, long long ldb,
                               const void* B_sc, long long ldsb, int b_square, void* C, long long ldc, int M, int N, int K, int c_dtype,
                               const void* group_rows, int num_groups, void* stream);
 
 /* Weight gradients on block-128 operands: for every group g, C_g [M][N] = dequant(A_t[:, rows_g]) . dequant(B_t[:, rows_g])^T, A_t [M][rows]
  * and B_t [N][rows] with row blocks along `rows` (the transposed outputs of mx8_quantize_block128), rows_g the consecutive
- * group_rows[g] columns of group g (device int32, multiples of 128; others are cut and set the device status word).  A group without
+ * group_rows[g] columns of group g (device int32, multiples of 128; others are cut and set the device status word to MX8_DEV_INPUT_GROUPS).  A group without
  * rows yields zeros.  C is [num_groups][M][ldc]. */
 MX8_API int mx8_gemm_block128_wgrad(const void* A_t, long long lda, const void* A_t_sc, long long ldsa, const void* B_t, long long ldb,
                                     const void* B_t_sc, long long ldsb, void* C, long long ldc, int M, int N, int rows, int c_dtype,
@@ -511,9 +523,10 @@ MX8_API int mx8_probe_mma_peak(int k_steps, double* flops_out, void* stream);
  * stays usable.  The reference's waits are unbounded (blackwell-ultra/022-…-mxfp8-bw.cu:703-711); no counterpart. */
 MX8_API int mx8_selftest_bounded_wait(unsigned limit_us, void* stream);
 
-/* Synchronizes `stream`, then reads and clears the current device's status word: 0 = healthy,
- * otherwise the code of the first bounded wait that expired (see csrc/mx8_ptx.cuh).
- * Returns MX8_OK, MX8_ERR_DEVICE_TIMEOUT (status != 0) or MX8_ERR_CUDA. */
+/* Synchronizes `stream`, then reads and clears the current device's status word: 0 = healthy, otherwise the first
+ * failure that a kernel recorded since the last call, one of MX8_DEV_*: below 16 a bounded wait that expired, 16 and 17 an
+ * input on the device that did not fit and was cut.
+ * Returns MX8_OK, MX8_ERR_DEVICE_TIMEOUT (status != 0, whichever it is) or MX8_ERR_CUDA. */
 MX8_API int mx8_device_status(int* status_out, void* stream);
 
 MX8_API const char* mx8_strerror(int code);

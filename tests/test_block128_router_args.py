@@ -107,3 +107,12 @@ def test_bwd_epilogue_with_ids_arguments(lib):
     assert f(None, None, P, P, 1, 8, 1, None) == _lib.ERR_ARG and f(None, P, P, None, 1, 8, 1, None) == _lib.ERR_ARG
     assert f(None, P, P, P, 0, 8, 1, None) == _lib.ERR_ARG and f(None, P, P, P, 1, 12, 1, None) == _lib.ERR_SHAPE
     assert f(None, P, ODD, P, 1, 8, 1, None) == _lib.ERR_ALIGN and f(ODD, P, None, P, 1, 8, 1, None) == _lib.ERR_ALIGN
+
+
+def test_status_words_of_the_header_have_names(lib):
+    import os
+    import re
+    hdr = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "mx8.h")).read()
+    words = {int(v) for v in re.findall(r"MX8_DEV_\w+\s*=\s*(\d+)", hdr)}
+    assert words == set(_lib.DEV_WORDS) and {16, 17} <= words
+    assert b"did not fit" in lib.mx8_strerror(_lib.ERR_DEVICE_TIMEOUT) and b"wait expired" in lib.mx8_strerror(_lib.ERR_DEVICE_TIMEOUT)

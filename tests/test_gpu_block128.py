@@ -642,3 +642,24 @@ def test_scales_whose_product_alone_is_in_range_in_weight_gradients():
             assert (c[1] == 0).all()
             for g, rows in ((0, 128), (2, R - 128)):
                 assert ((c[g].double() / (rows * one) - 1).abs() <= (rows // 64 + 1) * 2.0 ** -24).all()
+
+
+def test_sizes_that_do_not_fit_are_named_by_the_status():
+    import ctypes
+    lib = mx8.load()
+    qa, sa, _, _ = mx8.quantize_block128(make_x(100, 256))
+    qb, sb, _, _ = mx8.quantize_block128(make_x(3, 64, 256), square=True)
+    bad = torch.tensor([50, 60, 10], dtype=torch.int32, device=DEV)
+    for _ in range(2):                                             # reported once, then healthy again
+        mx8.gemm_block128(qa, sa, qb, sb, torch.empty(100, 64, device=DEV), group_rows=bad)
+        with pytest.raises(mx8.Mx8Error, match="group sizes do not fit") as e:
+            mx8.device_status()
+        assert e.value.word == 17 and "an input on the device did not fit" in str(e.value)
+        assert mx8.device_status() == 0
+    word = ctypes.c_int(0)
+    mx8.gemm_block128(qa[:6], sa[:, :6], qb, sb, torch.empty(6, 64, device=DEV), group_rows=bad)       # single tokens
+    assert lib.mx8_device_status(ctypes.byref(word), torch.cuda.current_stream().cuda_stream) == 6 and word.value == 17
+    with pytest.raises(mx8.Mx8Error, match="does not fit its capacity") as e:
+        mx8.schedule(torch.zeros(1, 300, 1, dtype=torch.int32, device=DEV), 1, 256, 0)
+        mx8.device_status()
+    assert e.value.word == 16
