@@ -663,3 +663,141 @@ def test_sizes_that_do_not_fit_are_named_by_the_status():
         mx8.schedule(torch.zeros(1, 300, 1, dtype=torch.int32, device=DEV), 1, 256, 0)
         mx8.device_status()
     assert e.value.word == 16
+
+
+# ------------------------------------------------------------------------------------------------ C of large tiles
+# More 128 x 64 tiles than twice the device's multiprocessors, which large tiles compute: shapes below are checked for it.
+def needs_large_tiles(M, N, groups=0):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    small = cdiv(N) * (M // 64 + groups if groups else (M + 63) // 64)
+    assert M > 64 and small > 2 * sms
+    return M, N
+
+
+def inside(rows, cols, dtype, before=(1, 3), after=(2, 4)):
+    """a slice with guards on its four sides, rows off 16-byte boundaries; and the check that the guards are as they were"""
+    store = torch.full((before[0] + rows + after[0], before[1] + cols + after[1]), 6.0, dtype=dtype, device=DEV)
+    c = store[before[0]:before[0] + rows, before[1]:before[1] + cols]
+
+    def untouched():
+        c.fill_(6.0)
+        return bool((store == 6.0).all())
+    return c, untouched
+
+
+@pytest.mark.parametrize("b", ["square", "rows"])
+@pytest.mark.parametrize("shape", [(1500, 1700, 700), (1300, 2049, 260), (2050, 1153, 130)])
+def test_product_on_large_tiles_stays_inside_a_slice(shape, b):
+    M, N = needs_large_tiles(*shape[:2])
+    qa, sa, qb, sb, a64, b64 = operands(*shape, b, seed=M)
+    for dtype in (torch.bfloat16, torch.float32):
+        for before, after in (((1, 3), (2, 4)), ((0, 8), (1, 8 - N % 8)), ((3, 2), (1, 2))):       # odd, 16-byte and 4-byte rows
+            c, untouched = inside(M, N, dtype, before, after)
+            mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks=b)
+            assert mx8.device_status() == 0
+            check_c(c, a64, b64, f"{shape} {b} {dtype} {before}")
+            assert untouched()
+
+
+@pytest.mark.parametrize("sizes", [[700, 3, 0, 129, 256, 128, 40], [1500, 1300]])
+def test_grouped_product_on_large_tiles_stays_inside_a_slice(sizes):
+    G, cap, K = len(sizes), sum(sizes) + 37, 272
+    N = needs_large_tiles(cap, 2100, G)[1]
+    qa, sa, _, _ = mx8.quantize_block128(make_x(cap, K, seed=cap))
+    qb, sb, _, _ = mx8.quantize_block128(make_x(G, N, K, seed=G, dtype=torch.float32) * 0.02, square=True)
+    for dtype in (torch.bfloat16, torch.float32):
+        c, untouched = inside(cap, N, dtype)
+        mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=torch.tensor(sizes, dtype=torch.int32, device=DEV))
+        assert mx8.device_status() == 0
+        a64, at = rows64(qa, sa), 0
+        for g, n in enumerate(sizes):
+            if n:
+                check_c(c[at:at + n], a64[at:at + n], square64(qb[g], sb[g]), f"group {g}")
+            at += n
+        assert (c[at:] == 6.0).all() and untouched()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sizes,mn", [([1280, 0, 128, 1024], (600, 1701)), ([256] * 3, (1030, 1153))])
+def test_weight_gradient_on_large_tiles_stays_inside_a_slice(sizes, mn, dtype):
+    G, R, (M, N) = len(sizes), sum(sizes), mn
+    needs_large_tiles(M * G, N)
+    _, _, qa, sa = mx8.quantize_block128(make_x(R, M, seed=R, dtype=torch.float32), False, True)
+    _, _, qb, sb = mx8.quantize_block128(make_x(R, N, seed=R + 1), False, True)
+    flat, untouched = inside(G * M, N, dtype)
+    c = flat.as_strided((G, M, N), (M * flat.stride(0), flat.stride(0), 1))
+    mx8.gemm_block128_wgrad(qa, sa, qb, sb, c, torch.tensor(sizes, dtype=torch.int32, device=DEV))
+    assert mx8.device_status() == 0
+    a64, b64, at = rows64(qa, sa), rows64(qb, sb), 0
+    for g, n in enumerate(sizes):
+        if n:
+            check_c(c[g], a64[:, at:at + n], b64[:, at:at + n], f"group {g}")
+        else:
+            assert (c[g] == 0).all()
+        at += n
+    assert untouched()
+
+
+@pytest.mark.parametrize("b", ["square", "rows"])
+def test_non_finite_scales_on_large_tiles_reach_their_rows_only(b):
+    M, N = needs_large_tiles(1500, 1700)
+    for bad in (float("nan"), float("inf")):
+        qa, sa, qb, sb, a64, b64 = operands(M, N, 384, b, seed=4)
+        sa[1, 7] = sa[2, 1499] = bad
+        rows, cols = torch.arange(M), torch.arange(N)
+        if b == "rows":
+            sb[0, 1000] = bad
+            gone = cols == 1000
+        else:
+            sb[13, 2] = bad                                        # columns 1664 to 1699
+            gone = cols >= 1664
+        hit = (rows == 7) | (rows == 1499)
+        c = torch.empty(M, N, device=DEV)
+        mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks=b)
+        assert not torch.isfinite(c[hit.to(DEV)]).any() and not torch.isfinite(c[:, gone.to(DEV)]).any()
+        check_c(c[(~hit).to(DEV)][:, (~gone).to(DEV)], a64[~hit], b64[~gone])
+
+
+@pytest.mark.parametrize("form", ["square", "rows", "grouped"])
+def test_large_tiles_beyond_32_bits(form):
+    """C that spans more than 2^32 elements: every row where it should be, nothing between"""
+    M, N, K = 65 if form != "grouped" else 130, 19100, 260
+    needs_large_tiles(M, N, 2 if form == "grouped" else 0)
+    pitch = 2 ** 32 // (M - 1) + 7
+    b = "rows" if form == "rows" else "square"
+    if form == "grouped":
+        qa, sa, _, _ = mx8.quantize_block128(make_x(M, K, seed=3))
+        qb, sb, _, _ = mx8.quantize_block128(make_x(2, N, K, seed=5, dtype=torch.float32) * 0.02, square=True)
+    else:
+        qa, sa, qb, sb, a64, b64 = operands(M, N, K, b, seed=M)
+    store = torch.full((M * pitch,), 2.0, dtype=torch.bfloat16, device=DEV)
+    c = store.as_strided((M, N), (pitch, 1))
+    if form == "grouped":
+        mx8.gemm_block128(qa, sa, qb, sb, c, group_rows=torch.tensor([40, 90], dtype=torch.int32, device=DEV))
+        a64 = rows64(qa, sa)
+        check_c(c[:40], a64[:40], square64(qb[0], sb[0]))
+        check_c(c[40:], a64[40:], square64(qb[1], sb[1]))
+    else:
+        mx8.gemm_block128(qa, sa, qb, sb, c, b_blocks=b)
+        check_c(c, a64, b64)
+    assert mx8.device_status() == 0
+    c.fill_(2.0)
+    assert all(bool((part == 2.0).all()) for part in store.split(2 ** 28))
+
+
+def test_weight_gradients_beyond_32_bits():
+    """more than 2^32 elements of C over the groups' matrices, most of them between the rows"""
+    M, N, G = 300, 2200, 4
+    needs_large_tiles(M * G, N)
+    pitch = 2 ** 32 // (M * G - 1) + 5
+    _, _, qa, sa = mx8.quantize_block128(make_x(128 * G, M, seed=1, dtype=torch.float32), False, True)
+    _, _, qb, sb = mx8.quantize_block128(make_x(128 * G, N, seed=2), False, True)
+    store = torch.full((M * G * pitch,), 2.0, dtype=torch.bfloat16, device=DEV)
+    c = store.as_strided((G, M, N), (M * pitch, pitch, 1))
+    mx8.gemm_block128_wgrad(qa, sa, qb, sb, c, torch.full((G,), 128, dtype=torch.int32, device=DEV))
+    assert mx8.device_status() == 0
+    a64, b64 = rows64(qa, sa), rows64(qb, sb)
+    for g in range(G):
+        check_c(c[g], a64[:, 128 * g:128 * g + 128], b64[:, 128 * g:128 * g + 128], f"group {g}")
+    c.fill_(2.0)
+    assert all(bool((part == 2.0).all()) for part in store.split(2 ** 28))
