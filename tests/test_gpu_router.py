@@ -479,3 +479,65 @@ def test_backward_of_shifted_logits(shape, shift):
         # the sum that is subtracted is off by its E / 32 + 5 additions and two products, every gradient by three roundings, 1 / sum by one,
         # all of 2^-24 and of terms that add up to at most twice `size`
         assert (got.sum(1, keepdim=True).abs() <= (E / 32 + 16) * 2.0 ** -23 * size).all()
+
+
+def test_mxfp8_layer_of_masked_tokens_needs_no_cleared_buffers():
+    """router, schedule, the MXFP8 layer forward and backward and both weighted sums on one rank: with buffers that held NaN or an earlier
+    step's values the outputs are those of cleared ones"""
+    from oracle import mx8_oracle as O
+    T, H, I, k, E = 256, 512, 256, 4, 6
+    g = torch.Generator().manual_seed(3)
+    l = torch.randn(T, E, generator=g)
+    l[5, 1:] = NEG
+    idx, w, _, counts, _, n, _ = mx8.router_topk(l.to(DEV), k, token_mask=torch.arange(T, device=DEV) < T - 30)
+    assert int(n) == T - 30 and int(counts.sum()) == (T - 30) * k - (k - 1)
+    cap = (T * k // 256 + E) * 256
+    make = lambda r, c, seed: torch.stack([O.make_input(r, c, seed=seed + e, std=c ** -0.5) for e in range(E)])  # noqa: E731
+    ws = [make(I, H, 100), make(I, H, 200), make(H, I, 300)]
+    fw = [tuple(t.to(DEV) for t in O.quantize_both(m)[:2]) for m in ws]
+    bw = [tuple(t.to(DEV) for t in O.quantize_both(m.transpose(1, 2).contiguous())[:2]) for m in ws]
+    x, d_out = O.make_input(T, H, seed=72).to(DEV), O.make_input(T, H, seed=73, std=H ** -0.5).to(DEV)
+    pr, pt, nt, tpe = mx8.schedule(idx[None].contiguous(), E, cap, 0)
+    assert int((pr >= 0).sum()) == int(counts.sum())
+
+    def step(fill, ids):
+        cb, d_xb = (torch.full((T * k, H), fill, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        f = mx8.dispatch_mlp_swiglu_combine_fwd(x, [x.data_ptr()], cb, [cb.data_ptr()], None, *fw[0], None, *fw[1], None, *fw[2], pr, pt, nt, tpe, k)
+        out = mx8.fwd_epilogue(None, cb, w)
+        d_cb = torch.full_like(cb, fill)
+        mx8.bwd_prologue(d_out, w, d_cb)
+        mx8.dispatch_mlp_swiglu_combine_bwd(None, d_cb, [d_cb.data_ptr()], d_xb, [d_xb.data_ptr()], None, *bw[0], None, *bw[1], None, *bw[2],
+                                            f[0], f[1], None, f[3], f[4], None, f[6], f[7], None, f[9], f[10], x, [x.data_ptr()], *fw[0], *fw[1],
+                                            pr, pt, nt, tpe, k)
+        res = out, mx8.bwd_epilogue_routed(None, d_xb, k, ids), mx8.bwd_topk_weights(d_out, cb, idx)
+        assert mx8.device_status() == 0
+        return res
+    want = step(0.0, None)
+    assert float(want[0].abs().sum()) > 0 and (want[0][T - 30:] == 0).all() and (want[1][T - 30:] == 0).all()
+    for fill in (0.0, 3.0, float("nan"), float("inf")):
+        for got, ref in zip(step(fill, idx), want):
+            assert torch.equal(got, ref)
+
+
+def test_outputs_are_ordinary_tensors():
+    """views of a shared allocation: autograd, in-place changes, copies and other streams treat them as any other"""
+    import copy
+    l = make_logits(9, 40, torch.float32, 2)
+    out = mx8.router_topk(l, 3)
+    held = [t.clone() for t in out]
+    w = out[1].requires_grad_(True)
+    (w * 2).sum().backward()
+    assert torch.equal(w.grad, torch.full_like(w, 2.0))
+    assert torch.equal(copy.deepcopy(out[3]), held[3])
+    out[3].zero_()
+    out[4].add_(1.0)
+    out[2].record_stream(torch.cuda.Stream())
+    for i in (0, 1, 2, 5, 6):
+        assert torch.equal(out[i], held[i])
+    assert (out[3] == 0).all() and torch.equal(out[4], held[4] + 1.0)
+    with pytest.raises(RuntimeError):                              # a saved tensor that was changed is noticed
+        v = out[2].requires_grad_(True)
+        y = v * v.detach()
+        z = (y.exp(), y)
+        z[0].mul_(2.0)
+        z[0].sum().backward()
