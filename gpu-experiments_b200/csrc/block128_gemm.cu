@@ -14,14 +14,16 @@
 // The promotion bounds the kernel: 128 x 256 values a CTA and block take 740 cycles, of which the reads of TMEM are 256, the FMAs 256 and
 // the rest one probe of a barrier and the latency of the first read; the MMAs take 512.  Under the power limit the clock falls to 1.5 GHz.
 // 8192^3 took 848 us with one CTA a tile and 8 promoting warps, 656 with pairs, 547 with 16 warps of 64 columns that hide one
-// another's waits, 487 with the scales on the accumulator's barrier (cuBLAS in bf16 on the same device: 690 us).
+// another's waits, 470 to 487 with the scales on the accumulator's barrier (cuBLAS in bf16 on the same device: 665 to 690 us).  These are
+// launches from idle; among other work, under the power limit, it takes 550 to 565 us.
 //
 // X is the operand whose rows are the lanes of TMEM, Y the one whose rows are its columns: X = A, Y = B.  For few rows of A (SWAP)
 // X = B: the weights fill the lanes and a tile has as many columns (a multiple of 16) as there are rows of A.
 // Scales that vary by lane cost a register; scales that vary by column would have to reach every lane through shared memory, 128 bytes a
 // cycle, 1024 cycles a block, where a lane has one row.  Squares (one scale per 128 columns) do not need them (ROW).  Where both vary,
 // the fragment loads of TMEM give a lane 4 rows x 16 columns (FRAG): 256 cycles of shared memory, at half the rate of TMEM.  Weight
-// gradients 16384 x 2048 x 7168 in 8 groups, fp32: 490 us with two rows of 32 columns a lane, 385 us so; squares would lose (253 to 290 us).
+// gradients 16384 x 2048 x 7168 in 8 groups, fp32, from idle: 490 us with two rows of 32 columns a lane, 383 us so (435 us among other
+// work); squares would lose (253 to 290 us).
 // split > 1 (with SWAP): `split` CTAs of one cluster share a tile, each takes a part of the K blocks, sends the others their shares of the
 // tile by bulk copies from shared memory to shared memory, and adds up its own in rank order: no workspace, no atomics, the same result
 // in every run.  (Words one by one took 3 us read and 6 us sent for 64 rows.)  A 256 x 256 tile has four times the words to exchange:
@@ -671,7 +673,8 @@ gemm_block128_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_cons
                     float xs[4];                                         // of this lane's four rows
 #pragma unroll
                     for (int i = 0; i < 4; ++i) xs[i] = slot[q * 32 + 8 * i + (lane >> 2)];
-                    // the scales' product first: it is in range, a sum times one of them may not be
+                    // the scales' product first: it is in range, a sum times one of them may not be.  The columns' scales are read a step ahead (a
+                    // step's own after its wait: weight gradients 364 -> 376 us)
                     auto add = [&](const uint32_t (&v)[8], int j, const float2& two) {
                         const uint64_t y = pair(two.x, two.y);
 #pragma unroll
@@ -1119,8 +1122,9 @@ static int run(const Args& a, cudaStream_t st) {
         return split > 1 ? launch<FewSplit>(a, split, st) : launch<Few>(a, 1, st);
     }
     if (!a.b_square) return launch<Rows>(a, 1, st);
-    // Groups of fewer than 1024 rows on average: 128 rows a tile instead of the 256 of a pair, as half of a pair's last tile is empty
-    // more often than not.  The pair reads a third less from L2.  N = 2048, K = 7168, one CTA and pairs, us: 512 rows in 32 groups 87 and
+    // Groups of fewer than 1024 rows on average (of what A has room for, as the sizes are on the device): 128 rows a tile instead of the
+    // 256 of a pair, as half of a pair's last tile is empty more often than not when the sizes are any; measured with such sizes alone, none
+    // of them multiples of 256.  The pair reads a third less from L2.  N = 2048, K = 7168, one CTA and pairs, us: 512 rows in 32 groups 87 and
     // 132, 9001 rows 191 and 200, 16384 rows 325 and 346, 16384 rows in 8 groups 270 and 252.
     return grouped && a.M / a.groups < 1024 ? launch<Single>(a, 1, st) : launch<Squares>(a, 1, st);
 }
